@@ -43,6 +43,9 @@ extern "C" {
 #define EKV_STATUS_LEN_OVER_WIDTH 2u /* a length beyond width*block_size: clamped to the table width */
 #define EKV_STATUS_BAD_QROW 4u      /* a query token index outside [0, q_tokens): the row was skipped */
 #define EKV_STATUS_WAIT_TIMEOUT 8u  /* a bounded wait on a bulk copy gave up: the output is invalid  */
+#define EKV_STATUS_BAD_SLOT 16u     /* a score slot past the table, or two rows': the row's scores are left */
+#define EKV_STATUS_BLOCK_SHARED 32u /* a block to be written is another row's too: the row is left as it was */
+#define EKV_STATUS_BAD_LIST 64u     /* a list of kept tokens does not ascend within its row: the row is left */
 
 /* ---- ranking policies of the view builder (observe/allocation.py:79-118, daemon.py:49) --------- */
 #define EKV_POLICY_SUM 0     /* highest share first; equal shares: the newer block first           */
@@ -458,6 +461,103 @@ int ekv_compact_block_table(const int32_t* table, int64_t table_stride, const in
                             const uint8_t* keep, int64_t keep_stride, int rows, int width,
                             int block_size, int32_t* view, int64_t view_stride,
                             int32_t* view_lens, void* stream);
+
+/* Bytes of workspace ekv_attend needs (256-byte aligned; its contents never matter); 0 for bad sizes. */
+size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads, int kv_heads, int head_dim);
+
+/*
+ * ekv_attend -- attention over the paged cache, with prefixes that groups of rows share read once.
+ *
+ * No counterpart in the reference, which leaves the attention to its engine: the attention that reads a block
+ * table, or a view of it, as the audit kernel reads it.
+ *   q      [tokens][q_heads][head_dim], element strides q_stride_token/head;
+ *   kv     [pool_blocks][2][block_size][kv_heads][head_dim] (keys, then values), element strides;
+ *   table  int32 [rows][width] block table (row stride table_stride), lens int32 [rows]: the row's tokens in the
+ *          cache, those of its query included;
+ *   query_start  int32 [rows + 1]: row r's query tokens are [query_start[r], query_start[r + 1]); NULL: one token
+ *          a row (tokens == rows). Token i of a row's n sees the positions below lens[r] - n + i + 1.
+ * out [tokens][q_heads][head_dim] (element strides) receives softmax(scale q K^T) V and lse (may be NULL;
+ * float32 [tokens][q_heads]) the natural log of the sum of exp(scale q.k); a query token that sees nothing gets
+ * 0 and -inf. Tokens of no row keep what they have.
+ *
+ * groups > 0: the rows [group_start[g], group_start[g + 1]) (int32 [groups + 1]; NULL with groups = 1: every row)
+ * share their first prefix_blocks[g] blocks (int32 [groups]; NULL with groups = 1: prefix_common blocks): their
+ * tables list the same ids there, of which the longest row's are read, once for the group.
+ *
+ * A table entry outside [0, pool_blocks) is skipped with EKV_STATUS_BAD_BLOCK_ID, a length past the table
+ * clamped with EKV_STATUS_LEN_OVER_WIDTH, a row whose query tokens are not tokens of the batch skipped with
+ * EKV_STATUS_BAD_QROW. Supported: head_dim 64 and 128, block_size 8, 16, 32 and 64, rows <= 2048, scale > 0, base
+ * addresses and strides in whole 16-byte units. Two kernels (three with groups), no host synchronisation.
+ */
+int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
+               int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos, int64_t kv_stride_head,
+               int64_t pool_blocks, const int32_t* table, int64_t table_stride, const int32_t* lens,
+               const int32_t* query_start, int tokens, int rows, int width, int block_size, int q_heads,
+               int kv_heads, int head_dim, int dtype, float scale, int groups, const int32_t* group_start,
+               const int32_t* prefix_blocks, int prefix_common, void* out, int64_t out_stride_token,
+               int64_t out_stride_head, float* lse, void* workspace, size_t workspace_bytes, uint32_t* status,
+               void* stream);
+
+/*
+ * ekv_attend_scored -- ekv_attend (without prefixes) for rows whose cached tokens accumulate the attention
+ * weight they receive, the score ekv_select_tokens ranks them by.
+ *
+ * scores float32 [n_slots][kv_heads][>= width * block_size] (element strides); row r's are those of slot slots[r]
+ * (int32 [rows]; NULL: slot r). A token of the row at position t < lens[r] receives, per KV head, the weight
+ * w = sum of exp(scale q.k - lse) over the row's query tokens and the head's query heads: its score becomes w
+ * when t is among the row's newest fresh[r] tokens (int32 [rows]; NULL: its query tokens), which have none
+ * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends without scoring; a
+ * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Same workspace as ekv_attend
+ * with groups = 0. Three kernels, no host synchronisation.
+ */
+int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
+                      int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                      int64_t kv_stride_head, int64_t pool_blocks, const int32_t* table, int64_t table_stride,
+                      const int32_t* lens, const int32_t* query_start, int tokens, int rows, int width,
+                      int block_size, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                      float* scores, int64_t score_stride_slot, int64_t score_stride_head, int n_slots,
+                      const int32_t* slots, const int32_t* fresh, float decay, void* out,
+                      int64_t out_stride_token, int64_t out_stride_head, float* lse, void* workspace,
+                      size_t workspace_bytes, uint32_t* status, void* stream);
+
+/*
+ * ekv_select_tokens -- which tokens of each row and KV head to keep, by score.
+ *
+ * A row holds n = lens[r] tokens (at most capacity) and keeps k = keep[r] of them (int32 [rows]; NULL: keep_all).
+ * k < 0 or k >= n keeps the row whole. Otherwise its first first_tokens and newest recent_tokens are kept
+ * whatever they score, and of the others the best by score -- scores [n_slots][heads][>= capacity] float32, slots as
+ * in ekv_attend_scored; NaN ranks as -inf, equal scores to the older token -- up to k in all: new_lens[r] (int32
+ * [rows]) = max(k, min(n, first_tokens + recent_tokens)). kept int32 [rows][heads][>= capacity] receives the kept
+ * positions in ascending order, then -1 up to capacity. A row with no slot is kept whole. One kernel, no host
+ * synchronisation.
+ */
+int ekv_select_tokens(const float* scores, int64_t score_stride_slot, int64_t score_stride_head, int n_slots,
+                      int capacity, const int32_t* slots, const int32_t* lens, const int32_t* keep, int keep_all,
+                      int first_tokens, int recent_tokens, int rows, int heads, int32_t* kept,
+                      int64_t kept_stride_row, int64_t kept_stride_head, int32_t* new_lens, uint32_t* status,
+                      void* stream);
+
+/* Bytes of workspace ekv_compact_tokens needs (256-byte aligned; its contents never matter). */
+size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_t pool_blocks);
+
+/*
+ * ekv_compact_tokens -- the kept tokens of each row and KV head moved to the front of the row's blocks, in place.
+ *
+ * kv [pool_blocks][2][block_size][heads] rows of head_bytes bytes (strides in bytes, whole 16-byte units; any element type).
+ * In every row with 0 <= new_lens[r] < lens[r], position j < new_lens[r] of KV head h takes the key, the value and,
+ * with scores (as in ekv_attend_scored; may be NULL), the score of position kept[r][h][j] (int32, `columns` entries a
+ * list, ascending strictly, below lens[r]); what lies behind new_lens[r] stays as it was. The lists keep the first
+ * first_tokens positions in place, so blocks wholly among them may be shared between rows; every other block a
+ * moving row holds must be its own. A row whose lists, blocks or slot break this is left as it was, with
+ * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. One memset and two kernels, no host synchronisation.
+ */
+int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                       int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
+                       int64_t table_stride, const int32_t* lens, int rows, int width, int heads, int block_size,
+                       const int32_t* kept, int64_t kept_stride_row, int64_t kept_stride_head, int columns,
+                       const int32_t* new_lens, int first_tokens, float* scores, int64_t score_stride_slot,
+                       int64_t score_stride_head, int n_slots, const int32_t* slots, void* workspace,
+                       size_t workspace_bytes, uint32_t* status, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -1,0 +1,757 @@
+// Attention over the paged cache, prefixes that groups of rows share read once: out = softmax(scale q K^T) V
+// and the log of each query's sum of exponentials.
+//
+// Mathematics. One pass over the keys: with x = scale log2(e) q.k, a running maximum m, sum
+// l = sum 2^(x - m) and output o = sum 2^(x - m) v; when m grows to m', l and o are multiplied by 2^(m - m').
+// Parts of a row (its group's prefix, its own tokens, tiles of different CTAs) join the same way, so a
+// shared prefix is one launch whose query rows are those of every row of the group, and the two results meet
+// in the combine kernel: out = sum_j 2^(m_j - m) o_j / sum_j 2^(m_j - m) l_j.
+//
+// attend_kernel. A CTA of four math warps and one copy warp walks its share of the launch's tiles
+// (attend.cuh). The copy warp reads block ids and asks the TMA engine for the tile's key and value rows of
+// one KV head, a block's 64-dim half per copy in the 128-byte swizzle, into a ring of stages. The math warps
+// stand WM along the query rows and WN along the tile's tokens: scores by mma.sync m16n8k16 with the query
+// fragments in registers for a whole item, probabilities rounded to the cache's type (the products' operands
+// have to be of one type) and multiplied with the values in the same registers; sums stay in float32 from the
+// unrounded probabilities. The WN warps join through shared memory at an item's end.
+#include "attend.cuh"
+
+namespace ekv {
+
+namespace {
+
+constexpr int kMathWarps = 4;
+constexpr int kThreads = (kMathWarps + 1) * 32;
+
+template <int D>
+struct Ring {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kPart = kHalves * kTile * 128;  // bytes of a tile's keys, or values
+  static constexpr int kStage = 2 * kPart;
+  static constexpr int kStages = 3;
+  static constexpr int kBytes = kStages * kStage;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// Bytes from a part's start to 16-byte chunk c of token t's row (128-byte swizzle, 64-dim halves).
+__device__ __forceinline__ uint32_t chunk_at(int t, int c) {
+  return (uint32_t)(c >> 3) * (kTile * 128) + (uint32_t)t * 128 + (uint32_t)((c & 7) ^ (t & 7)) * 16;
+}
+
+// The shared memory behind the ring.
+template <int D, int WM, int WN>
+struct Tail {
+  uint64_t full[Ring<D>::kStages], empty[Ring<D>::kStages];
+  uint32_t blocks[Ring<D>::kStages];  // which of the stage's blocks were copied (bit b: the tile's block b)
+  int scratch[kThreads / 32 + 1];
+  float m[WN > 1 ? WN : 1][16 * WM], l[WN > 1 ? WN : 1][16 * WM];
+  alignas(16) float o[WN > 1 ? WN / 2 : 1][16 * WM][WN > 1 ? D / 2 + 4 : 1];  // half the dims at a time
+};
+
+template <typename T, int D, int WM, int WN, bool PREFIX>
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ AttendParams p) {
+  using R = Ring<D>;
+  using TailT = Tail<D, WM, WN>;
+  constexpr int MT = 16 * WM;
+  constexpr int kWarpTokens = kTile / WN;  // tokens of the tile a warp works on
+  constexpr int kN = kWarpTokens / 8;      // its score fragments
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  TailT& tail = *reinterpret_cast<TailT*>(ring + R::kBytes);
+  const Plan plan = plan_at(ring + R::kBytes + (sizeof(TailT) + 15) / 16 * 16, PREFIX ? p.groups : p.rows, PREFIX);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < R::kStages; ++s) {
+      mbar_init(&tail.full[s], 1);
+      mbar_init(&tail.empty[s], kMathWarps);
+    }
+    fence_mbar_init();
+  }
+  chain_wait();  // the lengths, tables and caches may be the work of the launches before
+  make_plan<PREFIX, kThreads>(p, plan, MT, tail.scratch);
+  const int W = plan.cum[plan.units];
+  const int n = sharing_ctas(W, gridDim.x);
+  if (blockIdx.x == 0) {
+    for (int u = threadIdx.x; u <= plan.units; u += kThreads) p.cum[u] = plan.cum[u];
+    if (threadIdx.x == 0) p.cum[plan.units + 1] = n;
+  }
+  chain_release();
+  if ((int)blockIdx.x >= n || W == 0) return;
+  const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
+  const int per_tile = kTile >> p.block_shift;  // blocks of a tile
+
+  if (warp == kMathWarps) {  // ---- the copy warp ------------------------------------------------------
+    const uint64_t policy = l2_evict_first_policy();
+    const uint32_t block_bytes = (uint32_t)p.block_size * 128u;
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool good = true;
+    for (int t = begin; t < end && good;) {
+      const Item it = item_at<PREFIX>(p, plan, MT, t, end);
+      const int from = it.un.from, to = it.un.to;
+      const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
+      const int last_block = (to - 1) >> p.block_shift;
+      const int block0 = (from >> p.block_shift) + lane;
+      const bool mine = lane < per_tile;
+      int id = mine && block0 + it.first * per_tile <= last_block ? ids[block0 + it.first * per_tile] : -2;
+      for (int tile = it.first; tile < it.last && good; ++tile, ++t) {
+        const int b = block0 + tile * per_tile;
+        const int next = tile + 1 < it.last && mine && b + per_tile <= last_block ? ids[b + per_tile] : -2;
+        if (issued >= R::kStages) good = mbar_wait_bounded(&tail.empty[stage], phase ^ 1, p.status);
+        good = __all_sync(kFullMask, good);
+        if (!good) break;
+        const bool inside = mine && b <= last_block;
+        const bool ok = inside && id >= 0 && (int64_t)id < p.pool_blocks;
+        if (inside && !ok) set_status(p.status, EKV_STATUS_BAD_BLOCK_ID);
+        const uint32_t which = __ballot_sync(kFullMask, ok);
+        if (lane == 0) {
+          tail.blocks[stage] = which;
+          mbar_arrive_expect_tx(&tail.full[stage], (uint32_t)__popc(which) * block_bytes * 2 * R::kHalves);
+        }
+        __syncwarp();
+        if (ok) {
+          const uint32_t at = smem_u32(ring) + stage * R::kStage + lane * block_bytes;
+#pragma unroll
+          for (int h = 0; h < R::kHalves; ++h) {
+            tensor_copy_4d(at + h * (kTile * 128), &p.kmap, 64 * h, it.head, 0, id, &tail.full[stage], policy);
+            tensor_copy_4d(at + h * (kTile * 128) + R::kPart, &p.vmap, 64 * h, it.head, 0, id, &tail.full[stage], policy);
+          }
+        }
+        id = next;
+        ++issued;
+        if (++stage == R::kStages) stage = 0, phase ^= 1;
+      }
+    }
+    // no CTA leaves with copies in flight: the last phase of every stage that was used has to be complete
+    for (int s = 0; s < R::kStages; ++s) {
+      const int uses = issued > s ? (issued - s - 1) / R::kStages + 1 : 0;
+      if (uses > 0) mbar_wait_bounded(&tail.full[s], (uses - 1) & 1, p.status);
+    }
+    return;
+  }
+
+  // ---- the math warps ------------------------------------------------------------------------------------
+  const int wm = warp % WM, wn = warp / WM;
+  const int quad = lane >> 2, pair = lane & 3;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool good = true;
+  for (int t = begin; t < end;) {
+    const Item it = item_at<PREFIX>(p, plan, MT, t, end);
+    const QueryRange uq = it.un.q;
+    const int from = it.un.from, to = it.un.to;
+    const RowRange rows = PREFIX ? group_rows(p, it.unit) : RowRange{it.unit, it.unit + 1};
+    // this lane's two query rows: the tokens they see, and their fragments
+    uint32_t qf[D / 16][4];
+    int limit[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int mrow = it.mt * MT + wm * 16 + quad + 8 * j;
+      const int token = uq.q0 + mrow / p.G;
+      const bool real = mrow < uq.nq * p.G;
+      limit[j] = 0x7fffffff;
+      if (real) {
+        const int r = PREFIX ? row_of_token(p, rows, token) : it.unit;
+        limit[j] = r < 0 ? 0 : token_limit(p, r, token);
+      }
+      const T* src = static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 +
+                     (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 2 * pair;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][j] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+        qf[k][j + 2] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+      }
+    }
+    float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[d][j] = 0.f;
+
+    for (int tile = it.first; tile < it.last; ++tile, ++t) {
+      // after a wait that gave up the walk goes on without waiting, so that the warps' barriers stay paired
+      if (good) good = mbar_wait_bounded(&tail.full[stage], phase, p.status);
+      const uint32_t keys = smem_u32(ring) + stage * R::kStage, values = keys + R::kPart;
+      const uint32_t blocks = tail.blocks[stage];
+      const int pos0 = from + tile * kTile + wn * kWarpTokens;  // position of this warp's first token
+      float s[kN][4];
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+        for (int j = 0; j < kN; j += 2) {
+          uint32_t b[4];
+          ldmatrix_x4(b, keys + chunk_at(wn * kWarpTokens + 8 * j + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+          const uint32_t b0[2] = {b[0], b[1]}, b1[2] = {b[2], b[3]};
+          Mma<T>::run(s[j], qf[k], b0);
+          Mma<T>::run(s[j + 1], qf[k], b1);
+        }
+      }
+      const uint32_t all = per_tile == 32 ? ~0u : (1u << per_tile) - 1u;
+      const bool whole = blocks == all && pos0 + kWarpTokens <= to;
+      const bool seen = pos0 + kWarpTokens <= limit[0] && pos0 + kWarpTokens <= limit[1];
+      if (!whole) {
+        // rows of the stage that hold no token of the unit: their keys are masked below, their values cleared
+        // (a probability of zero times what lies there need not be zero)
+        for (int i = lane; i < kWarpTokens * (D / 8); i += 32) {
+          const int tk = wn * kWarpTokens + i / (D / 8);
+          if (from + tile * kTile + tk >= to || !((blocks >> (tk >> p.block_shift)) & 1u))
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + chunk_at(tk, i % (D / 8))), "r"(0)
+                         : "memory");
+        }
+        __syncwarp();
+      }
+      if (!__all_sync(kFullMask, whole && seen)) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tk = wn * kWarpTokens + 8 * j + 2 * pair + (e & 1);
+            const int pos = from + tile * kTile + tk;
+            if (pos >= to || pos >= limit[e >> 1] || !((blocks >> (tk >> p.block_shift)) & 1u)) s[j][e] = -INFINITY;
+          }
+      }
+      // the running maximum of each query row over this warp's tokens
+      float mx[2] = {s[0][0], s[0][2]};
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        mx[0] = fmaxf(mx[0], fmaxf(s[j][0], s[j][1]));
+        mx[1] = fmaxf(mx[1], fmaxf(s[j][2], s[j][3]));
+      }
+      float base[2];
+      bool grew = false;
+      float mn[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        mx[j] = fmaxf(mx[j], __shfl_xor_sync(kFullMask, mx[j], 1));
+        mx[j] = fmaxf(mx[j], __shfl_xor_sync(kFullMask, mx[j], 2));
+        mn[j] = fmaxf(m[j], mx[j] * p.scale_log2);
+        grew |= mn[j] > m[j];
+      }
+      if (__any_sync(kFullMask, grew)) {
+        float f[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          f[j] = mn[j] > m[j] ? exp2_fast(m[j] - mn[j]) : 1.f;  // 0 for a row's first keys
+          l[j] *= f[j];
+          m[j] = mn[j];
+        }
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) {
+          o[d][0] *= f[0];
+          o[d][1] *= f[0];
+          o[d][2] *= f[1];
+          o[d][3] *= f[1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) base[j] = m[j] == -INFINITY ? 0.f : m[j];
+      uint32_t pf[kN / 2][4];
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        const float a0 = exp2_fast(fmaf(s[j][0], p.scale_log2, -base[0]));
+        const float a1 = exp2_fast(fmaf(s[j][1], p.scale_log2, -base[0]));
+        const float a2 = exp2_fast(fmaf(s[j][2], p.scale_log2, -base[1]));
+        const float a3 = exp2_fast(fmaf(s[j][3], p.scale_log2, -base[1]));
+        l[0] += a0 + a1;
+        l[1] += a2 + a3;
+        pf[j / 2][(j & 1) * 2] = pack2<T>(a0, a1);
+        pf[j / 2][(j & 1) * 2 + 1] = pack2<T>(a2, a3);
+      }
+#pragma unroll
+      for (int k = 0; k < kN / 2; ++k) {
+#pragma unroll
+        for (int d = 0; d < D / 8; d += 2) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, values + chunk_at(wn * kWarpTokens + 16 * k + (lane & 15), d + (lane >> 4)));
+          const uint32_t b0[2] = {b[0], b[1]}, b1[2] = {b[2], b[3]};
+          Mma<T>::run(o[d], pf[k], b0);
+          Mma<T>::run(o[d + 1], pf[k], b1);
+        }
+      }
+      if (!whole) proxy_fence_smem();  // the cleared rows before the copy that refills the stage
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tail.empty[stage]);
+      if (++stage == R::kStages) stage = 0, phase ^= 1;
+    }
+
+    // ---- the item's end: the sums over the quad's lanes, then over the WN warps -----------------------------
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      l[j] += __shfl_xor_sync(kFullMask, l[j], 1);
+      l[j] += __shfl_xor_sync(kFullMask, l[j], 2);
+    }
+    if (WN > 1) {
+      if (pair == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          tail.m[wn][wm * 16 + quad + 8 * j] = m[j];
+          tail.l[wn][wm * 16 + quad + 8 * j] = l[j];
+        }
+      }
+      named_barrier(1, kMathWarps * 32);
+      float f[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = wm * 16 + quad + 8 * j;
+        float top = -INFINITY;
+        for (int w = 0; w < WN; ++w) top = fmaxf(top, tail.m[w][row]);
+        f[j] = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - top);
+        float sum = 0.f;
+        for (int w = 0; w < WN; ++w) sum += tail.m[w][row] == -INFINITY ? 0.f : tail.l[w][row] * exp2_fast(tail.m[w][row] - top);
+        m[j] = top;
+        l[j] = sum;
+      }
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) {
+        o[d][0] *= f[0];
+        o[d][1] *= f[0];
+        o[d][2] *= f[1];
+        o[d][3] *= f[1];
+      }
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+#pragma unroll
+        for (int half = WN / 2; half >= 1; half /= 2) {  // a tree, so the order of the additions is fixed
+          if (wn >= half && wn < 2 * half) {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              const float(&v)[4] = o[part * (D / 16) + d];
+              float* dst = &tail.o[wn - half][wm * 16 + quad][8 * d + 2 * pair];
+              *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+              *reinterpret_cast<float2*>(dst + 8 * (D / 2 + 4)) = make_float2(v[2], v[3]);
+            }
+          }
+          named_barrier(1, kMathWarps * 32);
+          if (wn < half) {
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              float(&v)[4] = o[part * (D / 16) + d];
+              const float* src = &tail.o[wn][wm * 16 + quad][8 * d + 2 * pair];
+              const float2 a = *reinterpret_cast<const float2*>(src);
+              const float2 b = *reinterpret_cast<const float2*>(src + 8 * (D / 2 + 4));
+              v[0] += a.x;
+              v[1] += a.y;
+              v[2] += b.x;
+              v[3] += b.y;
+            }
+          }
+          named_barrier(1, kMathWarps * 32);
+        }
+      }
+    }
+    if (wn == 0) {
+      const bool complete = it.first == 0 && it.last == it.tiles;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int mrow = it.mt * MT + wm * 16 + quad + 8 * j;
+        if (mrow >= uq.nq * p.G) continue;
+        const int token = uq.q0 + mrow / p.G, head = it.head * p.G + mrow % p.G;
+        if (complete && p.groups == 0) {
+          const float inv = l[j] > 0.f ? 1.f / l[j] : (l[j] == 0.f ? 0.f : l[j]);
+          T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)head * p.out_s1 + 2 * pair;
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d) {
+            const float x = l[j] == 0.f ? 0.f : o[d][2 * j] * inv, y = l[j] == 0.f ? 0.f : o[d][2 * j + 1] * inv;
+            *reinterpret_cast<uint32_t*>(dst + 8 * d) = pack2<T>(x, y);
+          }
+          if (p.lse != nullptr && pair == 0)
+            p.lse[(int64_t)token * p.q_heads + head] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * kLn2;
+        } else {
+          float *dst, *ml;
+          if (complete) {
+            const int64_t at = (int64_t)token * p.q_heads + head;
+            dst = p.whole + at * D;
+            ml = p.whole + (int64_t)p.tokens * p.q_heads * D + 2 * at;
+          } else {
+            const int64_t at = (int64_t)(2 * blockIdx.x + (it.first == 0 ? 1 : 0)) * MT + (mrow - it.mt * MT);
+            dst = p.parts + at * D;
+            ml = p.parts + (int64_t)2 * p.max_ctas * MT * D + 2 * at;
+          }
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d)
+            *reinterpret_cast<float2*>(dst + 8 * d + 2 * pair) = make_float2(o[d][2 * j], o[d][2 * j + 1]);
+          if (pair == 0) *reinterpret_cast<float2*>(ml) = make_float2(m[j], l[j]);
+        }
+      }
+    }
+  }
+}
+
+// ---- joining the parts ------------------------------------------------------------------------------------------
+
+// A phase's plan and parts, as its launch left them.
+struct PhaseOut {
+  const int32_t* cum;
+  const float* parts;
+  const float* whole;
+  int units, MT;
+};
+
+struct CombineParams {
+  AttendParams p;
+  PhaseOut own, prefix;
+};
+
+constexpr int kCombineThreads = 128;
+
+// The parts of one (query token, query head) in one phase: CTAs [c0, c1], or the one finished item (whole).
+struct PartList {
+  const float* o;   // part i: o + i * stride (the first one elsewhere: o_first)
+  const float* ml;
+  int count;
+  int64_t first, rest;  // index of the first part's row, and of the second's (the others follow 2 MT apart)
+  int64_t step;
+};
+
+__device__ __forceinline__ PartList list_parts(const AttendParams& p, const PhaseOut& ph, int unit, int nq, int m, int head,
+                                               int token, int qhead, int D) {
+  PartList out{nullptr, nullptr, 0, 0, 0, 0};
+  const int W = ph.cum[ph.units], n = ph.cum[ph.units + 1];
+  const int mts = (nq * p.G + ph.MT - 1) / ph.MT;
+  const int span = ph.cum[unit + 1] - ph.cum[unit];
+  if (span == 0 || mts == 0) return out;
+  const int tiles = span / (mts * p.heads), mt = m / ph.MT;
+  const int a = ph.cum[unit] + (head * mts + mt) * tiles, b = a + tiles;
+  const int c0 = cta_of(a, W, n), c1 = cta_of(b - 1, W, n);
+  if (c0 == c1) {
+    out.o = ph.whole;
+    out.ml = ph.whole + (int64_t)p.tokens * p.q_heads * D;
+    out.count = 1;
+    out.first = (int64_t)token * p.q_heads + qhead;
+    return out;
+  }
+  out.o = ph.parts;
+  out.ml = ph.parts + (int64_t)2 * p.max_ctas * ph.MT * D;
+  out.count = c1 - c0 + 1;
+  const int mi = m - mt * ph.MT;
+  out.first = (int64_t)(2 * c0 + 1) * ph.MT + mi;
+  out.rest = (int64_t)(2 * c0 + 2) * ph.MT + mi;
+  out.step = 2 * ph.MT;
+  return out;
+}
+
+__device__ __forceinline__ int64_t part_row(const PartList& l, int i) { return i == 0 ? l.first : l.rest + (i - 1) * l.step; }
+
+// A warp per (query token, query head); every lane holds D / 32 dims. The parts are added in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineParams c) {
+  const AttendParams& p = c.p;
+  chain_release();
+  chain_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
+  if (item >= (int64_t)p.tokens * p.q_heads) return;
+  const int token = (int)(item / p.q_heads), qhead = (int)(item - (int64_t)token * p.q_heads);
+  const int row = row_of_token(p, {0, p.rows}, token);
+  if (row < 0) return;  // a token of no row keeps its output
+  const QueryRange q = row_queries(p, row, false);
+  const int head = qhead / p.G, g = qhead - head * p.G;
+  PartList lists[2];
+  lists[0] = list_parts(p, c.own, row, q.nq, (token - q.q0) * p.G + g, head, token, qhead, D);
+  lists[1].count = 0;
+  const int group = group_of(p, row);
+  if (group >= 0) {
+    const QueryRange gq = group_queries(p, group_rows(p, group));
+    lists[1] = list_parts(p, c.prefix, group, gq.nq, (token - gq.q0) * p.G + g, head, token, qhead, D);
+  } else if (lists[0].count == 1 && p.groups == 0) {
+    return;  // the attention kernel wrote it
+  }
+  float m = -INFINITY;
+  for (int k = 0; k < 2; ++k)
+    for (int i = lane; i < lists[k].count; i += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], i)]);
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
+  float acc[D / 32], l = 0.f;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll 4
+    for (int i = 0; i < lists[k].count; ++i) {
+      const int64_t at = part_row(lists[k], i);
+      const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
+      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+      const float* o = lists[k].o + at * D + lane * (D / 32);
+      l += ml.x == -INFINITY ? 0.f : ml.y * f;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] = ml.x == -INFINITY ? acc[d] : fmaf(o[d], f, acc[d]);
+    }
+  }
+  const float inv = 1.f / l;
+  T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)qhead * p.out_s1 + lane * (D / 32);
+#pragma unroll
+  for (int d = 0; d < D / 32; d += 2)
+    *reinterpret_cast<uint32_t*>(dst + d) = l == 0.f ? 0u : pack2<T>(acc[d] * inv, acc[d + 1] * inv);
+  if (p.lse != nullptr && lane == 0) p.lse[item] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+
+struct Workspace {
+  size_t cum[2], parts[2], whole[2], total;
+};
+
+// Phase 0: the rows' own tokens; phase 1: the shared prefixes.
+Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, int ctas, const int (&mt)[2]) {
+  Workspace w{};
+  size_t at = 0;
+  for (int k = 0; k < (groups > 0 ? 2 : 1); ++k) {
+    w.cum[k] = at;
+    at += round_up(((size_t)(k == 0 ? rows : groups) + 2) * 4, 256);
+    w.parts[k] = at;
+    at += round_up((size_t)2 * ctas * mt[k] * (dim + 2) * 4, 256);
+    w.whole[k] = at;
+    if (groups > 0) at += round_up((size_t)tokens * q_heads * (dim + 2) * 4, 256);
+  }
+  w.total = at;
+  return w;
+}
+
+// Query rows of an M tile: the smallest variant that holds a unit's average in one tile.
+int pick_mt(int64_t tokens, int units, int G) {
+  const int64_t m = (tokens + units - 1) / units * G;
+  return m <= 16 ? 16 : m <= 32 ? 32 : 64;
+}
+
+template <typename T, int D, int WM, int WN, bool PREFIX>
+int launch_attend(const AttendParams& p, int sms, cudaStream_t s) {
+  const int units = PREFIX ? p.groups : p.rows;
+  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16 + plan_bytes(units, PREFIX);
+  auto kernel = attend_kernel<T, D, WM, WN, PREFIX>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return check_launch("cudaFuncSetAttribute(attend_kernel)");
+  int resident = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem) != cudaSuccess)
+    return check_launch("cudaOccupancyMaxActiveBlocksPerMultiprocessor(attend_kernel)");
+  if (resident < 1) return fail(EKV_ENOTSUP, "the attention kernel does not fit this device");
+  launch_chained(kernel, dim3(min(sms * resident, p.max_ctas)), dim3(kThreads), smem, s, p);
+  return check_launch("attend_kernel");
+}
+
+template <typename T, int D, bool PREFIX>
+int launch_phase(const AttendParams& p, int sms, cudaStream_t s) {
+  switch (p.mt_rows) {
+    case 16: return launch_attend<T, D, 1, 4, PREFIX>(p, sms, s);
+    case 32: return launch_attend<T, D, 2, 2, PREFIX>(p, sms, s);
+    default: return launch_attend<T, D, 4, 1, PREFIX>(p, sms, s);
+  }
+}
+
+template <typename T, int D>
+int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, int sms, cudaStream_t s) {
+  CombineParams c{};
+  const int phases = p.groups > 0 ? 2 : 1;
+  for (int k = phases - 1; k >= 0; --k) {  // the prefixes first
+    p.mt_rows = mt[k];
+    p.cum = reinterpret_cast<int32_t*>(ws + w.cum[k]);
+    p.parts = reinterpret_cast<float*>(ws + w.parts[k]);
+    p.whole = reinterpret_cast<float*>(ws + w.whole[k]);
+    (k == 0 ? c.own : c.prefix) = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k]};
+    const int rc = k == 1 ? launch_phase<T, D, true>(p, sms, s) : launch_phase<T, D, false>(p, sms, s);
+    if (rc != EKV_OK) return rc;
+  }
+  c.p = p;
+  const int64_t items = (int64_t)p.tokens * p.q_heads;
+  const int per = kCombineThreads / 32;
+  launch_chained(combine_kernel<T, D>, dim3((unsigned)((items + per - 1) / per)), dim3(kCombineThreads), 0, s, c);
+  return check_launch("combine_kernel");
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+}  // namespace
+
+int encode_cache_maps(AttendParams& p, const void* kv, int64_t s_block, int64_t s_part, int64_t s_pos, int64_t s_head,
+                      int dim, int dtype) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = map_encoder();
+  if (encode == nullptr) return fail(EKV_ECUDA, "the driver does not provide cuTensorMapEncodeTiled");
+  const cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)p.heads, (cuuint64_t)p.block_size, (cuuint64_t)p.pool_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_pos * 2, (cuuint64_t)s_block * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)p.block_size, 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  for (int part = 0; part < 2; ++part) {
+    const CUresult r = encode(part == 0 ? &p.kmap : &p.vmap,
+                              dtype == EKV_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                              const_cast<uint8_t*>(static_cast<const uint8_t*>(kv)) + part * s_part * 2, dims, strides, box,
+                              unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return fail(EKV_ENOTSUP, "the cache (strides %lld, %lld, %lld elements) has no tensor map (CUresult %d)",
+                  (long long)s_block, (long long)s_pos, (long long)s_head, (int)r);
+  }
+  return EKV_OK;
+}
+
+}  // namespace ekv
+
+using namespace ekv;
+
+namespace {
+
+struct AttendCall {
+  AttendParams p;
+  Workspace w;
+  int mt[2];
+  uint8_t* ws;
+  int sms;
+};
+
+// The checks of ekv_attend and ekv_attend_scored; fills the call.
+int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
+            int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos, int64_t kv_stride_head,
+            int64_t pool_blocks, const int32_t* table, int64_t table_stride, const int32_t* lens,
+            const int32_t* query_start, int tokens, int rows, int width, int block_size, int q_heads, int kv_heads,
+            int head_dim, int dtype, float scale, int groups, const int32_t* group_start, const int32_t* prefix_blocks,
+            int prefix_common, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse, void* workspace,
+            size_t workspace_bytes, uint32_t* status) {
+  if (!q || !kv || !table || !lens || !out) return fail(EKV_EINVAL, "a required device pointer is NULL");
+  if (rows <= 0 || tokens <= 0 || width <= 0 || pool_blocks <= 0)
+    return fail(EKV_EINVAL, "rows, tokens, width and pool_blocks must be positive");
+  if (rows > kAttendMaxRows) return fail(EKV_ENOTSUP, "%d rows: this build handles up to %d", rows, kAttendMaxRows);
+  if (!query_start && tokens != rows)
+    return fail(EKV_EINVAL, "%d query tokens for %d rows: without query_start every row has one", tokens, rows);
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads)
+    return fail(EKV_EINVAL, "%d query heads do not divide over %d KV heads", q_heads, kv_heads);
+  if (head_dim != 64 && head_dim != 128) return fail(EKV_ENOTSUP, "head_dim %d: this build has kernels for 64 and 128", head_dim);
+  if (block_size != 8 && block_size != 16 && block_size != 32 && block_size != 64)
+    return fail(EKV_ENOTSUP, "block_size %d: this build has kernels for 8, 16, 32 and 64", block_size);
+  if (dtype != EKV_DTYPE_F16 && dtype != EKV_DTYPE_BF16) return fail(EKV_EINVAL, "unknown dtype %d", dtype);
+  if (!(scale > 0.f) || scale > 3.4e38f) return fail(EKV_EINVAL, "the scale must be positive and finite");
+  if (pool_blocks > 0x7fffffffll) return fail(EKV_ENOTSUP, "%lld blocks in the pool exceed 2^31 - 1", (long long)pool_blocks);
+  if (table_stride < width) return fail(EKV_EINVAL, "the table's row stride is below the width");
+  if (((uintptr_t)kv & 15) || (kv_stride_block & 7) || (kv_stride_part & 7) || (kv_stride_pos & 7) || (kv_stride_head & 7))
+    return fail(EKV_EINVAL, "the cache must be 16-byte aligned with strides of whole 16-byte units");
+  if (kv_stride_block <= 0 || kv_stride_pos <= 0 || kv_stride_head <= 0 || kv_stride_part < 0)
+    return fail(EKV_EINVAL, "the cache's strides must be positive");
+  if (((uintptr_t)q & 15) || (q_stride_token & 7) || (q_stride_head & 7))
+    return fail(EKV_EINVAL, "the query must be 16-byte aligned with strides of whole 16-byte units");
+  if (((uintptr_t)out & 15) || (out_stride_token & 7) || (out_stride_head & 7))
+    return fail(EKV_EINVAL, "the output must be 16-byte aligned with strides of whole 16-byte units");
+  if (groups < 0 || groups > rows) return fail(EKV_EINVAL, "%d groups of %d rows", groups, rows);
+  if (groups > 1 && (!group_start || !prefix_blocks))
+    return fail(EKV_EINVAL, "%d groups need group_start and prefix_blocks", groups);
+  if (prefix_common < 0) return fail(EKV_EINVAL, "a prefix of %d blocks", prefix_common);
+  const int64_t tiles = (int64_t)width * block_size / kTile + 1;
+  const int G = q_heads / kv_heads;
+  if ((int64_t)width * block_size > 0x7fffffffll - 4096 ||
+      ((int64_t)rows + (int64_t)tokens * G / 16) * kv_heads * tiles > 0x7fffffffll)
+    return fail(EKV_ENOTSUP, "a launch of more than 2^31 - 1 tiles (rows x heads x tokens)");
+  if ((int64_t)tokens * q_heads > 0x7fffffffll / 4) return fail(EKV_ENOTSUP, "more than 2^29 query rows");
+  c.mt[0] = pick_mt(tokens, rows, G);
+  c.mt[1] = groups > 0 ? pick_mt(tokens, groups, G) : 0;
+  const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, kAttendMaxCtas, c.mt);
+  if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
+    return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
+  int device = 0, sms = 0;
+  int rc = current_device(&device);
+  if (rc != EKV_OK) return rc;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return check_launch("cudaDeviceGetAttribute");
+  c.sms = sms;
+  c.ws = static_cast<uint8_t*>(workspace);
+  AttendParams& p = c.p;
+  p.q = q; p.q_s0 = q_stride_token; p.q_s1 = q_stride_head;
+  p.table = table; p.table_s0 = table_stride; p.lens = lens; p.query_start = query_start;
+  p.out = out; p.out_s0 = out_stride_token; p.out_s1 = out_stride_head; p.lse = lse;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.rows = rows; p.width = width; p.block_size = block_size;
+  p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : block_size == 32 ? 5 : 6;
+  p.heads = kv_heads; p.G = G; p.q_heads = q_heads; p.pool_blocks = pool_blocks; p.tokens = tokens;
+  p.groups = groups; p.group_start = group_start; p.prefix_blocks = prefix_blocks; p.prefix_common = prefix_common;
+  p.status = status; p.max_ctas = kAttendMaxCtas;
+  return encode_cache_maps(p, kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, head_dim, dtype);
+}
+
+int run(const AttendCall& c, int head_dim, int dtype, cudaStream_t s) {
+  if (dtype == EKV_DTYPE_BF16)
+    return head_dim == 128 ? attend<__nv_bfloat16, 128>(c.p, c.w, c.mt, c.ws, c.sms, s)
+                           : attend<__nv_bfloat16, 64>(c.p, c.w, c.mt, c.ws, c.sms, s);
+  return head_dim == 128 ? attend<__half, 128>(c.p, c.w, c.mt, c.ws, c.sms, s)
+                         : attend<__half, 64>(c.p, c.w, c.mt, c.ws, c.sms, s);
+}
+
+}  // namespace
+
+extern "C" size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads, int kv_heads, int head_dim) {
+  if (rows <= 0 || tokens <= 0 || groups < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
+  const int G = q_heads / kv_heads;
+  const int mt[2] = {pick_mt(tokens, rows, G), groups > 0 ? pick_mt(tokens, groups, G) : 0};
+  return workspace_layout(rows, tokens, groups, q_heads, head_dim, kAttendMaxCtas, mt).total;
+}
+
+extern "C" int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
+                          int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos, int64_t kv_stride_head,
+                          int64_t pool_blocks, const int32_t* table, int64_t table_stride, const int32_t* lens,
+                          const int32_t* query_start, int tokens, int rows, int width, int block_size, int q_heads,
+                          int kv_heads, int head_dim, int dtype, float scale, int groups, const int32_t* group_start,
+                          const int32_t* prefix_blocks, int prefix_common, void* out, int64_t out_stride_token,
+                          int64_t out_stride_head, float* lse, void* workspace, size_t workspace_bytes, uint32_t* status,
+                          void* stream) {
+  clear_error();
+  AttendCall c{};
+  const int rc = prepare(c, q, q_stride_token, q_stride_head, kv, kv_stride_block, kv_stride_part, kv_stride_pos,
+                         kv_stride_head, pool_blocks, table, table_stride, lens, query_start, tokens, rows, width, block_size,
+                         q_heads, kv_heads, head_dim, dtype, scale, groups, group_start, prefix_blocks, prefix_common, out,
+                         out_stride_token, out_stride_head, lse, workspace, workspace_bytes, status);
+  return rc != EKV_OK ? rc : run(c, head_dim, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
+                                 int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                                 int64_t kv_stride_head, int64_t pool_blocks, const int32_t* table, int64_t table_stride,
+                                 const int32_t* lens, const int32_t* query_start, int tokens, int rows, int width,
+                                 int block_size, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                                 float* scores, int64_t score_stride_slot, int64_t score_stride_head, int n_slots,
+                                 const int32_t* slots, const int32_t* fresh, float decay, void* out,
+                                 int64_t out_stride_token, int64_t out_stride_head, float* lse, void* workspace,
+                                 size_t workspace_bytes, uint32_t* status, void* stream) {
+  clear_error();
+  if (!scores || !lse) return fail(EKV_EINVAL, "a required device pointer is NULL");
+  if (n_slots <= 0 || score_stride_slot < 0 || score_stride_head < (int64_t)width * block_size ||
+      (n_slots > 1 && score_stride_slot < score_stride_head))
+    return fail(EKV_EINVAL, "scores must hold a slot's heads of at least width * block_size tokens each");
+  if (!slots && n_slots < rows) return fail(EKV_EINVAL, "%d score slots for %d rows", n_slots, rows);
+  if (!(decay >= 0.f && decay <= 1.f)) return fail(EKV_EINVAL, "the decay must lie in [0, 1]");
+  AttendCall c{};
+  int rc = prepare(c, q, q_stride_token, q_stride_head, kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head,
+                   pool_blocks, table, table_stride, lens, query_start, tokens, rows, width, block_size, q_heads, kv_heads,
+                   head_dim, dtype, scale, 0, nullptr, nullptr, 0, out, out_stride_token, out_stride_head, lse, workspace,
+                   workspace_bytes, status);
+  if (rc != EKV_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = run(c, head_dim, dtype, s);
+  if (rc != EKV_OK) return rc;
+  return launch_score_kernel(c.p, head_dim, dtype, scores, score_stride_slot, score_stride_head, slots, fresh, n_slots,
+                             decay, c.sms, s);
+}

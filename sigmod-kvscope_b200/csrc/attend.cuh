@@ -1,0 +1,307 @@
+// Shared parts of the attention kernels over the paged cache (attend.cu, attend_mma5.cu, attend_scores.cu): the launch
+// parameters, what a unit of work is, and how the tiles of a launch are dealt out to its CTAs.
+//
+// Work. A unit is one row of the batch (its own tokens, behind its group's shared prefix), or, in a prefix
+// launch, one group of rows (the tokens they share). A unit's M = query tokens x query heads per KV head
+// query rows are cut into M tiles, its tokens into tiles of kTile; the launch's tiles, numbered unit by
+// unit, KV head, M tile, token tile, are dealt evenly: CTA c of n takes tiles [c W / n, (c + 1) W / n). Every
+// CTA computes the units' running tile counts itself (a scan of the rows' lengths), so no plan travels
+// through the host and no launch precedes the first load.
+//
+// Parts. A CTA that covers a whole (unit, KV head, M tile) finishes it; one that covers some of its tiles
+// leaves the part's running maximum, sum and unnormalised output in the workspace. A CTA has at most two
+// such parts: one that starts where the item started earlier (slot 2c), one that ends before it (2c + 1).
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "ekv_common.cuh"
+
+namespace ekv {
+
+constexpr int kTile = 64;          // tokens of a tile
+constexpr int kAttendMaxRows = 2048;
+constexpr int kAttendMaxCtas = 512;
+
+struct AttendParams {
+  CUtensorMap kmap, vmap;  // the caches as (head dim, KV head, token of the block, block)
+  const void* q;
+  int64_t q_s0, q_s1;
+  const int32_t* table;
+  int64_t table_s0;
+  const int32_t* lens;
+  const int32_t* query_start;  // [rows + 1], or NULL: row r's one query token is token r
+  void* out;
+  int64_t out_s0, out_s1;
+  float* lse;  // [tokens][q_heads], may be NULL
+  float scale_log2;  // scale * log2(e): the kernels work in powers of two
+  int rows, width, block_size, block_shift, heads, G, q_heads;
+  int64_t pool_blocks;
+  int tokens;
+  int groups;                    // 0: nothing is shared
+  const int32_t* group_start;    // [groups + 1], or NULL: one group of every row
+  const int32_t* prefix_blocks;  // [groups], or NULL: prefix_common
+  int prefix_common;
+  uint32_t* status;
+  // the workspace, of the launch's phase and (for the combine kernel) of both
+  int32_t* cum;   // [units + 1] running tile counts, then the number of CTAs that share them
+  float* parts;   // [2 CTAs][MT][D], and behind them their [2 CTAs][MT][2] maxima and sums
+  float* whole;   // [tokens * q_heads][D] and [tokens * q_heads][2]: finished items when another phase joins
+  int mt_rows;    // query rows of an M tile
+  int max_ctas;
+};
+
+// ---- units -----------------------------------------------------------------------------------------
+
+struct QueryRange {
+  int q0, nq;
+};
+
+// Row r's query tokens; none when query_start does not describe tokens of the batch.
+__device__ __forceinline__ QueryRange row_queries(const AttendParams& p, int r, bool report) {
+  if (p.query_start == nullptr) return {r, r < p.tokens ? 1 : 0};
+  const int a = p.query_start[r], b = p.query_start[r + 1];
+  if (a < 0 || b < a || b > p.tokens) {
+    if (report) set_status(p.status, EKV_STATUS_BAD_QROW);
+    return {0, 0};
+  }
+  return {a, b - a};
+}
+
+// Row r's cached tokens, at most what its table holds.
+__device__ __forceinline__ int row_tokens(const AttendParams& p, int r, bool report) {
+  const int len = p.lens[r];
+  const int most = p.width << p.block_shift;
+  if (len > most) {
+    if (report) set_status(p.status, EKV_STATUS_LEN_OVER_WIDTH);
+    return most;
+  }
+  return len > 0 ? len : 0;
+}
+
+struct RowRange {
+  int a, b;
+};
+
+__device__ __forceinline__ RowRange group_rows(const AttendParams& p, int g) {
+  if (p.group_start == nullptr) return {0, p.rows};
+  int a = p.group_start[g], b = p.group_start[g + 1];
+  a = min(max(a, 0), p.rows);
+  b = min(max(b, a), p.rows);
+  return {a, b};
+}
+
+__device__ __forceinline__ int group_prefix(const AttendParams& p, int g) {  // tokens
+  const int blocks = p.prefix_blocks != nullptr ? p.prefix_blocks[g] : p.prefix_common;
+  return min(max(blocks, 0), p.width) << p.block_shift;
+}
+
+// The group of row r, or -1.
+__device__ __forceinline__ int group_of(const AttendParams& p, int r) {
+  if (p.groups == 0) return -1;
+  if (p.group_start == nullptr) return 0;
+  int lo = 0, hi = p.groups;  // the last group that starts at or before r
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.group_start[mid] <= r) lo = mid; else hi = mid;
+  }
+  const RowRange rr = group_rows(p, lo);
+  return r >= rr.a && r < rr.b ? lo : -1;
+}
+
+// Tokens that row r leaves to its group's prefix launch.
+__device__ __forceinline__ int row_prefix(const AttendParams& p, int r) {
+  const int g = group_of(p, r);
+  return g < 0 ? 0 : group_prefix(p, g);
+}
+
+// The query tokens of a group: those of its rows, which follow one another.
+__device__ __forceinline__ QueryRange group_queries(const AttendParams& p, RowRange rr) {
+  if (rr.b <= rr.a) return {0, 0};
+  if (p.query_start == nullptr) {
+    const int b = min(rr.b, p.tokens);
+    return {rr.a, max(b - rr.a, 0)};
+  }
+  const int a = p.query_start[rr.a], b = p.query_start[rr.b];
+  if (a < 0 || b < a || b > p.tokens) return {0, 0};
+  return {a, b - a};
+}
+
+// The row in [rr.a, rr.b) that holds query token t (-1 if none does) by binary search of query_start.
+__device__ __forceinline__ int row_of_token(const AttendParams& p, RowRange rr, int t) {
+  if (p.query_start == nullptr) return t >= rr.a && t < rr.b ? t : -1;
+  int lo = rr.a, hi = rr.b;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.query_start[mid] <= t) lo = mid; else hi = mid;
+  }
+  if (lo >= rr.b) return -1;
+  const QueryRange q = row_queries(p, lo, false);
+  return t >= q.q0 && t < q.q0 + q.nq ? lo : -1;
+}
+
+// Positions below this are visible to query token t of row r.
+__device__ __forceinline__ int token_limit(const AttendParams& p, int r, int t) {
+  const QueryRange q = row_queries(p, r, false);
+  return row_tokens(p, r, false) - q.nq + (t - q.q0) + 1;
+}
+
+// ---- the plan ----------------------------------------------------------------------------------------
+
+// In shared memory: cum[units + 1], the running tile counts, and for a prefix launch lead[units], the longest
+// row of each group (its length << 32 | ~row), whose table is read.
+struct Plan {
+  int* cum;
+  unsigned long long* lead;
+  int units;
+};
+
+__device__ __forceinline__ int lead_row(unsigned long long v) { return (int)~(uint32_t)v; }
+__device__ __forceinline__ int lead_len(unsigned long long v) { return (int)(v >> 32); }
+
+__host__ __device__ inline size_t plan_bytes(int units, bool prefix) {
+  return ((size_t)(units + 1) * 4 + 15) / 16 * 16 + (prefix ? (size_t)units * 8 : 0);
+}
+
+__device__ __forceinline__ Plan plan_at(void* smem, int units, bool prefix) {
+  Plan plan;
+  plan.units = units;
+  plan.cum = static_cast<int*>(smem);
+  uint8_t* end = static_cast<uint8_t*>(smem) + ((size_t)(units + 1) * 4 + 15) / 16 * 16;
+  plan.lead = prefix ? reinterpret_cast<unsigned long long*>(end) : nullptr;
+  return plan;
+}
+
+// A unit: its query tokens, the table row its blocks are in, and its positions [from, to).
+struct Unit {
+  QueryRange q;
+  int row, from, to;
+  __device__ __forceinline__ int m_tiles(const AttendParams& p, int MT) const { return (q.nq * p.G + MT - 1) / MT; }
+  __device__ __forceinline__ int tiles() const {
+    return to > from && q.nq > 0 ? (to - from + kTile - 1) / kTile : 0;
+  }
+};
+
+template <bool PREFIX>
+__device__ __forceinline__ Unit unit_at(const AttendParams& p, const Plan& plan, int u, bool report) {
+  Unit un;
+  if (PREFIX) {
+    const RowRange rr = group_rows(p, u);
+    un.q = group_queries(p, rr);
+    un.row = lead_row(plan.lead[u]);
+    un.from = 0;
+    un.to = min(group_prefix(p, u), lead_len(plan.lead[u]));  // 0 for a group with no rows
+  } else {
+    un.q = row_queries(p, u, report);
+    un.row = u;
+    un.from = row_prefix(p, u);
+    un.to = row_tokens(p, u, report);
+  }
+  return un;
+}
+
+// Fills the plan with every thread of the CTA (THREADS of them); `scratch` holds THREADS / 32 + 1 ints.
+template <bool PREFIX, int THREADS>
+__device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& plan, int MT, int* scratch) {
+  const bool report = blockIdx.x == 0;
+  if (PREFIX) {
+    for (int g = threadIdx.x; g < plan.units; g += THREADS) plan.lead[g] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < p.rows; r += THREADS) {
+      const int g = group_of(p, r);
+      if (g >= 0)
+        atomicMax(plan.lead + g, (unsigned long long)(uint32_t)row_tokens(p, r, false) << 32 | (uint32_t)~(uint32_t)r);
+    }
+    __syncthreads();
+  }
+  int carry = 0;
+  for (int base = 0; base < plan.units; base += THREADS) {
+    const int u = base + threadIdx.x;
+    int n = 0;
+    if (u < plan.units) {
+      const Unit un = unit_at<PREFIX>(p, plan, u, report);
+      n = un.tiles() * p.heads * un.m_tiles(p, MT);
+    }
+    int total = 0;
+    const int before = block_exclusive_scan<THREADS>(n, scratch, &total);
+    if (u < plan.units) plan.cum[u] = carry + before;
+    carry += total;
+  }
+  if (threadIdx.x == 0) plan.cum[plan.units] = carry;
+  __syncthreads();
+}
+
+// The tiles of CTA c when n CTAs share W, and the CTA that holds tile t.
+__device__ __forceinline__ int first_tile(int c, int W, int n) { return (int)((int64_t)c * W / n); }
+__device__ __forceinline__ int cta_of(int t, int W, int n) { return (int)((((int64_t)t + 1) * n - 1) / W); }
+__device__ __forceinline__ int sharing_ctas(int W, int ctas) { return W < ctas ? (W > 0 ? W : 1) : ctas; }
+
+// One item of a CTA's range: (unit, KV head, M tile) and its tiles [first, last) that the CTA covers.
+struct Item {
+  Unit un;
+  int unit, head, mt, first, last, tiles;
+};
+
+template <bool PREFIX>
+__device__ __forceinline__ Item item_at(const AttendParams& p, const Plan& plan, int MT, int t, int end) {
+  int lo = 0, hi = plan.units;  // the last unit that starts at or before t (units without tiles never hold one)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (plan.cum[mid] <= t) lo = mid; else hi = mid;
+  }
+  Item it;
+  it.unit = lo;
+  it.un = unit_at<PREFIX>(p, plan, lo, false);
+  it.tiles = it.un.tiles();
+  const int mts = it.un.m_tiles(p, MT);
+  const int rem = t - plan.cum[lo], hm = rem / it.tiles;
+  it.head = hm / mts;
+  it.mt = hm - it.head * mts;
+  it.first = rem - hm * it.tiles;
+  it.last = min(it.tiles, it.first + end - t);
+  return it;
+}
+
+// ---- copies ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void tensor_copy_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                               uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+__device__ __forceinline__ void proxy_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLn2 = 0.69314718055994531f;
+
+// ---- host ---------------------------------------------------------------------------------------------------
+
+// Encodes p.kmap and p.vmap for a cache at `kv` ([blocks][2][block_size][heads][D], element strides).
+int encode_cache_maps(AttendParams& p, const void* kv, int64_t s_block, int64_t s_part, int64_t s_pos, int64_t s_head,
+                      int dim, int dtype);
+
+// Adds each token's weight to its score after an attention launch that left a.lse (attend_scores.cu).
+int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,
+                        const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int sms, cudaStream_t s);
+
+}  // namespace ekv

@@ -19,6 +19,7 @@ DTYPE_F16, DTYPE_BF16 = 0, 1
 AGG_MEAN, AGG_MAX = 0, 1
 SHARE_FINALIZE = 2
 STATUS_BAD_BLOCK_ID, STATUS_LEN_OVER_WIDTH, STATUS_BAD_QROW, STATUS_WAIT_TIMEOUT = 1, 2, 4, 8
+STATUS_BAD_SLOT, STATUS_BLOCK_SHARED, STATUS_BAD_LIST = 16, 32, 64
 POLICY_SUM, POLICY_UNIFORM, POLICY_NEWEST, POLICY_MAXMIN = 0, 1, 2, 3
 AUDIT_CHUNK_TILES = 8
 
@@ -115,6 +116,35 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i32, _i32, _i32, _p, _i64, _p, _p, _i64, _p],
     ),
     "ekv_compact_block_table": (_i32, [_p, _i64, _p, _p, _i64, _i32, _i32, _i32, _p, _i64, _p, _p]),
+    "ekv_attend_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "ekv_attend": (
+        _i32,
+        [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64,  # q and strides, kv and strides, pool_blocks
+         _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32,  # table lens query_start tokens rows width bs q_heads
+         _i32, _i32, _i32, _f32, _i32, _p, _p, _i32,  # kv_heads D dtype scale groups group_start prefix common
+         _p, _i64, _i64, _p, _p, _sz, _p, _p],  # out lse workspace bytes status stream
+    ),
+    "ekv_attend_scored": (
+        _i32,
+        [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64,  # q and strides, kv and strides, pool_blocks
+         _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32,  # table lens query_start tokens rows width bs q_heads
+         _i32, _i32, _i32, _f32,  # kv_heads D dtype scale
+         _p, _i64, _i64, _i32, _p, _p, _f32,  # scores and strides, n_slots slots fresh decay
+         _p, _i64, _i64, _p, _p, _sz, _p, _p],  # out lse workspace bytes status stream
+    ),
+    "ekv_select_tokens": (
+        _i32,
+        [_p, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i32,  # scores .. slots lens keep .. heads
+         _p, _i64, _i64, _p, _p, _p],  # kept new_lens status stream
+    ),
+    "ekv_compact_tokens_workspace_bytes": (_sz, [_i32, _i32, _i64]),
+    "ekv_compact_tokens": (
+        _i32,
+        [_p, _i64, _i64, _i64, _i64, _i64, _i32,  # kv and byte strides, pool_blocks head_bytes
+         _p, _i64, _p, _i32, _i32, _i32, _i32,  # table lens rows width heads block_size
+         _p, _i64, _i64, _i32, _p, _i32,  # kept columns new_lens first_tokens
+         _p, _i64, _i64, _i32, _p, _p, _sz, _p, _p],  # scores n_slots slots workspace bytes status stream
+    ),
 }
 
 _lib: ctypes.CDLL | None = None

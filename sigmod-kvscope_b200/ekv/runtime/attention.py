@@ -1,0 +1,216 @@
+"""Attention over the paged KV cache through a block table, on the sm_100a kernels.
+
+The audit kernel (``audit_kernel``) measures what each block of a row draws and the view (``block_view``)
+drops blocks from the row; ``attend`` is the attention that reads the row, whole or viewed: ``table`` and
+``lens`` are an engine's block table and lengths or the buffers of a ``DecodeView``. The reference leaves this
+step to its engine's backend.
+
+Rows that begin with the same blocks (samples of one prompt, requests under one system prompt) are read
+once: ``prefix_blocks`` says how many blocks each group of rows shares, and the queries of all the group's
+rows meet the shared keys and values together. The kernels take their work from the lengths on the device, so
+a call is the same for every batch of its shape and a CUDA graph can capture it.
+
+``attend_scored`` also adds up, per KV head, the attention weight each cached token receives from step to step:
+the score by which ``eviction`` decides which tokens of a bounded cache to keep.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _index(name: str, t: torch.Tensor | None, size: int, device: torch.device) -> int | None:
+    """The address of an int32 index array of at least ``size`` entries on the call's device."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < size or t.device != device or (size > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of at least {size} entries on {device}")
+    return t.data_ptr()
+
+
+def _check_batch(query: torch.Tensor, kv_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> None:
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
+        raise ValueError(f"expected a KV cache [blocks, 2, block, heads, dim], got {tuple(kv_cache.shape)}")
+    if query.dim() != 3 or query.shape[2] != kv_cache.shape[4]:
+        raise ValueError(f"expected a query [tokens, heads, {kv_cache.shape[4]}], got {tuple(query.shape)}")
+    if query.dtype not in _DTYPES or kv_cache.dtype != query.dtype:
+        raise ValueError(f"query and cache must both be float16 or bfloat16, got {query.dtype}, {kv_cache.dtype}")
+    if query.stride(2) != 1 or kv_cache.stride(4) != 1:
+        raise ValueError("the head dimension of the query and the cache must be contiguous")
+    if table.dtype != torch.int32 or lens.dtype != torch.int32:
+        raise ValueError("the block table and the lengths must be int32")
+    if table.dim() != 2 or lens.dim() != 1 or lens.shape[0] < table.shape[0]:
+        raise ValueError("the block table must be [rows, width] with a length per row")
+    if (table.shape[1] > 1 and table.stride(1) != 1) or (lens.shape[0] > 1 and lens.stride(0) != 1):
+        raise ValueError("the block table's rows and the lengths must be contiguous")
+    device = query.device
+    if device.type != "cuda":
+        raise ValueError("the attention runs on the device: the query must be a CUDA tensor")
+    if kv_cache.device != device or table.device != device or lens.device != device:
+        raise ValueError(f"the cache, the block table and the lengths must be on the query's device {device}")
+
+
+def _outputs(query: torch.Tensor, out: torch.Tensor | None, lse: torch.Tensor | None):
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(2) != 1:
+        raise ValueError("out must match the query's shape, dtype and device, its head dimension contiguous")
+    if lse is None:
+        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
+    elif lse.shape != query.shape[:2] or lse.dtype != torch.float32 or lse.device != query.device or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous float32 {tuple(query.shape[:2])} tensor on the query's device")
+    return out, lse
+
+
+def _status(status: torch.Tensor | None, device: torch.device) -> int | None:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+        raise ValueError(f"status must be one int32 on {device}")
+    return status.data_ptr()
+
+
+def attend(
+    query: torch.Tensor,
+    kv_cache: torch.Tensor,
+    table: torch.Tensor,
+    lens: torch.Tensor,
+    scale: float,
+    *,
+    query_start: torch.Tensor | None = None,
+    prefix_blocks: torch.Tensor | int | None = None,
+    group_start: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``softmax(scale * query keys) values`` of every query token, and the log of its sum of exponentials.
+
+    ``query`` is [tokens, q_heads, dim], ``kv_cache`` [blocks, 2, block, kv_heads, dim] (keys, then values) of
+    the same dtype, float16 or bfloat16, ``table`` int32 [rows, width] and ``lens`` int32 [rows] the row's tokens
+    in the cache, those of its query included. Row ``r`` has the query tokens ``query_start[r]`` to
+    ``query_start[r + 1]`` (int32 [rows + 1]; without it one token each), the last of which sees the whole row,
+    each one before it one position less.
+
+    ``prefix_blocks`` int32 [groups]: the rows ``group_start[g]`` to ``group_start[g + 1]`` (int32 [groups + 1];
+    without it one group of every row) begin with the same ``prefix_blocks[g]`` blocks, which are read once for
+    the group. An int is one group of every row, as an engine's common prefix length gives it.
+
+    Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a
+    token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
+    in the tables, which the kernels skip. The call runs on the current stream of the query's device.
+    """
+    _check_batch(query, kv_cache, table, lens)
+    device = query.device
+    tokens, q_heads, dim = query.shape
+    rows, width = table.shape
+    blocks, _, block_size, kv_heads, _ = kv_cache.shape
+    groups = common = 0
+    prefix = None
+    if isinstance(prefix_blocks, torch.Tensor):
+        groups = prefix_blocks.shape[0] if prefix_blocks.dim() == 1 else 0
+        if groups == 0 or (group_start is None and groups != 1):
+            raise ValueError("prefix_blocks must hold a count per group, and several groups need group_start")
+        prefix = _index("prefix_blocks", prefix_blocks, groups, device)
+    elif prefix_blocks is not None:
+        common = int(prefix_blocks)
+        if common < 0:
+            raise ValueError("prefix_blocks must not be negative")
+        groups = 1 if common else 0
+    if group_start is not None and prefix is None:
+        raise ValueError("group_start needs the groups' prefix_blocks")
+    starts = _index("query_start", query_start, rows + 1, device)
+    members = _index("group_start", group_start, groups + 1, device)
+    if starts is None and tokens != rows:
+        raise ValueError(f"{tokens} query tokens for {rows} rows: without query_start every row has one")
+    word = _status(status, device)
+    out, lse = _outputs(query, out, lse)
+    if tokens == 0 or rows == 0:
+        return out, lse
+    lib = _lib.load()
+    size = lib.ekv_attend_workspace_bytes(rows, tokens, groups, q_heads, kv_heads, dim)
+    with torch.cuda.device(device):
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        rc = lib.ekv_attend(
+            query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
+            kv_cache.stride(1), kv_cache.stride(2), kv_cache.stride(3), blocks, table.data_ptr(), table.stride(0),
+            lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
+            scale, groups, members, prefix, common, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+            workspace.data_ptr(), size, word, _lib.current_stream(),
+        )
+    _lib.check(rc, "ekv_attend")
+    return out, lse
+
+
+def check_scores(scores: torch.Tensor, heads: int, tokens: int, device: torch.device) -> None:
+    """A score table [slots, heads, >= tokens] float32 on ``device``, each head's scores contiguous."""
+    if scores.dtype != torch.float32 or scores.dim() != 3 or scores.device != device:
+        raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor on {device}")
+    if scores.shape[1] != heads or scores.shape[2] < tokens:
+        raise ValueError(f"scores of {heads} heads and at least {tokens} tokens are needed, got {tuple(scores.shape)}")
+    if scores.stride(2) != 1:
+        raise ValueError("the scores of a head must be contiguous")
+
+
+def attend_scored(
+    query: torch.Tensor,
+    kv_cache: torch.Tensor,
+    table: torch.Tensor,
+    lens: torch.Tensor,
+    scale: float,
+    scores: torch.Tensor,
+    *,
+    query_start: torch.Tensor | None = None,
+    slots: torch.Tensor | None = None,
+    fresh: torch.Tensor | None = None,
+    decay: float = 1.0,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    status: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """``attend``, and the weight that every cached token receives added to its score, in place.
+
+    ``scores`` is float32 [slots, kv_heads, >= width * block]; row ``r`` uses slot ``slots[r]`` (int32 [rows];
+    without it slot ``r``). Per KV head, the token at position ``t`` receives the sum of ``exp(scale q.k - lse)`` over
+    the row's query tokens and the head's query heads. The row's newest ``fresh[r]`` tokens (int32 [rows]; without it
+    the row's query tokens) have no score yet and take that sum; the others' scores become ``decay`` times
+    themselves plus it. A prompt's last tokens score the whole prompt with ``fresh = lens``. A negative slot attends
+    without scoring; slots must otherwise be one row's alone.
+
+    The other arguments, and the ``(out, lse)`` returned, are ``attend``'s.
+    """
+    _check_batch(query, kv_cache, table, lens)
+    device = query.device
+    tokens, q_heads, dim = query.shape
+    rows, width = table.shape
+    blocks, _, block_size, kv_heads, _ = kv_cache.shape
+    check_scores(scores, kv_heads, width * block_size, device)
+    starts = _index("query_start", query_start, rows + 1, device)
+    places = _index("slots", slots, rows, device)
+    new = _index("fresh", fresh, rows, device)
+    if starts is None and tokens != rows:
+        raise ValueError(f"{tokens} query tokens for {rows} rows: without query_start every row has one")
+    if not 0.0 <= decay <= 1.0:
+        raise ValueError("the decay must lie in [0, 1]")
+    word = _status(status, device)
+    out, lse = _outputs(query, out, lse)
+    if tokens == 0 or rows == 0:
+        return out, lse
+    lib = _lib.load()
+    size = lib.ekv_attend_workspace_bytes(rows, tokens, 0, q_heads, kv_heads, dim)
+    with torch.cuda.device(device):
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        rc = lib.ekv_attend_scored(
+            query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
+            kv_cache.stride(1), kv_cache.stride(2), kv_cache.stride(3), blocks, table.data_ptr(), table.stride(0),
+            lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
+            scale, scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[0], places, new, decay,
+            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), workspace.data_ptr(), size, word,
+            _lib.current_stream(),
+        )
+    _lib.check(rc, "ekv_attend_scored")
+    return out, lse

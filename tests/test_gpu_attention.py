@@ -1,0 +1,309 @@
+"""Attention over the paged cache against the float64 oracle: lengths, masks, layouts, shared prefixes.
+
+Tolerances. ``out`` is rounded to its type (half a step, u = eps / 2 relative) and its probabilities were rounded to
+the same type before the products with the values, each off by at most u relative: |error| <= u |out| + u (1 + u)
+sum_j p_j |v_j| <= u (|out| + 1.01 max |v|). Float32 work (scores of at most 128 products, sums) adds relative errors
+below 128 * 2^-24 * sum |q k| * scale in the exponent; with the inputs here (|x| <= 40) 3e-5 covers it. fp16
+probabilities below 2^-14 are off by at most 2^-25 each, 2^-25 * n * max |v| in all: 2^-25 * 1024 < u / 8.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as oat
+
+pytestmark = pytest.mark.gpu
+
+
+def make(seed, lens, queries=None, q_heads=8, kv_heads=2, dim=128, block=16, dtype=torch.bfloat16, width=None,
+         groups=None, spare=3):
+    """A batch: rows with their own blocks, except that a group (first row, last row, blocks) shares its prefix."""
+    gen = torch.Generator().manual_seed(seed)
+    rows = len(lens)
+    width = width or max(1, max(-(-n // block) for n in lens))
+    pool = rows * width + spare
+    table = torch.randperm(pool, generator=gen)[: rows * width].reshape(rows, width).to(torch.int32)
+    for a, b, shared in groups or []:
+        table[a:b, :shared] = table[a, :shared].clone()
+    queries = [1] * rows if queries is None else queries
+    start = torch.tensor(np.concatenate([[0], np.cumsum(queries)]), dtype=torch.int32)
+    query = torch.randn(int(start[-1]), q_heads, dim, generator=gen).to(dtype)
+    cache = torch.randn(pool, 2, block, kv_heads, dim, generator=gen).to(dtype)
+    return dict(query=query, cache=cache, table=table, lens=torch.tensor(lens, dtype=torch.int32), start=start)
+
+
+def on_device(x):
+    return {k: v.cuda() for k, v in x.items()}
+
+
+def check(got, x, scale, dtype, pool_ok=None, start=True):
+    out, lse, _ = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(),
+                             x["lens"].numpy(), scale, x["start"].numpy() if start else None, pool_ok)
+    u = torch.finfo(dtype).eps / 2
+    biggest = x["cache"][:, 1].float().nan_to_num(0, 0, 0).abs().max().item()
+    some = ~np.isnan(lse)
+    o, e = got[0].float().cpu().numpy().astype(np.float64)[some], got[1].cpu().numpy().astype(np.float64)[some]
+    np.testing.assert_array_equal(np.isinf(e), np.isinf(lse[some]))
+    live = np.isfinite(lse[some])
+    np.testing.assert_allclose(e[live], lse[some][live], rtol=0, atol=3e-5)
+    assert np.all(np.abs(o - out[some]) <= 1.05 * u * (np.abs(out[some]) + 1.01 * biggest) + 3e-5 * biggest)
+    assert np.all(o[~live] == 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, block", [(128, 16), (64, 16), (128, 8), (64, 32), (128, 64)])
+def test_decode_rows_of_every_length(cuda_lib, dtype, dim, block):
+    from ekv.runtime.attention import attend
+
+    lens = [1, 0, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 641]
+    x = make(1, lens, dim=dim, block=block, dtype=dtype)
+    d = on_device(x)
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 1 / math.sqrt(dim))
+    check(got, x, 1 / math.sqrt(dim), dtype, start=False)
+
+
+@pytest.mark.parametrize("q_heads, kv_heads", [(2, 2), (10, 2), (16, 1), (32, 1), (12, 3), (48, 1)])
+def test_head_groups(cuda_lib, q_heads, kv_heads):
+    from ekv.runtime.attention import attend
+
+    x = make(2, [70, 333, 5], q_heads=q_heads, kv_heads=kv_heads)
+    d = on_device(x)
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.09), x, 0.09, torch.bfloat16, start=False)
+
+
+@pytest.mark.parametrize("queries", [[1, 4, 2, 1], [0, 7, 0, 3], [33, 1, 20, 64], [5, 5, 5, 5]])
+def test_several_query_tokens_a_row(cuda_lib, queries):
+    from ekv.runtime.attention import attend
+
+    x = make(3, [100, 64, 33, 200], queries=queries, dtype=torch.float16)
+    d = on_device(x)
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"])
+    check(got, x, 0.1, torch.float16)
+
+
+def test_more_query_tokens_than_cached_ones(cuda_lib):
+    from ekv.runtime.attention import attend
+
+    x = make(4, [3, 0, 20], queries=[5, 2, 1])  # the first tokens of row 0 see nothing, nor do row 1's
+    d = on_device(x)
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"]), x, 0.1, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("queries", [1, 3])
+@pytest.mark.parametrize("groups", [[(0, 6, 5)], [(0, 2, 9), (2, 3, 1), (3, 6, 4)], [(0, 1, 3), (1, 6, 0)]])
+def test_shared_prefixes(cuda_lib, dim, queries, groups):
+    from ekv.runtime.attention import attend
+
+    lens = [max(b for a, b_, b in groups if a <= r < b_) * 16 + 1 + 37 * r + queries for r in range(6)]
+    x = make(5, lens, queries=[queries] * 6, dim=dim, groups=groups, q_heads=16, kv_heads=2)
+    d = on_device(x)
+    group_start = torch.tensor([a for a, _, _ in groups] + [6], dtype=torch.int32, device="cuda")
+    prefix = torch.tensor([b for _, _, b in groups], dtype=torch.int32, device="cuda")
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=prefix,
+                 group_start=group_start)
+    check(got, x, 0.1, torch.bfloat16)
+    if len(groups) == 1:
+        again = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=groups[0][2])
+        assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
+# ---- weights accumulated per token -------------------------------------------------------------------
+
+
+def run_scored(x, d, scale, scores, slots=None, fresh=None, decay=1.0):
+    from ekv.runtime.attention import attend_scored
+
+    dev = None if slots is None else torch.tensor(slots, dtype=torch.int32, device="cuda")
+    new = None if fresh is None else torch.tensor(fresh, dtype=torch.int32, device="cuda")
+    got = scores.cuda()
+    out = attend_scored(d["query"], d["cache"], d["table"], d["lens"], scale, got, query_start=d["start"], slots=dev,
+                        fresh=new, decay=decay)
+    queries = (x["start"][1:] - x["start"][:-1]).tolist()
+    _, _, w = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(),
+                         scale, x["start"].numpy())
+    want = oat.accumulate(scores.numpy(), slots or list(range(len(queries))), x["lens"].tolist(), queries, w, fresh, decay)
+    # a weight's exponent is off by at most 3e-5 (the log-sum-exp's and the score's error), the sum by float32 steps
+    weight = max(1.0, max(float(v.max()) if v.size else 0.0 for v in w))
+    np.testing.assert_allclose(got.cpu().numpy(), want, rtol=1e-6, atol=4e-5 * weight)
+    return out
+
+
+@pytest.mark.parametrize("dtype, dim, block", [(torch.bfloat16, 128, 16), (torch.float16, 64, 32), (torch.bfloat16, 64, 8)])
+@pytest.mark.parametrize("queries", [[1] * 6, [3, 1, 0, 9, 2, 40]])
+def test_scores_gather_the_weights(cuda_lib, dtype, dim, block, queries):
+    lens = [1, 64, 0, 130, 65, 333]
+    x = make(6, lens, queries=queries, dim=dim, block=block, dtype=dtype, q_heads=10)
+    capacity = x["table"].shape[1] * block
+    scores = torch.rand(8, 2, capacity, generator=torch.Generator().manual_seed(1))
+    got = run_scored(x, on_device(x), 0.1, scores, slots=[7, 0, 3, -1, 5, 1], decay=0.75)
+    check(got, x, 0.1, dtype)
+
+
+def test_a_prompt_with_no_scores_yet_and_scores_that_are_not_numbers(cuda_lib):
+    x = make(7, [200, 50, 100], queries=[16, 5, 1])
+    scores = torch.full((3, 2, x["table"].shape[1] * 16), float("nan"))
+    scores[2] = 0.25  # row 2 has scores but for its newest token
+    run_scored(x, on_device(x), 0.1, scores, fresh=[200, 60, 1])
+    run_scored(x, on_device(x), 0.1, torch.full_like(scores, float("nan")), decay=0.0)
+
+
+def test_slots_given_twice_or_past_the_table_are_left(cuda_lib):
+    import ekv._lib as L
+    from ekv.runtime.attention import attend, attend_scored
+
+    x = make(8, [40, 50, 60, 70])
+    d = on_device(x)
+    scores = torch.rand(4, 2, x["table"].shape[1] * 16, device="cuda")
+    before = scores.clone()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    slots = torch.tensor([1, 1, 4, 2], dtype=torch.int32, device="cuda")
+    got = attend_scored(d["query"], d["cache"], d["table"], d["lens"], 0.1, scores, slots=slots, status=status)
+    want = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert int(status) == L.STATUS_BAD_SLOT
+    assert torch.equal(scores[[0, 1, 3]], before[[0, 1, 3]]) and not torch.equal(scores[2], before[2])
+
+
+# ---- faults in the tables, strides, streams, graphs ------------------------------------------------------
+
+
+def test_bad_table_entries_are_skipped(cuda_lib):
+    import ekv._lib as L
+    from ekv.runtime.attention import attend
+
+    x = make(9, [100, 48, 16, 500])
+    ok = np.ones(tuple(x["table"].shape), dtype=bool)
+    for r, b, bad in [(0, 2, -1), (1, 0, 10**9), (2, 0, x["cache"].shape[0]), (3, 31, -7)]:
+        x["table"][r, b], ok[r, b] = bad, False
+    x["table"][1, 3:] = -5  # behind the row: never read
+    d = on_device(x)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, status=status)
+    check(got, x, 0.1, torch.bfloat16, pool_ok=ok, start=False)
+    assert int(status) == L.STATUS_BAD_BLOCK_ID
+
+
+def test_lengths_past_the_table_and_queries_outside_the_batch(cuda_lib):
+    import ekv._lib as L
+    from ekv.runtime.attention import attend
+
+    x = make(10, [64, 64, 64])
+    d = on_device(x)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([1000, 64, -5], dtype=torch.int32, device="cuda")
+    got = attend(d["query"], d["cache"], d["table"], lens, 0.1, status=status)
+    x["lens"] = torch.tensor([64, 64, 0], dtype=torch.int32)
+    check(got, x, 0.1, torch.bfloat16, start=False)
+    assert int(status) == L.STATUS_LEN_OVER_WIDTH
+    status.zero_()
+    out, lse = torch.full_like(got[0], 7.0), torch.full_like(got[1], 7.0)
+    start = torch.tensor([0, 1, 9, 3], dtype=torch.int32, device="cuda")
+    attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=start, out=out, lse=lse, status=status)
+    assert int(status) == L.STATUS_BAD_QROW
+    assert torch.equal(out[0], got[0][0]) and torch.all(out[1:] == 7.0) and torch.all(lse[1:] == 7.0)
+
+
+def test_values_behind_a_row_may_be_anything(cuda_lib):
+    from ekv.runtime.attention import attend
+
+    x = make(11, [70, 5, 16], dtype=torch.float16)
+    for r, n in enumerate([70, 5, 16]):
+        if n % 16:
+            x["cache"][x["table"][r, n // 16], :, n % 16:] = float("nan")
+            x["cache"][x["table"][r, n // 16], 1, 15] = float("inf")
+    d = on_device(x)
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1), x, 0.1, torch.float16, start=False)
+
+
+def test_strided_tensors_and_a_wider_table(cuda_lib):
+    from ekv.runtime.attention import attend
+
+    x = make(12, [90, 33], q_heads=4, kv_heads=2)
+    d = on_device(x)
+    want = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1)
+    q = torch.zeros(2, 6, 256, dtype=torch.bfloat16, device="cuda")[:, 1:5, 128:]
+    q.copy_(d["query"])
+    blocks, _, block, heads, dim = d["cache"].shape
+    cache = torch.zeros(blocks, block, heads, 2, dim, dtype=torch.bfloat16, device="cuda").permute(0, 3, 1, 2, 4)
+    cache.copy_(d["cache"])
+    table = torch.full((2, 50), -1, dtype=torch.int32, device="cuda")
+    table[:, : d["table"].shape[1]] = d["table"]
+    out = torch.zeros(2, 4, 256, dtype=torch.bfloat16, device="cuda")[:, :, :128]
+    got = attend(q, cache, table, d["lens"], 0.1, out=out)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_another_stream_and_a_replayed_graph(cuda_lib):
+    from ekv.runtime.attention import attend, attend_scored
+
+    x = make(13, [300, 64, 129, 1000], groups=[(0, 4, 4)])
+    d = on_device(x)
+    want = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, prefix_blocks=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, prefix_blocks=4)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    scores = torch.zeros(4, 2, x["table"].shape[1] * 16, device="cuda")
+    lens = d["lens"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = attend(d["query"], d["cache"], d["table"], lens, 0.1, prefix_blocks=4)
+        b = attend_scored(d["query"], d["cache"], d["table"], lens, 0.1, scores)
+    graph.replay()
+    assert torch.equal(a[0], want[0]) and torch.equal(a[1], want[1])
+    lens.copy_(torch.tensor([299, 70, 1, 0], dtype=torch.int32))  # the same graph, another batch
+    scores.zero_()
+    graph.replay()
+    x["lens"] = lens.cpu()
+    check(a, x, 0.1, torch.bfloat16, start=False)
+    check(b, x, 0.1, torch.bfloat16, start=False)
+    assert abs(float(scores[:3].sum()) - 3 * 8) < 1e-3  # each query head's weights sum to one
+
+
+def test_two_streams_at_once(cuda_lib):
+    from ekv.runtime.attention import attend
+
+    x, y = make(14, [4000] * 8, groups=[(0, 8, 100)]), make(15, [3000, 17] * 4)
+    dx, dy = on_device(x), on_device(y)
+    want = [attend(dx["query"], dx["cache"], dx["table"], dx["lens"], 0.1, prefix_blocks=100),
+            attend(dy["query"], dy["cache"], dy["table"], dy["lens"], 0.1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i in range(10):
+        with torch.cuda.stream(streams[0]):
+            got.append((0, attend(dx["query"], dx["cache"], dx["table"], dx["lens"], 0.1, prefix_blocks=100)))
+        with torch.cuda.stream(streams[1]):
+            got.append((1, attend(dy["query"], dy["cache"], dy["table"], dy["lens"], 0.1)))
+    torch.cuda.synchronize()
+    for k, (out, lse) in got:
+        assert torch.equal(out, want[k][0]) and torch.equal(lse, want[k][1])
+
+
+def test_a_row_that_is_shorter_than_its_groups_prefix(cuda_lib):
+    from ekv.runtime.attention import attend
+
+    x = make(16, [30, 0, 200, 97], groups=[(0, 4, 6)])
+    d = on_device(x)
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, prefix_blocks=6), x, 0.1, torch.bfloat16, start=False)
+
+
+def test_a_view_of_a_row_attends_to_its_blocks_alone(cuda_lib):
+    from ekv.runtime.attention import attend
+    from ekv.runtime.block_view import compact_block_table
+
+    x = make(17, [160, 90], block=16)
+    keep = torch.tensor(np.random.default_rng(0).random((2, x["table"].shape[1])) < 0.5)
+    d = on_device(x)
+    view, view_lens = compact_block_table(d["table"], d["lens"], keep.cuda(), 16)
+    got = attend(d["query"], d["cache"], view, view_lens, 0.1)
+    x["table"], x["lens"] = view.cpu(), view_lens.cpu()
+    check(got, x, 0.1, torch.bfloat16, start=False)
