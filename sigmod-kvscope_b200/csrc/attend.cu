@@ -535,31 +535,29 @@ int pick_mt(int64_t tokens, int units, int G) {
 }
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
-int launch_attend(const AttendParams& p, int sms, cudaStream_t s) {
+int launch_attend(const AttendParams& p, int device, int sms, cudaStream_t s) {
   const int units = PREFIX ? p.groups : p.rows;
   const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16 + plan_bytes(units, PREFIX);
   auto kernel = attend_kernel<T, D, WM, WN, PREFIX>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return check_launch("cudaFuncSetAttribute(attend_kernel)");
+  static LaunchCache cache;
   int resident = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem) != cudaSuccess)
-    return check_launch("cudaOccupancyMaxActiveBlocksPerMultiprocessor(attend_kernel)");
-  if (resident < 1) return fail(EKV_ENOTSUP, "the attention kernel does not fit this device");
+  const int rc = prepare_launch(cache, kernel, "attend_kernel", device, kThreads, smem, &resident);
+  if (rc != EKV_OK) return rc;
   launch_chained(kernel, dim3(min(sms * resident, p.max_ctas)), dim3(kThreads), smem, s, p);
   return check_launch("attend_kernel");
 }
 
 template <typename T, int D, bool PREFIX>
-int launch_phase(const AttendParams& p, int sms, cudaStream_t s) {
+int launch_phase(const AttendParams& p, int device, int sms, cudaStream_t s) {
   switch (p.mt_rows) {
-    case 16: return launch_attend<T, D, 1, 4, PREFIX>(p, sms, s);
-    case 32: return launch_attend<T, D, 2, 2, PREFIX>(p, sms, s);
-    default: return launch_attend<T, D, 4, 1, PREFIX>(p, sms, s);
+    case 16: return launch_attend<T, D, 1, 4, PREFIX>(p, device, sms, s);
+    case 32: return launch_attend<T, D, 2, 2, PREFIX>(p, device, sms, s);
+    default: return launch_attend<T, D, 4, 1, PREFIX>(p, device, sms, s);
   }
 }
 
 template <typename T, int D>
-int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, int sms, cudaStream_t s) {
+int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, int device, int sms, cudaStream_t s) {
   CombineParams c{};
   const int phases = p.groups > 0 ? 2 : 1;
   for (int k = phases - 1; k >= 0; --k) {  // the prefixes first
@@ -568,7 +566,7 @@ int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, 
     p.parts = reinterpret_cast<float*>(ws + w.parts[k]);
     p.whole = reinterpret_cast<float*>(ws + w.whole[k]);
     (k == 0 ? c.own : c.prefix) = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k]};
-    const int rc = k == 1 ? launch_phase<T, D, true>(p, sms, s) : launch_phase<T, D, false>(p, sms, s);
+    const int rc = k == 1 ? launch_phase<T, D, true>(p, device, sms, s) : launch_phase<T, D, false>(p, device, sms, s);
     if (rc != EKV_OK) return rc;
   }
   c.p = p;
@@ -624,7 +622,7 @@ struct AttendCall {
   Workspace w;
   int mt[2];
   uint8_t* ws;
-  int sms;
+  int device, sms;
 };
 
 // The checks of ekv_attend and ekv_attend_scored; fills the call.
@@ -673,12 +671,9 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, kAttendMaxCtas, c.mt);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
-  int device = 0, sms = 0;
-  int rc = current_device(&device);
+  int rc = current_device(&c.device);
   if (rc != EKV_OK) return rc;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return check_launch("cudaDeviceGetAttribute");
-  c.sms = sms;
+  if ((rc = sm_count(c.device, &c.sms)) != EKV_OK) return rc;
   c.ws = static_cast<uint8_t*>(workspace);
   AttendParams& p = c.p;
   p.q = q; p.q_s0 = q_stride_token; p.q_s1 = q_stride_head;
@@ -695,10 +690,10 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
 
 int run(const AttendCall& c, int head_dim, int dtype, cudaStream_t s) {
   if (dtype == EKV_DTYPE_BF16)
-    return head_dim == 128 ? attend<__nv_bfloat16, 128>(c.p, c.w, c.mt, c.ws, c.sms, s)
-                           : attend<__nv_bfloat16, 64>(c.p, c.w, c.mt, c.ws, c.sms, s);
-  return head_dim == 128 ? attend<__half, 128>(c.p, c.w, c.mt, c.ws, c.sms, s)
-                         : attend<__half, 64>(c.p, c.w, c.mt, c.ws, c.sms, s);
+    return head_dim == 128 ? attend<__nv_bfloat16, 128>(c.p, c.w, c.mt, c.ws, c.device, c.sms, s)
+                           : attend<__nv_bfloat16, 64>(c.p, c.w, c.mt, c.ws, c.device, c.sms, s);
+  return head_dim == 128 ? attend<__half, 128>(c.p, c.w, c.mt, c.ws, c.device, c.sms, s)
+                         : attend<__half, 64>(c.p, c.w, c.mt, c.ws, c.device, c.sms, s);
 }
 
 }  // namespace
@@ -753,5 +748,5 @@ extern "C" int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t 
   rc = run(c, head_dim, dtype, s);
   if (rc != EKV_OK) return rc;
   return launch_score_kernel(c.p, head_dim, dtype, scores, score_stride_slot, score_stride_head, slots, fresh, n_slots,
-                             decay, c.sms, s);
+                             decay, c.device, c.sms, s);
 }

@@ -16,6 +16,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <mutex>
+
 #include "ekv_common.cuh"
 
 namespace ekv {
@@ -296,12 +298,50 @@ constexpr float kLn2 = 0.69314718055994531f;
 
 // ---- host ---------------------------------------------------------------------------------------------------
 
+// The SMs of a device, asked once.
+inline int sm_count(int device, int* sms) {
+  static int known[kMaxDevices] = {};
+  if (known[device] == 0 &&
+      cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return check_launch("cudaDeviceGetAttribute");
+  *sms = known[device];
+  return EKV_OK;
+}
+
+// What a kernel of one instantiation was last set up for on each device: the attribute and occupancy calls cost
+// microseconds, and only a batch of another number of rows changes the shared memory it asks for.
+struct LaunchCache {
+  std::mutex lock;
+  size_t smem[kMaxDevices] = {};  // the most shared memory allowed so far
+  size_t asked[kMaxDevices] = {};  // the size `resident` was found for
+  int resident[kMaxDevices] = {};
+};
+
+template <typename Kernel>
+int prepare_launch(LaunchCache& cache, Kernel kernel, const char* name, int device, int threads, size_t smem, int* resident) {
+  std::lock_guard<std::mutex> hold(cache.lock);
+  if (smem > cache.smem[device]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return check_launch(name);
+    cache.smem[device] = smem;
+  }
+  if (cache.asked[device] != smem) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) return check_launch(name);
+    if (n < 1) return fail(EKV_ENOTSUP, "%s does not fit this device", name);
+    cache.asked[device] = smem;
+    cache.resident[device] = n;
+  }
+  *resident = cache.resident[device];
+  return EKV_OK;
+}
+
 // Encodes p.kmap and p.vmap for a cache at `kv` ([blocks][2][block_size][heads][D], element strides).
 int encode_cache_maps(AttendParams& p, const void* kv, int64_t s_block, int64_t s_part, int64_t s_pos, int64_t s_head,
                       int dim, int dtype);
 
 // Adds each token's weight to its score after an attention launch that left a.lse (attend_scores.cu).
 int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,
-                        const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int sms, cudaStream_t s);
+                        const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int device, int sms, cudaStream_t s);
 
 }  // namespace ekv

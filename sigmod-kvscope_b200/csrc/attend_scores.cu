@@ -192,23 +192,25 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const __grid_constan
 }
 
 template <typename T, int D>
-int launch_scores(const ScoreParams& p, int sms, cudaStream_t s) {
+int launch_scores(const ScoreParams& p, int device, int sms, cudaStream_t s) {
   const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows, false);
   auto kernel = score_kernel<T, D>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return check_launch("cudaFuncSetAttribute(score_kernel)");
-  launch_chained(kernel, dim3(min(2 * sms, kAttendMaxCtas)), dim3(kThreads), smem, s, p);
+  static LaunchCache cache;
+  int resident = 0;
+  const int rc = prepare_launch(cache, kernel, "score_kernel", device, kThreads, smem, &resident);
+  if (rc != EKV_OK) return rc;
+  launch_chained(kernel, dim3(min(resident * sms, kAttendMaxCtas)), dim3(kThreads), smem, s, p);
   return check_launch("score_kernel");
 }
 
 }  // namespace
 
 int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,
-                        const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int sms, cudaStream_t s) {
+                        const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int device, int sms, cudaStream_t s) {
   const ScoreParams p{a, scores, s0, s1, slots, fresh, n_slots, decay};
   if (dtype == EKV_DTYPE_BF16)
-    return dim == 128 ? launch_scores<__nv_bfloat16, 128>(p, sms, s) : launch_scores<__nv_bfloat16, 64>(p, sms, s);
-  return dim == 128 ? launch_scores<__half, 128>(p, sms, s) : launch_scores<__half, 64>(p, sms, s);
+    return dim == 128 ? launch_scores<__nv_bfloat16, 128>(p, device, sms, s) : launch_scores<__nv_bfloat16, 64>(p, device, sms, s);
+  return dim == 128 ? launch_scores<__half, 128>(p, device, sms, s) : launch_scores<__half, 64>(p, device, sms, s);
 }
 
 }  // namespace ekv

@@ -188,3 +188,29 @@ def current_stream() -> int:
     import torch
 
     return torch.cuda.current_stream().cuda_stream
+
+
+class on_device:
+    """``with on_device(device) as stream``: the device is current, and ``stream`` its current stream's handle.
+
+    Switching and asking through torch's public calls costs more than a small kernel, so a call whose tensors are on
+    the current device, as nearly all are, does neither."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device) -> None:
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        import torch
+
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_) -> None:
+        if self.before != self.index:
+            import torch
+
+            torch.cuda.set_device(self.before)

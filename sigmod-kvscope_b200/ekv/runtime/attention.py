@@ -133,14 +133,14 @@ def attend(
         return out, lse
     lib = _lib.load()
     size = lib.ekv_attend_workspace_bytes(rows, tokens, groups, q_heads, kv_heads, dim)
-    with torch.cuda.device(device):
+    with _lib.on_device(device) as stream:
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         rc = lib.ekv_attend(
             query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
             kv_cache.stride(1), kv_cache.stride(2), kv_cache.stride(3), blocks, table.data_ptr(), table.stride(0),
             lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
             scale, groups, members, prefix, common, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-            workspace.data_ptr(), size, word, _lib.current_stream(),
+            workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_attend")
     return out, lse
@@ -202,7 +202,7 @@ def attend_scored(
         return out, lse
     lib = _lib.load()
     size = lib.ekv_attend_workspace_bytes(rows, tokens, 0, q_heads, kv_heads, dim)
-    with torch.cuda.device(device):
+    with _lib.on_device(device) as stream:
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         rc = lib.ekv_attend_scored(
             query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
@@ -210,7 +210,7 @@ def attend_scored(
             lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
             scale, scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[0], places, new, decay,
             out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), workspace.data_ptr(), size, word,
-            _lib.current_stream(),
+            stream,
         )
     _lib.check(rc, "ekv_attend_scored")
     return out, lse

@@ -63,11 +63,11 @@ def select_tokens(
     word = _status(status, device)
     if rows == 0:
         return kept, new_lens
-    with torch.cuda.device(device):
+    with _lib.on_device(device) as stream:
         rc = _lib.load().ekv_select_tokens(
             scores.data_ptr(), scores.stride(0), scores.stride(1), n_slots, capacity, places, length, counts,
             max(min(count, 0x7FFFFFFF), -1), min(first_tokens, capacity), min(recent_tokens, capacity), rows, heads,
-            kept.data_ptr(), kept.stride(0), kept.stride(1), new, word, _lib.current_stream(),
+            kept.data_ptr(), kept.stride(0), kept.stride(1), new, word, stream,
         )
     _lib.check(rc, "ekv_select_tokens")
     return kept, new_lens
@@ -124,7 +124,7 @@ def compact_tokens(
     lib = _lib.load()
     size = lib.ekv_compact_tokens_workspace_bytes(rows, heads, blocks)
     item = kv_cache.element_size()
-    with torch.cuda.device(device):
+    with _lib.on_device(device) as stream:
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         rc = lib.ekv_compact_tokens(
             kv_cache.data_ptr(), kv_cache.stride(0) * item, kv_cache.stride(1) * item, kv_cache.stride(2) * item,
@@ -132,6 +132,6 @@ def compact_tokens(
             block_size, kept.data_ptr(), kept.stride(0), kept.stride(1), kept.shape[2], new,
             min(first_tokens, width * block_size), _lib.ptr(scores), scores.stride(0) if scores is not None else 0,
             scores.stride(1) if scores is not None else 0, scores.shape[0] if scores is not None else 0, places,
-            workspace.data_ptr(), size, word, _lib.current_stream(),
+            workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_compact_tokens")
