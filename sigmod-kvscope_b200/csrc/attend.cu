@@ -14,6 +14,8 @@
 // fragments in registers for a whole item, probabilities rounded to the cache's type (the products' operands
 // have to be of one type) and multiplied with the values in the same registers; sums stay in float32 from the
 // unrounded probabilities. The WN warps join through shared memory at an item's end.
+#include <type_traits>
+
 #include "attend.cuh"
 
 namespace ekv {
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       limit[j] = 0x7fffffff;
       if (real) {
         const int r = PREFIX ? row_of_token(p, rows, token) : it.unit;
-        limit[j] = r < 0 ? 0 : token_limit(p, r, token);
+        limit[j] = r < 0 ? 0 : token_limit<PREFIX>(p, r, token);
       }
       const T* src = static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 +
                      (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 2 * pair;
@@ -407,7 +409,7 @@ struct PhaseOut {
   const int32_t* cum;
   const float* parts;
   const float* whole;
-  int units, MT;
+  int units, MT, max_ctas;
 };
 
 struct CombineParams {
@@ -417,18 +419,18 @@ struct CombineParams {
 
 constexpr int kCombineThreads = 128;
 
-// The parts of one (query token, query head) in one phase: CTAs [c0, c1], or the one finished item (whole).
+// The parts of one (query token, query head) in one phase: those of CTAs [c0, c1], or the one finished item. A wide
+// launch leaves an item of at most kWideRows / 2 query rows in two halves, over alternate tiles.
 struct PartList {
-  const float* o;   // part i: o + i * stride (the first one elsewhere: o_first)
-  const float* ml;
+  const float *o, *ml;
   int count;
-  int64_t first, rest;  // index of the first part's row, and of the second's (the others follow 2 MT apart)
-  int64_t step;
+  int halves;
+  int64_t first, rest, step, half;  // rows of the first CTA's part, of the second's, from there on, and of the other half
 };
 
 __device__ __forceinline__ PartList list_parts(const AttendParams& p, const PhaseOut& ph, int unit, int nq, int m, int head,
                                                int token, int qhead, int D) {
-  PartList out{nullptr, nullptr, 0, 0, 0, 0};
+  PartList out{nullptr, nullptr, 0, 1, 0, 0, 0, 0};
   const int W = ph.cum[ph.units], n = ph.cum[ph.units + 1];
   const int mts = (nq * p.G + ph.MT - 1) / ph.MT;
   const int span = ph.cum[unit + 1] - ph.cum[unit];
@@ -436,24 +438,32 @@ __device__ __forceinline__ PartList list_parts(const AttendParams& p, const Phas
   const int tiles = span / (mts * p.heads), mt = m / ph.MT;
   const int a = ph.cum[unit] + (head * mts + mt) * tiles, b = a + tiles;
   const int c0 = cta_of(a, W, n), c1 = cta_of(b - 1, W, n);
+  const int64_t all = (int64_t)p.tokens * p.q_heads;
+  if (ph.MT == kWideRows && nq * p.G - mt * ph.MT <= kWideRows / 2) out.halves = 2;
   if (c0 == c1) {
     out.o = ph.whole;
-    out.ml = ph.whole + (int64_t)p.tokens * p.q_heads * D;
+    out.ml = ph.whole + all * (ph.MT == kWideRows ? 2 : 1) * D;
     out.count = 1;
     out.first = (int64_t)token * p.q_heads + qhead;
-    return out;
+    out.half = all;
+  } else {
+    out.o = ph.parts;
+    out.ml = ph.parts + (int64_t)2 * ph.max_ctas * ph.MT * D;
+    out.count = c1 - c0 + 1;
+    const int mi = m - mt * ph.MT;
+    out.first = (int64_t)(2 * c0 + 1) * ph.MT + mi;
+    out.rest = (int64_t)(2 * c0 + 2) * ph.MT + mi;
+    out.step = 2 * ph.MT;
+    out.half = kWideRows / 2;
   }
-  out.o = ph.parts;
-  out.ml = ph.parts + (int64_t)2 * p.max_ctas * ph.MT * D;
-  out.count = c1 - c0 + 1;
-  const int mi = m - mt * ph.MT;
-  out.first = (int64_t)(2 * c0 + 1) * ph.MT + mi;
-  out.rest = (int64_t)(2 * c0 + 2) * ph.MT + mi;
-  out.step = 2 * ph.MT;
+  out.count *= out.halves;
   return out;
 }
 
-__device__ __forceinline__ int64_t part_row(const PartList& l, int i) { return i == 0 ? l.first : l.rest + (i - 1) * l.step; }
+__device__ __forceinline__ int64_t part_row(const PartList& l, int i) {
+  const int c = l.halves == 2 ? i >> 1 : i;
+  return (c == 0 ? l.first : l.rest + (c - 1) * l.step) + (l.halves == 2 && (i & 1) ? l.half : 0);
+}
 
 // A warp per (query token, query head); every lane holds D / 32 dims. The parts are added in order.
 template <typename T, int D>
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
   if (group >= 0) {
     const QueryRange gq = group_queries(p, group_rows(p, group));
     lists[1] = list_parts(p, c.prefix, group, gq.nq, (token - gq.q0) * p.G + g, head, token, qhead, D);
-  } else if (lists[0].count == 1 && p.groups == 0) {
+  } else if (lists[0].count == 1 && p.groups == 0 && c.own.MT != kWideRows) {
     return;  // the attention kernel wrote it
   }
   float m = -INFINITY;
@@ -512,17 +522,20 @@ struct Workspace {
   size_t cum[2], parts[2], whole[2], total;
 };
 
+int max_ctas(int mt) { return mt == kWideRows ? kWideMaxCtas : kAttendMaxCtas; }
+
 // Phase 0: the rows' own tokens; phase 1: the shared prefixes.
-Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, int ctas, const int (&mt)[2]) {
+Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, const int (&mt)[2]) {
   Workspace w{};
   size_t at = 0;
   for (int k = 0; k < (groups > 0 ? 2 : 1); ++k) {
     w.cum[k] = at;
     at += round_up(((size_t)(k == 0 ? rows : groups) + 2) * 4, 256);
     w.parts[k] = at;
-    at += round_up((size_t)2 * ctas * mt[k] * (dim + 2) * 4, 256);
+    at += round_up((size_t)2 * max_ctas(mt[k]) * mt[k] * (dim + 2) * 4, 256);
     w.whole[k] = at;
-    if (groups > 0) at += round_up((size_t)tokens * q_heads * (dim + 2) * 4, 256);
+    if (groups > 0 || mt[k] == kWideRows)
+      at += round_up((size_t)tokens * q_heads * (dim + 2) * 4 * (mt[k] == kWideRows ? 2 : 1), 256);
   }
   w.total = at;
   return w;
@@ -531,7 +544,7 @@ Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int di
 // Query rows of an M tile: the smallest variant that holds a unit's average in one tile.
 int pick_mt(int64_t tokens, int units, int G) {
   const int64_t m = (tokens + units - 1) / units * G;
-  return m <= 16 ? 16 : m <= 32 ? 32 : 64;
+  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : kWideRows;
 }
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
@@ -565,8 +578,11 @@ int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, 
     p.cum = reinterpret_cast<int32_t*>(ws + w.cum[k]);
     p.parts = reinterpret_cast<float*>(ws + w.parts[k]);
     p.whole = reinterpret_cast<float*>(ws + w.whole[k]);
-    (k == 0 ? c.own : c.prefix) = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k]};
-    const int rc = k == 1 ? launch_phase<T, D, true>(p, device, sms, s) : launch_phase<T, D, false>(p, device, sms, s);
+    p.max_ctas = max_ctas(mt[k]);
+    (k == 0 ? c.own : c.prefix) = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k], p.max_ctas};
+    const int type = std::is_same<T, __half>::value ? EKV_DTYPE_F16 : EKV_DTYPE_BF16;
+    const int rc = mt[k] == kWideRows ? (k == 1 ? launch_wide<true>(p, D, type, device, sms, s) : launch_wide<false>(p, D, type, device, sms, s))
+                   : k == 1 ? launch_phase<T, D, true>(p, device, sms, s) : launch_phase<T, D, false>(p, device, sms, s);
     if (rc != EKV_OK) return rc;
   }
   c.p = p;
@@ -668,7 +684,7 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   if ((int64_t)tokens * q_heads > 0x7fffffffll / 4) return fail(EKV_ENOTSUP, "more than 2^29 query rows");
   c.mt[0] = pick_mt(tokens, rows, G);
   c.mt[1] = groups > 0 ? pick_mt(tokens, groups, G) : 0;
-  const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, kAttendMaxCtas, c.mt);
+  const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, c.mt);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
   int rc = current_device(&c.device);
@@ -684,7 +700,7 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   p.block_shift = block_size == 8 ? 3 : block_size == 16 ? 4 : block_size == 32 ? 5 : 6;
   p.heads = kv_heads; p.G = G; p.q_heads = q_heads; p.pool_blocks = pool_blocks; p.tokens = tokens;
   p.groups = groups; p.group_start = group_start; p.prefix_blocks = prefix_blocks; p.prefix_common = prefix_common;
-  p.status = status; p.max_ctas = kAttendMaxCtas;
+  p.status = status;
   return encode_cache_maps(p, kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, head_dim, dtype);
 }
 
@@ -702,7 +718,7 @@ extern "C" size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, i
   if (rows <= 0 || tokens <= 0 || groups < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
   const int G = q_heads / kv_heads;
   const int mt[2] = {pick_mt(tokens, rows, G), groups > 0 ? pick_mt(tokens, groups, G) : 0};
-  return workspace_layout(rows, tokens, groups, q_heads, head_dim, kAttendMaxCtas, mt).total;
+  return workspace_layout(rows, tokens, groups, q_heads, head_dim, mt).total;
 }
 
 extern "C" int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,

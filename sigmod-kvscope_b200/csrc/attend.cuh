@@ -49,7 +49,8 @@ struct AttendParams {
   // the workspace, of the launch's phase and (for the combine kernel) of both
   int32_t* cum;   // [units + 1] running tile counts, then the number of CTAs that share them
   float* parts;   // [2 CTAs][MT][D], and behind them their [2 CTAs][MT][2] maxima and sums
-  float* whole;   // [tokens * q_heads][D] and [tokens * q_heads][2]: finished items when another phase joins
+  float* whole;   // [tokens * q_heads][D] and [tokens * q_heads][2]: finished items when another phase joins (twice that
+                  // in a wide launch, whose items of few query rows end in two halves)
   int mt_rows;    // query rows of an M tile
   int max_ctas;
 };
@@ -112,10 +113,11 @@ __device__ __forceinline__ int group_of(const AttendParams& p, int r) {
   return r >= rr.a && r < rr.b ? lo : -1;
 }
 
-// Tokens that row r leaves to its group's prefix launch.
+// Tokens that row r leaves to its group's prefix launch: whole blocks that it has, so that the launch reads no
+// position that no row of the group holds.
 __device__ __forceinline__ int row_prefix(const AttendParams& p, int r) {
   const int g = group_of(p, r);
-  return g < 0 ? 0 : group_prefix(p, g);
+  return g < 0 ? 0 : min(group_prefix(p, g), row_tokens(p, r, false) >> p.block_shift << p.block_shift);
 }
 
 // The query tokens of a group: those of its rows, which follow one another.
@@ -143,16 +145,18 @@ __device__ __forceinline__ int row_of_token(const AttendParams& p, RowRange rr, 
   return t >= q.q0 && t < q.q0 + q.nq ? lo : -1;
 }
 
-// Positions below this are visible to query token t of row r.
+// Positions below this are visible to query token t of row r (in a prefix launch: of those the row left to it).
+template <bool PREFIX>
 __device__ __forceinline__ int token_limit(const AttendParams& p, int r, int t) {
   const QueryRange q = row_queries(p, r, false);
-  return row_tokens(p, r, false) - q.nq + (t - q.q0) + 1;
+  const int limit = row_tokens(p, r, false) - q.nq + (t - q.q0) + 1;
+  return PREFIX ? min(limit, row_prefix(p, r)) : limit;
 }
 
 // ---- the plan ----------------------------------------------------------------------------------------
 
 // In shared memory: cum[units + 1], the running tile counts, and for a prefix launch lead[units], the longest
-// row of each group (its length << 32 | ~row), whose table is read.
+// row of each group (its shared tokens << 32 | ~row), whose table is read.
 struct Plan {
   int* cum;
   unsigned long long* lead;
@@ -180,8 +184,9 @@ struct Unit {
   QueryRange q;
   int row, from, to;
   __device__ __forceinline__ int m_tiles(const AttendParams& p, int MT) const { return (q.nq * p.G + MT - 1) / MT; }
+  template <int TOKENS>
   __device__ __forceinline__ int tiles() const {
-    return to > from && q.nq > 0 ? (to - from + kTile - 1) / kTile : 0;
+    return to > from && q.nq > 0 ? (to - from + TOKENS - 1) / TOKENS : 0;
   }
 };
 
@@ -193,7 +198,7 @@ __device__ __forceinline__ Unit unit_at(const AttendParams& p, const Plan& plan,
     un.q = group_queries(p, rr);
     un.row = lead_row(plan.lead[u]);
     un.from = 0;
-    un.to = min(group_prefix(p, u), lead_len(plan.lead[u]));  // 0 for a group with no rows
+    un.to = lead_len(plan.lead[u]);  // 0 for a group with no rows
   } else {
     un.q = row_queries(p, u, report);
     un.row = u;
@@ -204,7 +209,7 @@ __device__ __forceinline__ Unit unit_at(const AttendParams& p, const Plan& plan,
 }
 
 // Fills the plan with every thread of the CTA (THREADS of them); `scratch` holds THREADS / 32 + 1 ints.
-template <bool PREFIX, int THREADS>
+template <bool PREFIX, int THREADS, int TOKENS = kTile>
 __device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& plan, int MT, int* scratch) {
   const bool report = blockIdx.x == 0;
   if (PREFIX) {
@@ -213,7 +218,7 @@ __device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& pla
     for (int r = threadIdx.x; r < p.rows; r += THREADS) {
       const int g = group_of(p, r);
       if (g >= 0)
-        atomicMax(plan.lead + g, (unsigned long long)(uint32_t)row_tokens(p, r, false) << 32 | (uint32_t)~(uint32_t)r);
+        atomicMax(plan.lead + g, (unsigned long long)(uint32_t)row_prefix(p, r) << 32 | (uint32_t)~(uint32_t)r);
     }
     __syncthreads();
   }
@@ -223,7 +228,7 @@ __device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& pla
     int n = 0;
     if (u < plan.units) {
       const Unit un = unit_at<PREFIX>(p, plan, u, report);
-      n = un.tiles() * p.heads * un.m_tiles(p, MT);
+      n = un.template tiles<TOKENS>() * p.heads * un.m_tiles(p, MT);
     }
     int total = 0;
     const int before = block_exclusive_scan<THREADS>(n, scratch, &total);
@@ -245,7 +250,7 @@ struct Item {
   int unit, head, mt, first, last, tiles;
 };
 
-template <bool PREFIX>
+template <bool PREFIX, int TOKENS = kTile>
 __device__ __forceinline__ Item item_at(const AttendParams& p, const Plan& plan, int MT, int t, int end) {
   int lo = 0, hi = plan.units;  // the last unit that starts at or before t (units without tiles never hold one)
   while (hi - lo > 1) {
@@ -255,7 +260,7 @@ __device__ __forceinline__ Item item_at(const AttendParams& p, const Plan& plan,
   Item it;
   it.unit = lo;
   it.un = unit_at<PREFIX>(p, plan, lo, false);
-  it.tiles = it.un.tiles();
+  it.tiles = it.un.template tiles<TOKENS>();
   const int mts = it.un.m_tiles(p, MT);
   const int rem = t - plan.cum[lo], hm = rem / it.tiles;
   it.head = hm / mts;
@@ -339,6 +344,12 @@ int prepare_launch(LaunchCache& cache, Kernel kernel, const char* name, int devi
 // Encodes p.kmap and p.vmap for a cache at `kv` ([blocks][2][block_size][heads][D], element strides).
 int encode_cache_maps(AttendParams& p, const void* kv, int64_t s_block, int64_t s_part, int64_t s_pos, int64_t s_head,
                       int dim, int dtype);
+
+// An attention launch on the tcgen05 tensor cores (attend_mma5.cu): M tiles of kWideRows query rows, one CTA an SM.
+constexpr int kWideRows = 256;
+constexpr int kWideMaxCtas = 160;
+template <bool PREFIX>
+int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, cudaStream_t s);
 
 // Adds each token's weight to its score after an attention launch that left a.lse (attend_scores.cu).
 int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,

@@ -1,0 +1,537 @@
+// The attention kernel for units of many query rows, on the tcgen05 tensor cores: the same mathematics as
+// attend_kernel (attend.cu), with accumulators in tensor memory.
+//
+// A CTA an SM. Its M tile is 256 query rows in two subtiles of 128, one for each of two softmax warpgroups (a
+// thread a row), and both meet the same 128-token tiles of keys and values in shared memory: at 512 bytes a token
+// and head, one such tile feeds 4 x 128^3 multiply-adds. An item of at most 128 query rows gives both
+// warpgroups the same rows and alternate tiles, so the tensor cores still have one warpgroup's scores to work on while
+// the other takes its exponentials; its two halves join in the combine kernel.
+//   copy warp: block ids, then the TMA copies of K0 K1 V0 K2 V1 ... into a ring of 128-token slots (a block that is not
+//     there is copied from past the pool, which the TMA engine reads as zeros).
+//   mma warp: S = Q K^T into tensor memory, then O += P V with P from tensor memory; one thread issues. S of the next
+//     tile follows O of this one, so a score's arrival also says that the output below it is at rest.
+//   softmax warpgroups: a row's 128 scores 32 at a time, once for their maximum and once for their exponentials (all 128
+//     in registers spilled); the running maximum is only raised when it grew by more than 2^8, so the output in tensor
+//     memory is rescaled a few times a row, by the same threads; probabilities go back to tensor memory over the scores
+//     already read, rounded to the values' type.
+#include <type_traits>
+
+#include "attend.cuh"
+
+namespace ekv {
+
+namespace {
+
+constexpr int kTokens = 128;  // of a tile
+constexpr int kSub = 128;     // query rows of a subtile
+constexpr int kThreads = 320;
+constexpr int kCopyWarp = 8, kMmaWarp = 9;
+constexpr int kColumns = 512;  // of tensor memory: S of both subtiles, then O of both
+
+template <int D>
+struct Wide {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kHalf = kTokens * 128;         // bytes of a 64-dim half of 128 rows
+  static constexpr int kSlot = kHalves * kHalf;       // of a tile's keys, or values, or a subtile's queries
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr int kRing = kSlots * kSlot;
+};
+
+template <int D>
+struct WideTail {
+  uint64_t full[Wide<D>::kSlots], empty[Wide<D>::kSlots];
+  uint64_t q_full[2], s_full[2], p_ready[2], o_full[2], o_free[2], drained;
+  uint32_t tmem;
+  int scratch[kThreads / 32 + 1];
+};
+
+// ---- tensor memory and descriptors ---------------------------------------------------------------------
+
+__device__ __forceinline__ void tmem_ld32(float* r, uint32_t addr) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
+      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
+      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+      : "memory");
+}
+
+// Waits for the loads; naming the values keeps their first use behind the wait.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(float (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// A shared-memory operand in the 128-byte swizzle: `lead` and `stride` are the byte distances between 64-element
+// groups of the major dimension and between groups of eight rows.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+// ---- the walk that all warps share ---------------------------------------------------------------------------
+
+// How an item's tiles fall to the two warpgroups: with one subtile of rows the even tiles to the first and the odd ones
+// to the second, otherwise all to both.
+struct Share {
+  bool single;
+  int tiles;  // of the item that this CTA covers
+  __device__ __forceinline__ int of(int w) const { return single ? (tiles + 1 - w) / 2 : tiles; }
+};
+
+__device__ __forceinline__ Share share_of(const AttendParams& p, const Item& it) {
+  const int rows = it.un.q.nq * p.G - it.mt * kWideRows;
+  return {rows <= kSub, it.last - it.first};
+}
+
+template <typename T, int D, bool PREFIX>
+__global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant__ AttendParams p) {
+  using R = Wide<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* queries = base;              // [2] subtiles
+  uint8_t* ring = base + 2 * R::kSlot;  // [kSlots]
+  WideTail<D>& tail = *reinterpret_cast<WideTail<D>*>(ring + R::kRing);
+  const Plan plan = plan_at(ring + R::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16, PREFIX ? p.groups : p.rows, PREFIX);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < R::kSlots; ++s) {
+      mbar_init(&tail.full[s], 1);
+      mbar_init(&tail.empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&tail.q_full[w], kSub);
+      mbar_init(&tail.s_full[w], 1);
+      mbar_init(&tail.p_ready[w], kSub);
+      mbar_init(&tail.o_full[w], 1);
+      mbar_init(&tail.o_free[w], kSub);
+    }
+    mbar_init(&tail.drained, 1);
+    fence_mbar_init();
+  }
+  chain_wait();
+  make_plan<PREFIX, kThreads, kTokens>(p, plan, kWideRows, tail.scratch);
+  const int W = plan.cum[plan.units];
+  const int n = sharing_ctas(W, gridDim.x);
+  if (blockIdx.x == 0) {
+    for (int u = threadIdx.x; u <= plan.units; u += kThreads) p.cum[u] = plan.cum[u];
+    if (threadIdx.x == 0) p.cum[plan.units + 1] = n;
+  }
+  chain_release();
+  if ((int)blockIdx.x >= n || W == 0) return;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem)), "r"(kColumns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tail.tmem;
+  const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
+  const int per_tile = kTokens >> p.block_shift;  // blocks of a tile
+  bool good = true;  // after a wait that gave up a role goes on without waiting, so that every role ends
+
+  if (warp == kCopyWarp) {
+    const uint64_t policy = l2_evict_first_policy();
+    const uint32_t block_bytes = (uint32_t)p.block_size * 128u;
+    int slot = 0, issued = 0;
+    uint32_t phase = 0;
+    for (int t = begin; t < end && good;) {
+      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
+      const int block0 = it.un.from >> p.block_shift, last_block = (it.un.to - 1) >> p.block_shift;
+      const int tiles = it.last - it.first;
+      auto copy = [&](int tile, bool values) {
+        if (issued >= R::kSlots) good = good && mbar_wait_bounded(&tail.empty[slot], phase ^ 1, p.status);
+        good = __all_sync(kFullMask, good);
+        if (!good) return;
+        if (lane == 0) mbar_arrive_expect_tx(&tail.full[slot], R::kSlot);
+        __syncwarp();
+        if (lane < per_tile) {
+          const int b = block0 + (it.first + tile) * per_tile + lane;
+          int id = b <= last_block ? ids[b] : -2;
+          if (id < 0 || (int64_t)id >= p.pool_blocks) {
+            if (b <= last_block) set_status(p.status, EKV_STATUS_BAD_BLOCK_ID);
+            id = (int)p.pool_blocks;  // past the tensor: zeros
+          }
+          const uint32_t at = smem_u32(ring) + slot * R::kSlot + lane * block_bytes;
+#pragma unroll
+          for (int h = 0; h < R::kHalves; ++h)
+            tensor_copy_4d(at + h * R::kHalf, values ? &p.vmap : &p.kmap, 64 * h, it.head, 0, id, &tail.full[slot], policy);
+        }
+        ++issued;
+        if (++slot == R::kSlots) slot = 0, phase ^= 1;
+      };
+      copy(0, false);
+      for (int tile = 0; tile < tiles; ++tile) {
+        if (tile + 1 < tiles) copy(tile + 1, false);
+        copy(tile, true);
+      }
+      t += tiles;
+    }
+    for (int s = 0; s < R::kSlots; ++s) {  // no CTA leaves with copies in flight
+      const int uses = issued > s ? (issued - s - 1) / R::kSlots + 1 : 0;
+      if (uses > 0) mbar_wait_bounded(&tail.full[s], (uses - 1) & 1, p.status);
+    }
+  } else if (warp == kMmaWarp) {
+    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t kShape = 1u << 4 | kType << 7 | kType << 10 | (uint32_t)(kSub >> 4) << 24;
+    constexpr uint32_t kScores = kShape | (uint32_t)(kTokens >> 3) << 17;
+    constexpr uint32_t kOutput = kShape | 1u << 16 | (uint32_t)(D >> 3) << 17;  // the values' tokens are their rows
+    const uint32_t q_at = smem_u32(queries), ring_at = smem_u32(ring);
+    int slot = 0;
+    uint32_t phase = 0;
+    uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, items[2] = {0, 0};
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (good) good = mbar_wait_bounded(bar, parity, p.status);
+      good = __all_sync(kFullMask, good);
+      tc_fence_after();
+    };
+    // the next ring slot, waited for
+    auto take = [&]() {
+      const int s = slot;
+      wait(&tail.full[s], phase);
+      if (++slot == R::kSlots) slot = 0, phase ^= 1;
+      return s;
+    };
+    auto scores = [&](int w, int s) {
+      if (lane != 0 || !good) return;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = (uint32_t)(k >> 2) * R::kHalf + (uint32_t)(k & 3) * 32;
+        mma_ss(tmem + w * 128, operand(q_at + w * R::kSlot + at, 16, 1024), operand(ring_at + s * R::kSlot + at, 16, 1024),
+               kScores, k > 0);
+      }
+    };
+    auto output = [&](int w, int s, bool add) {
+      if (lane != 0 || !good) return;
+#pragma unroll
+      for (int k = 0; k < kTokens / 16; ++k)
+        mma_ts(tmem + 256 + w * 128, tmem + w * 128 + 8 * k, operand(ring_at + s * R::kSlot + k * 2048, R::kHalf, 1024),
+               kOutput, add || k > 0);
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (lane == 0) tc_commit(bar);
+    };
+    // rows of a value tile behind the unit's last token hold whatever the block holds: cleared, since a probability
+    // of zero times that need not be zero
+    auto clear_tail = [&](const Item& it, int tile, int s) {
+      const int first = it.un.to - it.un.from - (it.first + tile) * kTokens;
+      const int last = min(kTokens, (first + p.block_size - 1) >> p.block_shift << p.block_shift);
+      if (first >= last) return;
+      for (int i = lane; i < (last - first) * (D / 8); i += 32) {
+        const int r = first + i / (D / 8), c = i % (D / 8);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring_at + s * R::kSlot + (c >> 3) * R::kHalf + r * 128 +
+                                                                     (((c & 7) ^ (r & 7)) << 4)),
+                     "r"(0)
+                     : "memory");
+      }
+      proxy_fence_smem();
+      __syncwarp();
+    };
+    for (int t = begin; t < end;) {
+      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const Share sh = share_of(p, it);
+      int ks = take();
+      if (sh.single) {
+        for (int w = 0; w < 2 && w < sh.tiles; ++w) {
+          if (w == 1) ks = take();
+          wait(&tail.q_full[w], q_uses[w]++ & 1);
+          scores(w, ks);
+          commit(&tail.s_full[w]);
+          commit(&tail.empty[ks]);
+          // the tiles of this walk come as K0 K1 V0 K2 V1 ...: V0 stands before K2
+        }
+        for (int j = 0; j < sh.tiles; ++j) {
+          const int w = j & 1;
+          if (j > 0 && j + 1 < sh.tiles) {  // K(j + 1), taken before V(j): its scores wait for this warpgroup's turn
+            ks = take();
+          }
+          const int vs = take();
+          clear_tail(it, j, vs);
+          // K(j + 1) belongs to the other warpgroup, whose P(j - 1) has been used: its scores can go first
+          if (j > 0 && j + 1 < sh.tiles) {
+            scores(w ^ 1, ks);
+            commit(&tail.s_full[w ^ 1]);
+            commit(&tail.empty[ks]);
+          }
+          wait(&tail.p_ready[w], p_uses[w]++ & 1);
+          if (j < 2 && items[w] > 0) wait(&tail.o_free[w], (items[w] - 1) & 1);
+          output(w, vs, j >= 2);
+          commit(&tail.empty[vs]);
+          if (j + 2 >= sh.tiles) commit(&tail.o_full[w]);
+        }
+      } else {
+        for (int w = 0; w < 2; ++w) {
+          wait(&tail.q_full[w], q_uses[w]++ & 1);
+          scores(w, ks);
+          commit(&tail.s_full[w]);
+        }
+        commit(&tail.empty[ks]);
+        for (int j = 0; j < sh.tiles; ++j) {
+          const bool more = j + 1 < sh.tiles;
+          if (more) ks = take();
+          const int vs = take();
+          clear_tail(it, j, vs);
+          for (int w = 0; w < 2; ++w) {
+            wait(&tail.p_ready[w], p_uses[w]++ & 1);
+            if (j == 0 && items[w] > 0) wait(&tail.o_free[w], (items[w] - 1) & 1);
+            output(w, vs, j > 0);
+            if (w == 1) commit(&tail.empty[vs]);
+            if (more) {
+              scores(w, ks);
+              commit(&tail.s_full[w]);
+            } else {
+              commit(&tail.o_full[w]);
+            }
+          }
+          if (more) commit(&tail.empty[ks]);
+        }
+      }
+      for (int w = 0; w < 2; ++w) items[w] += sh.of(w) > 0;
+      t += sh.tiles;
+    }
+    commit(&tail.drained);
+    mbar_wait_bounded(&tail.drained, 0, p.status);
+  } else {  // ---- the softmax warpgroups ---------------------------------------------------------------------
+    const int w = warp >> 2, row = threadIdx.x & (kSub - 1);
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
+    const uint32_t s_at = tmem + w * 128 + lanes, o_at = tmem + 256 + w * 128 + lanes;
+    uint32_t s_uses = 0, o_uses = 0;
+    const float grow = 8.f / p.scale_log2;
+    for (int t = begin; t < end;) {
+      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const Share sh = share_of(p, it);
+      const QueryRange uq = it.un.q;
+      const int mi = sh.single ? row : w * kSub + row, mrow = it.mt * kWideRows + mi;
+      const bool real = mrow < uq.nq * p.G;
+      const int token = uq.q0 + mrow / p.G, qhead = it.head * p.G + mrow % p.G;
+      float m = -INFINITY, l = 0.f;
+      if (sh.of(w) > 0) {
+        // this thread's query row, into the subtile's swizzled rows
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 + (int64_t)qhead * p.q_s1);
+        const uint32_t dst = smem_u32(queries) + w * R::kSlot + row * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = real ? src[c] : make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * R::kHalf + (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                       : "memory");
+        }
+        proxy_fence_smem();
+        mbar_arrive(&tail.q_full[w]);
+        int limit = 0x7fffffff;
+        if (real) {
+          const int r = PREFIX ? row_of_token(p, group_rows(p, it.unit), token) : it.unit;
+          limit = r < 0 ? 0 : token_limit<PREFIX>(p, r, token);
+        }
+        limit = min(limit, it.un.to);
+        const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
+        const int block0 = it.un.from >> p.block_shift, last_block = (it.un.to - 1) >> p.block_shift;
+        const int step = sh.single ? 2 : 1;
+        auto block_id = [&](int tile) {
+          const int b = block0 + tile * per_tile + lane;
+          return lane < per_tile && b <= last_block && tile < it.last ? ids[b] : 0;
+        };
+        int id = block_id(it.first + (sh.single ? w : 0));
+        for (int tile = it.first + (sh.single ? w : 0); tile < it.last; tile += step) {
+          const uint32_t missing = __ballot_sync(kFullMask, id < 0 || (int64_t)id >= p.pool_blocks);
+          id = block_id(tile + step);
+          if (good) good = mbar_wait_bounded(&tail.s_full[w], s_uses & 1, p.status);
+          ++s_uses;
+          tc_fence_after();
+          __syncwarp();
+          const int pos = it.un.from + tile * kTokens;
+          const bool masked = missing != 0 || __any_sync(kFullMask, pos + kTokens > limit);
+          float s[2][32];
+          // chunk c of the scores is waited for while chunk c + 1 is on its way
+          auto fetch = [&](int c) { tmem_ld32(s[c & 1], s_at + 32 * c); };
+          auto mask = [&](int c) {
+            if (!masked) return;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (pos + 32 * c + i >= limit || (missing >> ((32 * c + i) >> p.block_shift) & 1u)) s[c & 1][i] = -INFINITY;
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          fetch(0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld(s[c & 1]);
+            if (c < 3) fetch(c + 1);
+            mask(c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[c & 1][i]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool raise = top > m + grow;  // also a row's first scores: m is -inf
+          if (__any_sync(kFullMask, raise)) {
+            const float f = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * p.scale_log2)) : 1.f;
+            if (raise) m = top;
+            l *= f;
+            if (tile >= it.first + step) {  // the output holds earlier tiles
+#pragma unroll
+              for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tmem_ld32(o, o_at + c);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= f;
+                tmem_st32(o_at + c, reinterpret_cast<const uint32_t*>(o));
+              }
+              // waited for with the probabilities below
+            }
+          }
+          const float from = m == -INFINITY ? 0.f : m * p.scale_log2;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          fetch(0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld(s[c & 1]);
+            if (c < 3) fetch(c + 1);
+            mask(c);
+            uint32_t u[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float a = exp2_fast(fmaf(s[c & 1][2 * i], p.scale_log2, -from));
+              const float b = exp2_fast(fmaf(s[c & 1][2 * i + 1], p.scale_log2, -from));
+              sum[(2 * i) & 3] += a;
+              sum[(2 * i + 1) & 3] += b;
+              u[i] = pack2<T>(a, b);
+            }
+            tmem_st16(s_at + 16 * c, u);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&tail.p_ready[w]);
+        }
+        if (good) good = mbar_wait_bounded(&tail.o_full[w], o_uses & 1, p.status);
+        ++o_uses;
+        tc_fence_after();
+      }
+      const bool complete = it.first == 0 && it.last == it.tiles;
+      const int64_t all = (int64_t)p.tokens * p.q_heads;
+      float *dst, *ml;
+      if (complete) {
+        const int64_t at = (int64_t)token * p.q_heads + qhead + (sh.single && w == 1 ? all : 0);
+        dst = p.whole + at * D;
+        ml = p.whole + 2 * all * D + 2 * at;
+      } else {
+        const int64_t at = (int64_t)(2 * blockIdx.x + (it.first == 0 ? 1 : 0)) * kWideRows + w * kSub + row;
+        dst = p.parts + at * D;
+        ml = p.parts + (int64_t)2 * p.max_ctas * kWideRows * D + 2 * at;
+      }
+      if (real) *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
+      if (sh.of(w) > 0) {
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(o, o_at + c);
+          tmem_wait_ld(o);
+          if (real) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(dst + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          __syncwarp();
+        }
+        tc_fence_before();
+        mbar_arrive(&tail.o_free[w]);
+      }
+      t += sh.tiles;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
+}
+
+template <typename T, int D, bool PREFIX>
+int launch(const AttendParams& p, int device, int sms, cudaStream_t s) {
+  const int units = PREFIX ? p.groups : p.rows;
+  const size_t smem = 1024 + 2 * Wide<D>::kSlot + Wide<D>::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16 + plan_bytes(units, PREFIX);
+  auto kernel = wide_kernel<T, D, PREFIX>;
+  static LaunchCache cache;
+  int resident = 0;
+  const int rc = prepare_launch(cache, kernel, "wide_kernel", device, kThreads, smem, &resident);
+  if (rc != EKV_OK) return rc;
+  launch_chained(kernel, dim3(min(sms, p.max_ctas)), dim3(kThreads), smem, s, p);
+  return check_launch("wide_kernel");
+}
+
+}  // namespace
+
+template <bool PREFIX>
+int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, cudaStream_t s) {
+  if (dtype == EKV_DTYPE_BF16)
+    return dim == 128 ? launch<__nv_bfloat16, 128, PREFIX>(p, device, sms, s) : launch<__nv_bfloat16, 64, PREFIX>(p, device, sms, s);
+  return dim == 128 ? launch<__half, 128, PREFIX>(p, device, sms, s) : launch<__half, 64, PREFIX>(p, device, sms, s);
+}
+
+template int launch_wide<true>(const AttendParams&, int, int, int, int, cudaStream_t);
+template int launch_wide<false>(const AttendParams&, int, int, int, int, cudaStream_t);
+
+}  // namespace ekv

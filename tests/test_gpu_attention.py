@@ -113,6 +113,45 @@ def test_shared_prefixes(cuda_lib, dim, queries, groups):
         assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
 
 
+@pytest.mark.parametrize("dtype, dim, block", [(torch.bfloat16, 128, 16), (torch.float16, 64, 32), (torch.float16, 128, 8),
+                                               (torch.bfloat16, 64, 64)])
+@pytest.mark.parametrize("rows, q_heads, queries", [(20, 8, 1), (40, 16, 1), (9, 32, 4), (70, 8, 1)])
+def test_prefixes_of_many_query_rows(cuda_lib, dtype, dim, block, rows, q_heads, queries):
+    """80, 320, 576 and 280 query rows a KV head: one subtile, several, and a last one of few rows; prefixes that CTAs
+    share, that one covers, that end inside a tile, and one of two."""
+    from ekv.runtime.attention import attend
+
+    for blocks in (1, 3, 1000 // block, 5000 // block):
+        x = make(20 + blocks, [blocks * block + 1 + r % 37 + queries for r in range(rows)], queries=[queries] * rows, dim=dim,
+                 block=block, dtype=dtype, q_heads=q_heads, groups=[(0, rows, blocks)], width=blocks + -(-50 // block))
+        d = on_device(x)
+        got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=blocks)
+        check(got, x, 0.1, dtype)
+
+
+def test_wide_rows_with_gaps_and_growing_scores(cuda_lib):
+    """Query windows of 40 tokens on the wide kernel: bad table entries, an unfinished last block whose rest holds NaN,
+    and keys that grow along the row, so that the running maximum is raised again and again."""
+    import ekv._lib as L
+    from ekv.runtime.attention import attend
+
+    x = make(30, [1000, 700, 129, 40], queries=[40] * 4, q_heads=16, dtype=torch.float16)
+    x["cache"][:, 0] *= 0.2
+    for r, n in enumerate([1000, 700, 129, 40]):
+        for b in range(-(-n // 16)):
+            x["cache"][x["table"][r, b], 0] += 0.02 * b * torch.sign(x["query"][int(x["start"][r]), :2]).to(torch.float16)
+        if n % 16:
+            x["cache"][x["table"][r, n // 16], :, n % 16:] = float("nan")
+    ok = np.ones(tuple(x["table"].shape), dtype=bool)
+    for r, b, bad in [(0, 2, -1), (0, 40, 10**9), (1, 0, x["cache"].shape[0]), (1, 30, -7)]:
+        x["table"][r, b], ok[r, b] = bad, False
+    d = on_device(x)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], status=status)
+    check(got, x, 0.1, torch.float16, pool_ok=ok)
+    assert int(status) == L.STATUS_BAD_BLOCK_ID
+
+
 # ---- weights accumulated per token -------------------------------------------------------------------
 
 
