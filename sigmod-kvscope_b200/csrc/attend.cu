@@ -14,6 +14,7 @@
 // fragments in registers for a whole item, probabilities rounded to the cache's type (the products' operands
 // have to be of one type) and multiplied with the values in the same registers; sums stay in float32 from the
 // unrounded probabilities. The WN warps join through shared memory at an item's end.
+#include <algorithm>
 #include <type_traits>
 
 #include "attend.cuh"
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   TailT& tail = *reinterpret_cast<TailT*>(ring + R::kBytes);
-  const Plan plan = plan_at(ring + R::kBytes + (sizeof(TailT) + 15) / 16 * 16, PREFIX ? p.groups : p.rows, PREFIX);
+  const Plan plan{reinterpret_cast<int*>(ring + R::kBytes + (sizeof(TailT) + 15) / 16 * 16), PREFIX ? p.groups : p.rows};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -88,16 +89,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     }
     fence_mbar_init();
   }
-  chain_wait();  // the lengths, tables and caches may be the work of the launches before
+  // The lengths, tables and caches may be the work of the launches before. A launch that follows a prefix launch
+  // starts after that one has waited for them, reads nothing that it writes, and so runs beside its last CTAs; it
+  // waits at its end, so that what follows finds both complete.
+  if (!p.follows) chain_wait();
   make_plan<PREFIX, kThreads>(p, plan, MT, tail.scratch);
   const int W = plan.cum[plan.units];
   const int n = sharing_ctas(W, gridDim.x);
-  if (blockIdx.x == 0) {
-    for (int u = threadIdx.x; u <= plan.units; u += kThreads) p.cum[u] = plan.cum[u];
-    if (threadIdx.x == 0) p.cum[plan.units + 1] = n;
-  }
   chain_release();
-  if ((int)blockIdx.x >= n || W == 0) return;
+  if ((int)blockIdx.x >= n || W == 0) {
+    if (p.follows) chain_wait();
+    return;
+  }
   const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
   const int per_tile = kTile >> p.block_shift;  // blocks of a tile
 
@@ -148,6 +151,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       const int uses = issued > s ? (issued - s - 1) / R::kStages + 1 : 0;
       if (uses > 0) mbar_wait_bounded(&tail.full[s], (uses - 1) & 1, p.status);
     }
+    if (p.follows) chain_wait();
     return;
   }
 
@@ -161,7 +165,6 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     const Item it = item_at<PREFIX>(p, plan, MT, t, end);
     const QueryRange uq = it.un.q;
     const int from = it.un.from, to = it.un.to;
-    const RowRange rows = PREFIX ? group_rows(p, it.unit) : RowRange{it.unit, it.unit + 1};
     // this lane's two query rows: the tokens they see, and their fragments
     uint32_t qf[D / 16][4];
     int limit[2];
@@ -171,10 +174,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       const int token = uq.q0 + mrow / p.G;
       const bool real = mrow < uq.nq * p.G;
       limit[j] = 0x7fffffff;
-      if (real) {
-        const int r = PREFIX ? row_of_token(p, rows, token) : it.unit;
-        limit[j] = r < 0 ? 0 : token_limit<PREFIX>(p, r, token);
-      }
+      if (real) limit[j] = token_limit<PREFIX>(p, it.un, token);
       const T* src = static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 +
                      (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 2 * pair;
 #pragma unroll
@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       }
     }
   }
+  if (p.follows) chain_wait();
 }
 
 // ---- joining the parts ------------------------------------------------------------------------------------------
@@ -409,7 +410,7 @@ struct PhaseOut {
   const int32_t* cum;
   const float* parts;
   const float* whole;
-  int units, MT, max_ctas;
+  int units, MT, max_ctas, ctas;
 };
 
 struct CombineParams {
@@ -431,7 +432,7 @@ struct PartList {
 __device__ __forceinline__ PartList list_parts(const AttendParams& p, const PhaseOut& ph, int unit, int nq, int m, int head,
                                                int token, int qhead, int D) {
   PartList out{nullptr, nullptr, 0, 1, 0, 0, 0, 0};
-  const int W = ph.cum[ph.units], n = ph.cum[ph.units + 1];
+  const int W = ph.cum[ph.units], n = sharing_ctas(W, ph.ctas);
   const int mts = (nq * p.G + ph.MT - 1) / ph.MT;
   const int span = ph.cum[unit + 1] - ph.cum[unit];
   if (span == 0 || mts == 0) return out;
@@ -465,61 +466,150 @@ __device__ __forceinline__ int64_t part_row(const PartList& l, int i) {
   return (c == 0 ? l.first : l.rest + (c - 1) * l.step) + (l.halves == 2 && (i & 1) ? l.half : 0);
 }
 
-// A warp per (query token, query head); every lane holds D / 32 dims. The parts are added in order.
+// CTAs per (row, KV head), a warp per query row in turn; every lane holds D / 32 dims. The parts are added in order.
 template <typename T, int D>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineParams c) {
   const AttendParams& p = c.p;
   chain_release();
   chain_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
-  if (item >= (int64_t)p.tokens * p.q_heads) return;
-  const int token = (int)(item / p.q_heads), qhead = (int)(item - (int64_t)token * p.q_heads);
-  const int row = row_of_token(p, {0, p.rows}, token);
-  if (row < 0) return;  // a token of no row keeps its output
-  const QueryRange q = row_queries(p, row, false);
-  const int head = qhead / p.G, g = qhead - head * p.G;
-  PartList lists[2];
-  lists[0] = list_parts(p, c.own, row, q.nq, (token - q.q0) * p.G + g, head, token, qhead, D);
-  lists[1].count = 0;
-  const int group = group_of(p, row);
-  if (group >= 0) {
-    const QueryRange gq = group_queries(p, group_rows(p, group));
-    lists[1] = list_parts(p, c.prefix, group, gq.nq, (token - gq.q0) * p.G + g, head, token, qhead, D);
-  } else if (lists[0].count == 1 && p.groups == 0 && c.own.MT != kWideRows) {
-    return;  // the attention kernel wrote it
-  }
-  float m = -INFINITY;
-  for (int k = 0; k < 2; ++k)
-    for (int i = lane; i < lists[k].count; i += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], i)]);
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
-  float acc[D / 32], l = 0.f;
+  const int row = blockIdx.x / p.heads, head = blockIdx.x - row * p.heads;
+  const Unit un = unit_at<false>(p, row, false);
+  const int group = p.groups > 0 ? p.row_group[row] : -1;
+  const int4 gi = group >= 0 ? p.group_info[group] : make_int4(0, 0, 0, 0);
+  for (int m0 = blockIdx.y * (kCombineThreads / 32) + (threadIdx.x >> 5); m0 < un.q.nq * p.G;
+       m0 += gridDim.y * (kCombineThreads / 32)) {
+    const int token = un.q.q0 + m0 / p.G, qhead = head * p.G + m0 % p.G;
+    PartList lists[2];
+    lists[0] = list_parts(p, c.own, row, un.q.nq, m0, head, token, qhead, D);
+    lists[1].count = 0;
+    if (group >= 0 && token >= gi.x && token < gi.x + gi.y)
+      lists[1] = list_parts(p, c.prefix, group, gi.y, (token - gi.x) * p.G + m0 % p.G, head, token, qhead, D);
+    else if (lists[0].count == 1 && p.groups == 0 && c.own.MT != kWideRows)
+      continue;  // the attention kernel wrote it
+    float m = -INFINITY;
+    for (int k = 0; k < 2; ++k)
+      for (int i = lane; i < lists[k].count; i += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], i)]);
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
+    float acc[D / 32], l = 0.f;
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
-  for (int k = 0; k < 2; ++k) {
+    for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll 4
-    for (int i = 0; i < lists[k].count; ++i) {
-      const int64_t at = part_row(lists[k], i);
-      const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
-      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-      const float* o = lists[k].o + at * D + lane * (D / 32);
-      l += ml.x == -INFINITY ? 0.f : ml.y * f;
+      for (int i = 0; i < lists[k].count; ++i) {
+        const int64_t at = part_row(lists[k], i);
+        const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
+        const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+        float o[D / 32];
+        if constexpr (D == 128)
+          *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(lists[k].o + at * D + lane * 4);
+        else
+          *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(lists[k].o + at * D + lane * 2);
+        l += ml.x == -INFINITY ? 0.f : ml.y * f;
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) acc[d] = ml.x == -INFINITY ? acc[d] : fmaf(o[d], f, acc[d]);
+        for (int d = 0; d < D / 32; ++d) acc[d] = ml.x == -INFINITY ? acc[d] : fmaf(o[d], f, acc[d]);
+      }
+    }
+    const float inv = 1.f / l;
+    T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)qhead * p.out_s1 + lane * (D / 32);
+#pragma unroll
+    for (int d = 0; d < D / 32; d += 2)
+      *reinterpret_cast<uint32_t*>(dst + d) = l == 0.f ? 0u : pack2<T>(acc[d] * inv, acc[d + 1] * inv);
+    if (p.lse != nullptr && lane == 0)
+      p.lse[(int64_t)token * p.q_heads + qhead] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  }
+}
+
+// ---- the plan of a batch with groups ------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 512;
+
+struct PlanParams {
+  AttendParams p;
+  int32_t *cum_own, *cum_prefix;
+  int mt_own, mt_prefix;
+};
+
+// Running sums of n over [0, units) into cum, with every thread; count(u) is unit u's tiles.
+template <typename Count>
+__device__ __forceinline__ void running_sum(int32_t* cum, int units, int* scratch, Count count) {
+  int carry = 0;
+  for (int base = 0; base < units; base += kPlanThreads) {
+    const int u = base + threadIdx.x;
+    int total = 0;
+    const int n = u < units ? count(u) : 0;
+    const int before = block_exclusive_scan<kPlanThreads>(n, scratch, &total);
+    if (u < units) cum[u] = carry + before;
+    carry += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) cum[units] = carry;
+}
+
+// One CTA: what every row leaves to its group (whole blocks that it has, so that the prefix launch reads no position
+// that no row of the group holds), each group's longest such part and the row it is read from, and both phases' counts.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams pp) {
+  const AttendParams& p = pp.p;
+  extern __shared__ uint8_t s_plan[];
+  unsigned long long* lead = reinterpret_cast<unsigned long long*>(s_plan);  // [groups] shared tokens << 32 | ~row
+  int* starts = reinterpret_cast<int*>(lead + p.groups);                     // [groups + 1]
+  int* blocks = starts + p.groups + 1;                                       // [groups]
+  __shared__ int scratch[kPlanThreads / 32 + 1];
+  const int lane = threadIdx.x & 31;
+  chain_release();
+  chain_wait();
+  for (int g = threadIdx.x; g <= p.groups; g += kPlanThreads) {
+    starts[g] = p.group_start == nullptr ? (g == 0 ? 0 : p.rows) : min(max(p.group_start[g], 0), p.rows);
+    if (g < p.groups) {
+      lead[g] = 0;
+      blocks[g] = min(max(p.prefix_blocks != nullptr ? p.prefix_blocks[g] : p.prefix_common, 0), p.width);
     }
   }
-  const float inv = 1.f / l;
-  T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)qhead * p.out_s1 + lane * (D / 32);
-#pragma unroll
-  for (int d = 0; d < D / 32; d += 2)
-    *reinterpret_cast<uint32_t*>(dst + d) = l == 0.f ? 0u : pack2<T>(acc[d] * inv, acc[d + 1] * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[item] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  __syncthreads();
+  const int own_tokens = pp.mt_own == kWideRows ? 2 * kTile : kTile;
+  running_sum(pp.cum_own, p.rows, scratch, [&](int r) {
+    const QueryRange q = row_queries(p, r, true);
+    const int to = row_tokens(p, r, true);
+    int lo = 0, hi = p.groups;  // the last group that starts at or before r
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= r) lo = mid; else hi = mid;
+    }
+    const bool in = r >= starts[lo] && r < starts[lo + 1];
+    const int from = in ? min(blocks[lo] << p.block_shift, to >> p.block_shift << p.block_shift) : 0;
+    if (in) atomicMax(lead + lo, (unsigned long long)(uint32_t)from << 32 | (uint32_t)~(uint32_t)r);
+    p.row_info[r] = make_int4(q.q0, q.nq, from, to);
+    p.row_group[r] = in ? lo : -1;
+    for (int i = 0; i < min(q.nq, 8); ++i) p.limits[q.q0 + i] = min(to - q.nq + i + 1, from);
+    return to > from && q.nq > 0 ? (to - from + own_tokens - 1) / own_tokens * p.heads * ((q.nq * p.G + pp.mt_own - 1) / pp.mt_own)
+                                 : 0;
+  });
+  __syncthreads();
+  // rows of many query tokens: their limits by a warp
+  for (int r = threadIdx.x >> 5; r < p.rows && p.tokens > 8; r += kPlanThreads / 32) {
+    const int4 v = p.row_info[r];
+    for (int i = 8 + lane; i < v.y; i += 32) p.limits[v.x + i] = min(v.w - v.y + i + 1, v.z);
+  }
+  const int prefix_tokens = pp.mt_prefix == kWideRows ? 2 * kTile : kTile;
+  running_sum(pp.cum_prefix, p.groups, scratch, [&](int g) {
+    const int a = starts[g], b = starts[g + 1];
+    const int to = b > a ? (int)(lead[g] >> 32) : 0, row = to > 0 ? (int)~(uint32_t)lead[g] : 0;
+    // the query tokens of the rows [a, b), which follow one another
+    int q0 = 0, nq = 0;
+    if (b > a) {
+      q0 = p.query_start == nullptr ? a : p.query_start[a];
+      nq = (p.query_start == nullptr ? min(b, p.tokens) : p.query_start[b]) - q0;
+      if (q0 < 0 || nq < 0 || nq > p.tokens - q0) q0 = nq = 0;
+    }
+    p.group_info[g] = make_int4(q0, nq, row, to);
+    return to > 0 && nq > 0 ? (to + prefix_tokens - 1) / prefix_tokens * p.heads * ((nq * p.G + pp.mt_prefix - 1) / pp.mt_prefix) : 0;
+  });
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 struct Workspace {
-  size_t cum[2], parts[2], whole[2], total;
+  size_t cum[2], parts[2], whole[2], row_info, group_info, row_group, limits, total;
 };
 
 int max_ctas(int mt) { return mt == kWideRows ? kWideMaxCtas : kAttendMaxCtas; }
@@ -528,9 +618,19 @@ int max_ctas(int mt) { return mt == kWideRows ? kWideMaxCtas : kAttendMaxCtas; }
 Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, const int (&mt)[2]) {
   Workspace w{};
   size_t at = 0;
+  if (groups > 0) {
+    w.row_info = at;
+    at += round_up((size_t)rows * 16, 256);
+    w.group_info = at;
+    at += round_up((size_t)groups * 16, 256);
+    w.row_group = at;
+    at += round_up((size_t)rows * 4, 256);
+    w.limits = at;
+    at += round_up((size_t)tokens * 4, 256);
+  }
   for (int k = 0; k < (groups > 0 ? 2 : 1); ++k) {
     w.cum[k] = at;
-    at += round_up(((size_t)(k == 0 ? rows : groups) + 2) * 4, 256);
+    at += round_up(((size_t)(k == 0 ? rows : groups) + 1) * 4, 256);
     w.parts[k] = at;
     at += round_up((size_t)2 * max_ctas(mt[k]) * mt[k] * (dim + 2) * 4, 256);
     w.whole[k] = at;
@@ -548,24 +648,25 @@ int pick_mt(int64_t tokens, int units, int G) {
 }
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
-int launch_attend(const AttendParams& p, int device, int sms, cudaStream_t s) {
+int launch_attend(const AttendParams& p, int device, int sms, int* ctas, cudaStream_t s) {
   const int units = PREFIX ? p.groups : p.rows;
-  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16 + plan_bytes(units, PREFIX);
+  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16 + plan_bytes(units);
   auto kernel = attend_kernel<T, D, WM, WN, PREFIX>;
   static LaunchCache cache;
   int resident = 0;
   const int rc = prepare_launch(cache, kernel, "attend_kernel", device, kThreads, smem, &resident);
   if (rc != EKV_OK) return rc;
-  launch_chained(kernel, dim3(min(sms * resident, p.max_ctas)), dim3(kThreads), smem, s, p);
+  *ctas = min(sms * resident, p.max_ctas);
+  launch_chained(kernel, dim3(*ctas), dim3(kThreads), smem, s, p);
   return check_launch("attend_kernel");
 }
 
 template <typename T, int D, bool PREFIX>
-int launch_phase(const AttendParams& p, int device, int sms, cudaStream_t s) {
+int launch_phase(const AttendParams& p, int device, int sms, int* ctas, cudaStream_t s) {
   switch (p.mt_rows) {
-    case 16: return launch_attend<T, D, 1, 4, PREFIX>(p, device, sms, s);
-    case 32: return launch_attend<T, D, 2, 2, PREFIX>(p, device, sms, s);
-    default: return launch_attend<T, D, 4, 1, PREFIX>(p, device, sms, s);
+    case 16: return launch_attend<T, D, 1, 4, PREFIX>(p, device, sms, ctas, s);
+    case 32: return launch_attend<T, D, 2, 2, PREFIX>(p, device, sms, ctas, s);
+    default: return launch_attend<T, D, 4, 1, PREFIX>(p, device, sms, ctas, s);
   }
 }
 
@@ -573,22 +674,37 @@ template <typename T, int D>
 int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, int device, int sms, cudaStream_t s) {
   CombineParams c{};
   const int phases = p.groups > 0 ? 2 : 1;
+  const int type = std::is_same<T, __half>::value ? EKV_DTYPE_F16 : EKV_DTYPE_BF16;
+  if (p.groups > 0) {
+    p.row_info = reinterpret_cast<int4*>(ws + w.row_info);
+    p.group_info = reinterpret_cast<int4*>(ws + w.group_info);
+    p.row_group = reinterpret_cast<int32_t*>(ws + w.row_group);
+    p.limits = reinterpret_cast<int32_t*>(ws + w.limits);
+    const PlanParams plan{p, reinterpret_cast<int32_t*>(ws + w.cum[0]), reinterpret_cast<int32_t*>(ws + w.cum[1]), mt[0], mt[1]};
+    launch_chained(plan_kernel, dim3(1), dim3(kPlanThreads), (size_t)p.groups * 16 + 16, s, plan);
+    const int rc = check_launch("plan_kernel");
+    if (rc != EKV_OK) return rc;
+  }
   for (int k = phases - 1; k >= 0; --k) {  // the prefixes first
     p.mt_rows = mt[k];
     p.cum = reinterpret_cast<int32_t*>(ws + w.cum[k]);
     p.parts = reinterpret_cast<float*>(ws + w.parts[k]);
     p.whole = reinterpret_cast<float*>(ws + w.whole[k]);
     p.max_ctas = max_ctas(mt[k]);
-    (k == 0 ? c.own : c.prefix) = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k], p.max_ctas};
-    const int type = std::is_same<T, __half>::value ? EKV_DTYPE_F16 : EKV_DTYPE_BF16;
-    const int rc = mt[k] == kWideRows ? (k == 1 ? launch_wide<true>(p, D, type, device, sms, s) : launch_wide<false>(p, D, type, device, sms, s))
-                   : k == 1 ? launch_phase<T, D, true>(p, device, sms, s) : launch_phase<T, D, false>(p, device, sms, s);
+    p.follows = k == 0 && phases == 2 && mt[0] != kWideRows;
+    PhaseOut& out = k == 0 ? c.own : c.prefix;
+    out = PhaseOut{p.cum, p.parts, p.whole, k == 0 ? p.rows : p.groups, mt[k], p.max_ctas, 0};
+    int* ctas = &out.ctas;
+    const int rc = mt[k] == kWideRows ? (k == 1 ? launch_wide<true>(p, D, type, device, sms, ctas, s)
+                                                : launch_wide<false>(p, D, type, device, sms, ctas, s))
+                   : k == 1 ? launch_phase<T, D, true>(p, device, sms, ctas, s)
+                            : launch_phase<T, D, false>(p, device, sms, ctas, s);
     if (rc != EKV_OK) return rc;
   }
   c.p = p;
-  const int64_t items = (int64_t)p.tokens * p.q_heads;
-  const int per = kCombineThreads / 32;
-  launch_chained(combine_kernel<T, D>, dim3((unsigned)((items + per - 1) / per)), dim3(kCombineThreads), 0, s, c);
+  // warps for a row's average of query rows
+  const int per = kCombineThreads / 32, spread = (int)std::min<int64_t>(64, ((int64_t)p.tokens * p.G / p.rows + per - 1) / per);
+  launch_chained(combine_kernel<T, D>, dim3(p.rows * p.heads, max(spread, 1)), dim3(kCombineThreads), 0, s, c);
   return check_launch("combine_kernel");
 }
 

@@ -4,9 +4,10 @@
 // Work. A unit is one row of the batch (its own tokens, behind its group's shared prefix), or, in a prefix
 // launch, one group of rows (the tokens they share). A unit's M = query tokens x query heads per KV head
 // query rows are cut into M tiles, its tokens into tiles of kTile; the launch's tiles, numbered unit by
-// unit, KV head, M tile, token tile, are dealt evenly: CTA c of n takes tiles [c W / n, (c + 1) W / n). Every
-// CTA computes the units' running tile counts itself (a scan of the rows' lengths), so no plan travels
-// through the host and no launch precedes the first load.
+// unit, KV head, M tile, token tile, are dealt evenly: CTA c of n takes tiles [c W / n, (c + 1) W / n). The units'
+// running tile counts come from the lengths on the device, so no plan travels through the host: without
+// groups every CTA scans them itself (one level of loads), with groups a one-CTA kernel goes ahead, since what a
+// row shares takes a chain of dependent loads that would otherwise stand at the start of every CTA of every launch.
 //
 // Parts. A CTA that covers a whole (unit, KV head, M tile) finishes it; one that covers some of its tiles
 // leaves the part's running maximum, sum and unnormalised output in the workspace. A CTA has at most two
@@ -46,11 +47,17 @@ struct AttendParams {
   const int32_t* prefix_blocks;  // [groups], or NULL: prefix_common
   int prefix_common;
   uint32_t* status;
-  // the workspace, of the launch's phase and (for the combine kernel) of both
-  int32_t* cum;   // [units + 1] running tile counts, then the number of CTAs that share them
+  // the workspace. With groups, what plan_kernel leaves:
+  int4* row_info;    // [rows] q0, nq, from, to
+  int4* group_info;  // [groups] q0, nq, table row, to
+  int32_t* row_group;  // [rows] or -1
+  int32_t* limits;     // [tokens] the positions of its group's prefix that a query token sees
+  // of the launch's phase:
+  int32_t* cum;   // [units + 1] running tile counts
   float* parts;   // [2 CTAs][MT][D], and behind them their [2 CTAs][MT][2] maxima and sums
   float* whole;   // [tokens * q_heads][D] and [tokens * q_heads][2]: finished items when another phase joins (twice that
                   // in a wide launch, whose items of few query rows end in two halves)
+  int follows;    // the launch before this one is the same call's prefix launch
   int mt_rows;    // query rows of an M tile
   int max_ctas;
 };
@@ -83,101 +90,7 @@ __device__ __forceinline__ int row_tokens(const AttendParams& p, int r, bool rep
   return len > 0 ? len : 0;
 }
 
-struct RowRange {
-  int a, b;
-};
-
-__device__ __forceinline__ RowRange group_rows(const AttendParams& p, int g) {
-  if (p.group_start == nullptr) return {0, p.rows};
-  int a = p.group_start[g], b = p.group_start[g + 1];
-  a = min(max(a, 0), p.rows);
-  b = min(max(b, a), p.rows);
-  return {a, b};
-}
-
-__device__ __forceinline__ int group_prefix(const AttendParams& p, int g) {  // tokens
-  const int blocks = p.prefix_blocks != nullptr ? p.prefix_blocks[g] : p.prefix_common;
-  return min(max(blocks, 0), p.width) << p.block_shift;
-}
-
-// The group of row r, or -1.
-__device__ __forceinline__ int group_of(const AttendParams& p, int r) {
-  if (p.groups == 0) return -1;
-  if (p.group_start == nullptr) return 0;
-  int lo = 0, hi = p.groups;  // the last group that starts at or before r
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.group_start[mid] <= r) lo = mid; else hi = mid;
-  }
-  const RowRange rr = group_rows(p, lo);
-  return r >= rr.a && r < rr.b ? lo : -1;
-}
-
-// Tokens that row r leaves to its group's prefix launch: whole blocks that it has, so that the launch reads no
-// position that no row of the group holds.
-__device__ __forceinline__ int row_prefix(const AttendParams& p, int r) {
-  const int g = group_of(p, r);
-  return g < 0 ? 0 : min(group_prefix(p, g), row_tokens(p, r, false) >> p.block_shift << p.block_shift);
-}
-
-// The query tokens of a group: those of its rows, which follow one another.
-__device__ __forceinline__ QueryRange group_queries(const AttendParams& p, RowRange rr) {
-  if (rr.b <= rr.a) return {0, 0};
-  if (p.query_start == nullptr) {
-    const int b = min(rr.b, p.tokens);
-    return {rr.a, max(b - rr.a, 0)};
-  }
-  const int a = p.query_start[rr.a], b = p.query_start[rr.b];
-  if (a < 0 || b < a || b > p.tokens) return {0, 0};
-  return {a, b - a};
-}
-
-// The row in [rr.a, rr.b) that holds query token t (-1 if none does) by binary search of query_start.
-__device__ __forceinline__ int row_of_token(const AttendParams& p, RowRange rr, int t) {
-  if (p.query_start == nullptr) return t >= rr.a && t < rr.b ? t : -1;
-  int lo = rr.a, hi = rr.b;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.query_start[mid] <= t) lo = mid; else hi = mid;
-  }
-  if (lo >= rr.b) return -1;
-  const QueryRange q = row_queries(p, lo, false);
-  return t >= q.q0 && t < q.q0 + q.nq ? lo : -1;
-}
-
-// Positions below this are visible to query token t of row r (in a prefix launch: of those the row left to it).
-template <bool PREFIX>
-__device__ __forceinline__ int token_limit(const AttendParams& p, int r, int t) {
-  const QueryRange q = row_queries(p, r, false);
-  const int limit = row_tokens(p, r, false) - q.nq + (t - q.q0) + 1;
-  return PREFIX ? min(limit, row_prefix(p, r)) : limit;
-}
-
 // ---- the plan ----------------------------------------------------------------------------------------
-
-// In shared memory: cum[units + 1], the running tile counts, and for a prefix launch lead[units], the longest
-// row of each group (its shared tokens << 32 | ~row), whose table is read.
-struct Plan {
-  int* cum;
-  unsigned long long* lead;
-  int units;
-};
-
-__device__ __forceinline__ int lead_row(unsigned long long v) { return (int)~(uint32_t)v; }
-__device__ __forceinline__ int lead_len(unsigned long long v) { return (int)(v >> 32); }
-
-__host__ __device__ inline size_t plan_bytes(int units, bool prefix) {
-  return ((size_t)(units + 1) * 4 + 15) / 16 * 16 + (prefix ? (size_t)units * 8 : 0);
-}
-
-__device__ __forceinline__ Plan plan_at(void* smem, int units, bool prefix) {
-  Plan plan;
-  plan.units = units;
-  plan.cum = static_cast<int*>(smem);
-  uint8_t* end = static_cast<uint8_t*>(smem) + ((size_t)(units + 1) * 4 + 15) / 16 * 16;
-  plan.lead = prefix ? reinterpret_cast<unsigned long long*>(end) : nullptr;
-  return plan;
-}
 
 // A unit: its query tokens, the table row its blocks are in, and its positions [from, to).
 struct Unit {
@@ -191,43 +104,47 @@ struct Unit {
 };
 
 template <bool PREFIX>
-__device__ __forceinline__ Unit unit_at(const AttendParams& p, const Plan& plan, int u, bool report) {
-  Unit un;
+__device__ __forceinline__ Unit unit_at(const AttendParams& p, int u, bool report) {
   if (PREFIX) {
-    const RowRange rr = group_rows(p, u);
-    un.q = group_queries(p, rr);
-    un.row = lead_row(plan.lead[u]);
-    un.from = 0;
-    un.to = lead_len(plan.lead[u]);  // 0 for a group with no rows
-  } else {
-    un.q = row_queries(p, u, report);
-    un.row = u;
-    un.from = row_prefix(p, u);
-    un.to = row_tokens(p, u, report);
+    const int4 v = __ldcg(p.group_info + u);
+    return {{v.x, v.y}, v.z, 0, v.w};
   }
-  return un;
+  if (p.groups > 0) {
+    const int4 v = __ldcg(p.row_info + u);  // from L2: a launch that follows another has not waited itself
+    return {{v.x, v.y}, u, v.z, v.w};
+  }
+  return {row_queries(p, u, report), u, 0, row_tokens(p, u, report)};
 }
+
+// The positions that query token t of a unit sees end here.
+template <bool PREFIX>
+__device__ __forceinline__ int token_limit(const AttendParams& p, const Unit& un, int t) {
+  return PREFIX ? p.limits[t] : un.to - un.q.nq + (t - un.q.q0) + 1;
+}
+
+// The running tile counts, in shared memory.
+struct Plan {
+  int* cum;  // [units + 1]
+  int units;
+};
+
+__host__ __device__ inline size_t plan_bytes(int units) { return ((size_t)(units + 1) * 4 + 15) / 16 * 16; }
 
 // Fills the plan with every thread of the CTA (THREADS of them); `scratch` holds THREADS / 32 + 1 ints.
 template <bool PREFIX, int THREADS, int TOKENS = kTile>
 __device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& plan, int MT, int* scratch) {
-  const bool report = blockIdx.x == 0;
-  if (PREFIX) {
-    for (int g = threadIdx.x; g < plan.units; g += THREADS) plan.lead[g] = 0;
+  if (PREFIX || p.groups > 0) {
+    for (int u = threadIdx.x; u <= plan.units; u += THREADS) plan.cum[u] = __ldcg(p.cum + u);
     __syncthreads();
-    for (int r = threadIdx.x; r < p.rows; r += THREADS) {
-      const int g = group_of(p, r);
-      if (g >= 0)
-        atomicMax(plan.lead + g, (unsigned long long)(uint32_t)row_prefix(p, r) << 32 | (uint32_t)~(uint32_t)r);
-    }
-    __syncthreads();
+    return;
   }
+  const bool report = blockIdx.x == 0;
   int carry = 0;
   for (int base = 0; base < plan.units; base += THREADS) {
     const int u = base + threadIdx.x;
     int n = 0;
     if (u < plan.units) {
-      const Unit un = unit_at<PREFIX>(p, plan, u, report);
+      const Unit un = unit_at<PREFIX>(p, u, report);
       n = un.template tiles<TOKENS>() * p.heads * un.m_tiles(p, MT);
     }
     int total = 0;
@@ -237,6 +154,8 @@ __device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& pla
   }
   if (threadIdx.x == 0) plan.cum[plan.units] = carry;
   __syncthreads();
+  if (report && p.cum != nullptr)  // for the combine kernel
+    for (int u = threadIdx.x; u <= plan.units; u += THREADS) p.cum[u] = plan.cum[u];
 }
 
 // The tiles of CTA c when n CTAs share W, and the CTA that holds tile t.
@@ -259,7 +178,7 @@ __device__ __forceinline__ Item item_at(const AttendParams& p, const Plan& plan,
   }
   Item it;
   it.unit = lo;
-  it.un = unit_at<PREFIX>(p, plan, lo, false);
+  it.un = unit_at<PREFIX>(p, lo, false);
   it.tiles = it.un.template tiles<TOKENS>();
   const int mts = it.un.m_tiles(p, MT);
   const int rem = t - plan.cum[lo], hm = rem / it.tiles;
@@ -349,7 +268,7 @@ int encode_cache_maps(AttendParams& p, const void* kv, int64_t s_block, int64_t 
 constexpr int kWideRows = 256;
 constexpr int kWideMaxCtas = 160;
 template <bool PREFIX>
-int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, cudaStream_t s);
+int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, int* ctas, cudaStream_t s);
 
 // Adds each token's weight to its score after an attention launch that left a.lse (attend_scores.cu).
 int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,

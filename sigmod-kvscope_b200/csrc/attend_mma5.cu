@@ -96,25 +96,33 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// A shared-memory operand in the 128-byte swizzle: `lead` and `stride` are the byte distances between 64-element
-// groups of the major dimension and between groups of eight rows.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// One lane of the converged warp, always the same one. The issuing code goes by this vote and not by the lane's
+// number, and its addresses are made of values that are the same in the whole warp: then the tensor-core instructions
+// take them from uniform registers (with per-lane ones each instruction took 115 cycles to issue, twice its work).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+  return chosen != 0;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// A shared-memory operand in the 128-byte swizzle, in two words: where it starts with the distance `lead` in bytes
+// between 64-element groups of the major dimension, and (constant) 1024 bytes between groups of eight rows.
+__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t lead) { return (addr & 0x3ffff) >> 4 | (lead >> 4) << 16; }
+constexpr uint32_t kOperandHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kOperandHigh)
       : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kOperandHigh)
       : "memory");
 }
 
@@ -152,8 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   uint8_t* queries = base;              // [2] subtiles
   uint8_t* ring = base + 2 * R::kSlot;  // [kSlots]
   WideTail<D>& tail = *reinterpret_cast<WideTail<D>*>(ring + R::kRing);
-  const Plan plan = plan_at(ring + R::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16, PREFIX ? p.groups : p.rows, PREFIX);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Plan plan{reinterpret_cast<int*>(ring + R::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16), PREFIX ? p.groups : p.rows};
+  const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < R::kSlots; ++s) {
       mbar_init(&tail.full[s], 1);
@@ -173,10 +181,6 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   make_plan<PREFIX, kThreads, kTokens>(p, plan, kWideRows, tail.scratch);
   const int W = plan.cum[plan.units];
   const int n = sharing_ctas(W, gridDim.x);
-  if (blockIdx.x == 0) {
-    for (int u = threadIdx.x; u <= plan.units; u += kThreads) p.cum[u] = plan.cum[u];
-    if (threadIdx.x == 0) p.cum[plan.units + 1] = n;
-  }
   chain_release();
   if ((int)blockIdx.x >= n || W == 0) return;
   if (warp == kMmaWarp) {
@@ -240,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     constexpr uint32_t kScores = kShape | (uint32_t)(kTokens >> 3) << 17;
     constexpr uint32_t kOutput = kShape | 1u << 16 | (uint32_t)(D >> 3) << 17;  // the values' tokens are their rows
     const uint32_t q_at = smem_u32(queries), ring_at = smem_u32(ring);
+    const uint32_t tm = __shfl_sync(kFullMask, tmem, 0);
     int slot = 0;
     uint32_t phase = 0;
     uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0}, items[2] = {0, 0};
@@ -255,24 +260,23 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       if (++slot == R::kSlots) slot = 0, phase ^= 1;
       return s;
     };
+    const uint32_t q_low = operand_low(q_at, 16), ring_low = operand_low(ring_at, 16), value_low = operand_low(ring_at, R::kHalf);
     auto scores = [&](int w, int s) {
-      if (lane != 0 || !good) return;
+      if (!good || !elect_one()) return;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const uint32_t at = (uint32_t)(k >> 2) * R::kHalf + (uint32_t)(k & 3) * 32;
-        mma_ss(tmem + w * 128, operand(q_at + w * R::kSlot + at, 16, 1024), operand(ring_at + s * R::kSlot + at, 16, 1024),
-               kScores, k > 0);
+        const uint32_t at = ((uint32_t)(k >> 2) * R::kHalf + (uint32_t)(k & 3) * 32) >> 4;
+        mma_ss(tm + w * 128, q_low + w * (R::kSlot >> 4) + at, ring_low + s * (R::kSlot >> 4) + at, kScores, k > 0);
       }
     };
     auto output = [&](int w, int s, bool add) {
-      if (lane != 0 || !good) return;
+      if (!good || !elect_one()) return;
 #pragma unroll
       for (int k = 0; k < kTokens / 16; ++k)
-        mma_ts(tmem + 256 + w * 128, tmem + w * 128 + 8 * k, operand(ring_at + s * R::kSlot + k * 2048, R::kHalf, 1024),
-               kOutput, add || k > 0);
+        mma_ts(tm + 256 + w * 128, tm + w * 128 + 8 * k, value_low + s * (R::kSlot >> 4) + k * (2048 >> 4), kOutput, add || k > 0);
     };
     auto commit = [&](uint64_t* bar) {
-      if (lane == 0) tc_commit(bar);
+      if (elect_one()) tc_commit(bar);
     };
     // rows of a value tile behind the unit's last token hold whatever the block holds: cleared, since a probability
     // of zero times that need not be zero
@@ -382,10 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
         proxy_fence_smem();
         mbar_arrive(&tail.q_full[w]);
         int limit = 0x7fffffff;
-        if (real) {
-          const int r = PREFIX ? row_of_token(p, group_rows(p, it.unit), token) : it.unit;
-          limit = r < 0 ? 0 : token_limit<PREFIX>(p, r, token);
-        }
+        if (real) limit = token_limit<PREFIX>(p, it.un, token);
         limit = min(limit, it.un.to);
         const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
         const int block0 = it.un.from >> p.block_shift, last_block = (it.un.to - 1) >> p.block_shift;
@@ -510,28 +511,29 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 }
 
 template <typename T, int D, bool PREFIX>
-int launch(const AttendParams& p, int device, int sms, cudaStream_t s) {
+int launch(const AttendParams& p, int device, int sms, int* ctas, cudaStream_t s) {
   const int units = PREFIX ? p.groups : p.rows;
-  const size_t smem = 1024 + 2 * Wide<D>::kSlot + Wide<D>::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16 + plan_bytes(units, PREFIX);
+  const size_t smem = 1024 + 2 * Wide<D>::kSlot + Wide<D>::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16 + plan_bytes(units);
   auto kernel = wide_kernel<T, D, PREFIX>;
   static LaunchCache cache;
   int resident = 0;
   const int rc = prepare_launch(cache, kernel, "wide_kernel", device, kThreads, smem, &resident);
   if (rc != EKV_OK) return rc;
-  launch_chained(kernel, dim3(min(sms, p.max_ctas)), dim3(kThreads), smem, s, p);
+  *ctas = min(sms, p.max_ctas);
+  launch_chained(kernel, dim3(*ctas), dim3(kThreads), smem, s, p);
   return check_launch("wide_kernel");
 }
 
 }  // namespace
 
 template <bool PREFIX>
-int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, cudaStream_t s) {
+int launch_wide(const AttendParams& p, int dim, int dtype, int device, int sms, int* ctas, cudaStream_t s) {
   if (dtype == EKV_DTYPE_BF16)
-    return dim == 128 ? launch<__nv_bfloat16, 128, PREFIX>(p, device, sms, s) : launch<__nv_bfloat16, 64, PREFIX>(p, device, sms, s);
-  return dim == 128 ? launch<__half, 128, PREFIX>(p, device, sms, s) : launch<__half, 64, PREFIX>(p, device, sms, s);
+    return dim == 128 ? launch<__nv_bfloat16, 128, PREFIX>(p, device, sms, ctas, s) : launch<__nv_bfloat16, 64, PREFIX>(p, device, sms, ctas, s);
+  return dim == 128 ? launch<__half, 128, PREFIX>(p, device, sms, ctas, s) : launch<__half, 64, PREFIX>(p, device, sms, ctas, s);
 }
 
-template int launch_wide<true>(const AttendParams&, int, int, int, int, cudaStream_t);
-template int launch_wide<false>(const AttendParams&, int, int, int, int, cudaStream_t);
+template int launch_wide<true>(const AttendParams&, int, int, int, int, int*, cudaStream_t);
+template int launch_wide<false>(const AttendParams&, int, int, int, int, int*, cudaStream_t);
 
 }  // namespace ekv

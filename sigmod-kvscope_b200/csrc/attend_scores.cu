@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   Tail<D>& tail = *reinterpret_cast<Tail<D>*>(ring + R::kBytes);
-  const Plan plan = plan_at(ring + R::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16, p.rows, false);
+  const Plan plan{reinterpret_cast<int*>(ring + R::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16), p.rows};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < R::kStages; ++s) {
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const __grid_constan
 
 template <typename T, int D>
 int launch_scores(const ScoreParams& p, int device, int sms, cudaStream_t s) {
-  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows, false);
+  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows);
   auto kernel = score_kernel<T, D>;
   static LaunchCache cache;
   int resident = 0;
