@@ -507,9 +507,11 @@ int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, con
  * w = sum of exp(scale q.k - lse) over the row's query tokens and the head's query heads: its score becomes w
  * when t is among the row's newest fresh[r] tokens (int32 [rows]; NULL: its query tokens), which have none
  * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends without scoring; a
- * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Same workspace as ekv_attend
- * with groups = 0. Three kernels, no host synchronisation.
+ * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Three kernels, no host
+ * synchronisation.
  */
+size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,
+                                         int head_dim);
 int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
                       int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
                       int64_t kv_stride_head, int64_t pool_blocks, const int32_t* table, int64_t table_stride,
@@ -543,7 +545,7 @@ size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_t pool_bloc
 /*
  * ekv_compact_tokens -- the kept tokens of each row and KV head moved to the front of the row's blocks, in place.
  *
- * kv [pool_blocks][2][block_size][heads] rows of head_bytes bytes (strides in bytes, whole 16-byte units; any element type).
+ * kv [pool_blocks][2][block_size][heads] rows of head_bytes bytes (strides in bytes, whole 16-byte units, 16 to 1024 bytes; any element type).
  * In every row with 0 <= new_lens[r] < lens[r], position j < new_lens[r] of KV head h takes the key, the value and,
  * with scores (as in ekv_attend_scored; may be NULL), the score of position kept[r][h][j] (int32, `columns` entries a
  * list, ascending strictly, below lens[r]); what lies behind new_lens[r] stays as it was. The lists keep the first

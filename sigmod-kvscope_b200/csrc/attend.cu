@@ -235,6 +235,19 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
             if (pos >= to || pos >= limit[e >> 1] || !((blocks >> (tk >> p.block_shift)) & 1u)) s[j][e] = -INFINITY;
           }
       }
+      if constexpr (WM == 1 && !PREFIX) {
+        if (p.logits != nullptr) {  // for the pass that adds up the tokens' weights
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int mrow = it.mt * MT + quad + 8 * j;
+            if (mrow >= uq.nq * p.G) continue;
+            float* dst = p.logits + ((int64_t)(uq.q0 + mrow / p.G) * p.q_heads + it.head * p.G + mrow % p.G) * p.logits_s0 + pos0 + 2 * pair;
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+              *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(s[i][2 * j] * p.scale_log2, s[i][2 * j + 1] * p.scale_log2);
+          }
+        }
+      }
       // the running maximum of each query row over this warp's tokens
       float mx[2] = {s[0][0], s[0][2]};
 #pragma unroll
@@ -609,13 +622,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
 // ---- host ----------------------------------------------------------------------------------------------------------
 
 struct Workspace {
-  size_t cum[2], parts[2], whole[2], row_info, group_info, row_group, limits, total;
+  size_t cum[2], parts[2], whole[2], row_info, group_info, row_group, limits, logits, total;
 };
 
 int max_ctas(int mt) { return mt == kWideRows ? kWideMaxCtas : kAttendMaxCtas; }
 
 // Phase 0: the rows' own tokens; phase 1: the shared prefixes.
-Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, const int (&mt)[2]) {
+Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int dim, const int (&mt)[2], int64_t logits) {
   Workspace w{};
   size_t at = 0;
   if (groups > 0) {
@@ -637,7 +650,8 @@ Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int di
     if (groups > 0 || mt[k] == kWideRows)
       at += round_up((size_t)tokens * q_heads * (dim + 2) * 4 * (mt[k] == kWideRows ? 2 : 1), 256);
   }
-  w.total = at;
+  w.logits = at;
+  w.total = at + round_up((size_t)logits * 4, 256);
   return w;
 }
 
@@ -749,6 +763,15 @@ using namespace ekv;
 
 namespace {
 
+// The scores' row length where the attention keeps its logits for the pass over the weights, and how many floats that
+// takes: for at most 16 query rows a KV head, whose logits (8 bytes of traffic a token and query row) cost less than
+// the keys again (256); not beyond 1 GiB, which is a table far wider than its rows.
+int64_t logits_row(int width, int block_size) { return ((int64_t)width * block_size + kTile - 1) / kTile * kTile; }
+int64_t kept_logits(int tokens, int rows, int width, int block_size, int q_heads, int kv_heads) {
+  const int64_t n = (int64_t)tokens * q_heads * logits_row(width, block_size);
+  return pick_mt(tokens, rows, q_heads / kv_heads) == 16 && n <= (1ll << 28) ? n : 0;
+}
+
 struct AttendCall {
   AttendParams p;
   Workspace w;
@@ -764,7 +787,7 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
             const int32_t* query_start, int tokens, int rows, int width, int block_size, int q_heads, int kv_heads,
             int head_dim, int dtype, float scale, int groups, const int32_t* group_start, const int32_t* prefix_blocks,
             int prefix_common, void* out, int64_t out_stride_token, int64_t out_stride_head, float* lse, void* workspace,
-            size_t workspace_bytes, uint32_t* status) {
+            size_t workspace_bytes, uint32_t* status, bool scored) {
   if (!q || !kv || !table || !lens || !out) return fail(EKV_EINVAL, "a required device pointer is NULL");
   if (rows <= 0 || tokens <= 0 || width <= 0 || pool_blocks <= 0)
     return fail(EKV_EINVAL, "rows, tokens, width and pool_blocks must be positive");
@@ -800,7 +823,8 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   if ((int64_t)tokens * q_heads > 0x7fffffffll / 4) return fail(EKV_ENOTSUP, "more than 2^29 query rows");
   c.mt[0] = pick_mt(tokens, rows, G);
   c.mt[1] = groups > 0 ? pick_mt(tokens, groups, G) : 0;
-  const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, c.mt);
+  const int64_t logits = scored ? kept_logits(tokens, rows, width, block_size, q_heads, kv_heads) : 0;
+  const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, c.mt, logits);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
   int rc = current_device(&c.device);
@@ -817,6 +841,10 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   p.heads = kv_heads; p.G = G; p.q_heads = q_heads; p.pool_blocks = pool_blocks; p.tokens = tokens;
   p.groups = groups; p.group_start = group_start; p.prefix_blocks = prefix_blocks; p.prefix_common = prefix_common;
   p.status = status;
+  if (logits > 0) {
+    p.logits = reinterpret_cast<float*>(c.ws + w.logits);
+    p.logits_s0 = logits_row(width, block_size);
+  }
   return encode_cache_maps(p, kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, head_dim, dtype);
 }
 
@@ -834,7 +862,15 @@ extern "C" size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, i
   if (rows <= 0 || tokens <= 0 || groups < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
   const int G = q_heads / kv_heads;
   const int mt[2] = {pick_mt(tokens, rows, G), groups > 0 ? pick_mt(tokens, groups, G) : 0};
-  return workspace_layout(rows, tokens, groups, q_heads, head_dim, mt).total;
+  return workspace_layout(rows, tokens, groups, q_heads, head_dim, mt, 0).total;
+}
+
+extern "C" size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,
+                                                    int head_dim) {
+  if (rows <= 0 || tokens <= 0 || width <= 0 || block_size <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads)
+    return 0;
+  const int mt[2] = {pick_mt(tokens, rows, q_heads / kv_heads), 0};
+  return workspace_layout(rows, tokens, 0, q_heads, head_dim, mt, kept_logits(tokens, rows, width, block_size, q_heads, kv_heads)).total;
 }
 
 extern "C" int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
@@ -850,7 +886,7 @@ extern "C" int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_strid
   const int rc = prepare(c, q, q_stride_token, q_stride_head, kv, kv_stride_block, kv_stride_part, kv_stride_pos,
                          kv_stride_head, pool_blocks, table, table_stride, lens, query_start, tokens, rows, width, block_size,
                          q_heads, kv_heads, head_dim, dtype, scale, groups, group_start, prefix_blocks, prefix_common, out,
-                         out_stride_token, out_stride_head, lse, workspace, workspace_bytes, status);
+                         out_stride_token, out_stride_head, lse, workspace, workspace_bytes, status, false);
   return rc != EKV_OK ? rc : run(c, head_dim, dtype, static_cast<cudaStream_t>(stream));
 }
 
@@ -874,7 +910,7 @@ extern "C" int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t 
   int rc = prepare(c, q, q_stride_token, q_stride_head, kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head,
                    pool_blocks, table, table_stride, lens, query_start, tokens, rows, width, block_size, q_heads, kv_heads,
                    head_dim, dtype, scale, 0, nullptr, nullptr, 0, out, out_stride_token, out_stride_head, lse, workspace,
-                   workspace_bytes, status);
+                   workspace_bytes, status, true);
   if (rc != EKV_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   rc = run(c, head_dim, dtype, s);

@@ -47,6 +47,8 @@ struct AttendParams {
   const int32_t* prefix_blocks;  // [groups], or NULL: prefix_common
   int prefix_common;
   uint32_t* status;
+  float* logits;      // [tokens][q_heads][logits_s0] scores in powers of two, or NULL
+  int64_t logits_s0;
   // the workspace. With groups, what plan_kernel leaves:
   int4* row_info;    // [rows] q0, nq, from, to
   int4* group_info;  // [groups] q0, nq, table row, to
@@ -221,16 +223,6 @@ __device__ __forceinline__ float log2_fast(float x) {
 constexpr float kLn2 = 0.69314718055994531f;
 
 // ---- host ---------------------------------------------------------------------------------------------------
-
-// The SMs of a device, asked once.
-inline int sm_count(int device, int* sms) {
-  static int known[kMaxDevices] = {};
-  if (known[device] == 0 &&
-      cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return check_launch("cudaDeviceGetAttribute");
-  *sms = known[device];
-  return EKV_OK;
-}
 
 // What a kernel of one instantiation was last set up for on each device: the attribute and occupancy calls cost
 // microseconds, and only a batch of another number of rows changes the shared memory it asks for.

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "attend.cuh"
+#include "mma5.cuh"
 
 namespace ekv {
 
@@ -44,87 +45,6 @@ struct WideTail {
   uint32_t tmem;
   int scratch[kThreads / 32 + 1];
 };
-
-// ---- tensor memory and descriptors ---------------------------------------------------------------------
-
-__device__ __forceinline__ void tmem_ld32(float* r, uint32_t addr) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
-        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
-        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(addr));
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]),
-      "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]),
-      "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
-}
-
-// Waits for the loads; naming the values keeps their first use behind the wait.
-template <int N>
-__device__ __forceinline__ void tmem_wait_ld(float (&r)[N]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i]));
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// One lane of the converged warp, always the same one. The issuing code goes by this vote and not by the lane's
-// number, and its addresses are made of values that are the same in the whole warp: then the tensor-core instructions
-// take them from uniform registers (with per-lane ones each instruction took 115 cycles to issue, twice its work).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t chosen;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
-  return chosen != 0;
-}
-
-// A shared-memory operand in the 128-byte swizzle, in two words: where it starts with the distance `lead` in bytes
-// between 64-element groups of the major dimension, and (constant) 1024 bytes between groups of eight rows.
-__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t lead) { return (addr & 0x3ffff) >> 4 | (lead >> 4) << 16; }
-constexpr uint32_t kOperandHigh = 1024u >> 4 | 1u << 14 | 2u << 29;
-
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kOperandHigh)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(kOperandHigh)
-      : "memory");
-}
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -239,10 +159,8 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       if (uses > 0) mbar_wait_bounded(&tail.full[s], (uses - 1) & 1, p.status);
     }
   } else if (warp == kMmaWarp) {
-    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t kShape = 1u << 4 | kType << 7 | kType << 10 | (uint32_t)(kSub >> 4) << 24;
-    constexpr uint32_t kScores = kShape | (uint32_t)(kTokens >> 3) << 17;
-    constexpr uint32_t kOutput = kShape | 1u << 16 | (uint32_t)(D >> 3) << 17;  // the values' tokens are their rows
+    constexpr uint32_t kScores = mma_shape<std::is_same<T, __half>::value>(kTokens, false);
+    constexpr uint32_t kOutput = mma_shape<std::is_same<T, __half>::value>(D, true);
     const uint32_t q_at = smem_u32(queries), ring_at = smem_u32(ring);
     const uint32_t tm = __shfl_sync(kFullMask, tmem, 0);
     int slot = 0;

@@ -1,21 +1,27 @@
 // The attention weight that cached tokens receive, accumulated per (row, KV head, token).
 //
 // Mathematics. Once the attention has left each query row's log-sum-exp, the weight of query row i on token t
-// is p = exp(scale q_i.k_t - lse_i), so a token's weight w_t = sum_i p needs the keys alone and no second softmax:
-// scores_t becomes w_t for a token with no score yet and decay * scores_t + w_t for the others.
+// is p = exp(scale q_i.k_t - lse_i), so a token's weight w_t = sum_i p needs no second softmax: scores_t becomes w_t for
+// a token with no score yet and decay * scores_t + w_t for the others. Every token's sum is one thread's, in a fixed
+// order; nothing is added atomically.
 //
-// score_kernel walks tiles of 64 tokens as attend_kernel does (attend.cuh), keys only. A math warp takes 16 of the
-// tile's tokens as the rows of mma.sync m16n8k16 and eight query rows as its columns, so a token's sum is two
-// registers and two shuffles, in a fixed order; every token belongs to one CTA and nothing is added atomically.
+// Few query rows (decode): the attention kernel has left its logits, and add_kernel reads them back, 4 bytes a token
+// and query row, mostly from L2 (64 rows of 4096 tokens, four query rows a KV head: see the figures at launch_score_kernel).
+//
+// Many query rows (a window that scores a prompt): weigh_kernel multiplies the keys again, on the tcgen05 tensor cores with
+// the roles turned: 128 tokens are the rows of the product and up to 256 query rows its columns, so a token is a lane of
+// tensor memory, its thread reads the columns 32 at a time, takes their exponentials and adds them up in a register. Two
+// warpgroups take alternate tiles. The exponentials bound it: 16 a clock and SM, 2048 clocks for 128 x 256 against 1024
+// of the products.
+#include <algorithm>
+#include <type_traits>
+
 #include "attend.cuh"
+#include "mma5.cuh"
 
 namespace ekv {
 
 namespace {
-
-constexpr int kMathWarps = 4;
-constexpr int kThreads = (kMathWarps + 1) * 32;
-constexpr int kOneTile = 1 << 30;  // query rows of an M tile: a unit's rows are all in one
 
 struct ScoreParams {
   AttendParams a;
@@ -27,26 +33,9 @@ struct ScoreParams {
   float decay;
 };
 
-template <int D>
-struct Ring {
-  static constexpr int kHalves = D / 64;
-  static constexpr int kStage = kHalves * kTile * 128;
-  static constexpr int kStages = 5;
-  static constexpr int kBytes = kStages * kStage;
-};
+constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D>
-struct Tail {
-  uint64_t full[Ring<D>::kStages], empty[Ring<D>::kStages];
-  uint32_t blocks[Ring<D>::kStages];
-  int scratch[kThreads / 32 + 1];
-};
-
-__device__ __forceinline__ uint32_t chunk_at(int t, int c) {
-  return (uint32_t)(c >> 3) * (kTile * 128) + (uint32_t)t * 128 + (uint32_t)((c & 7) ^ (t & 7)) * 16;
-}
-
-// The score row of batch row r, or -1: none is wanted, or the slot is not one row's alone.
+// The score row of batch row r, or -1: none is wanted, or the slot is not one row's alone. With the whole warp.
 __device__ __forceinline__ int slot_of(const ScoreParams& p, int r, int lane) {
   if (p.slots == nullptr) return r < p.n_slots ? r : -1;
   const int slot = p.slots[r];
@@ -58,149 +47,288 @@ __device__ __forceinline__ int slot_of(const ScoreParams& p, int r, int lane) {
   return bad ? -1 : slot;
 }
 
+// ---- from the attention's logits ---------------------------------------------------------------------------
+
+constexpr int kAddThreads = 256;
+
+// CTAs of a (row, KV head) take its tokens 4 a thread; a warp's 128 tokens are read from every query row in turn.
+__global__ void __launch_bounds__(kAddThreads) add_kernel(const __grid_constant__ ScoreParams sp) {
+  const AttendParams& p = sp.a;
+  chain_release();
+  chain_wait();  // the logits and the log-sum-exps
+  const int row = blockIdx.x / p.heads, head = blockIdx.x - row * p.heads;
+  const Unit un = unit_at<false>(p, row, false);
+  const int M = un.q.nq * p.G;
+  if (M == 0) return;
+  const int slot = slot_of(sp, row, threadIdx.x & 31);
+  if (slot < 0) return;
+  const int fresh = sp.fresh != nullptr ? sp.fresh[row] : un.q.nq;
+  const int old_end = un.to - max(fresh, 0);  // tokens from here on have no score yet
+  float* dst = sp.scores + (int64_t)slot * sp.s0 + (int64_t)head * sp.s1;
+  const float* first = p.logits + ((int64_t)un.q.q0 * p.q_heads + head * p.G) * p.logits_s0;
+  const float* lses = p.lse + (int64_t)un.q.q0 * p.q_heads + head * p.G;
+  for (int pos = 4 * (blockIdx.y * kAddThreads + threadIdx.x); pos < un.to; pos += 4 * gridDim.y * kAddThreads) {
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < un.q.nq; ++i) {
+#pragma unroll 4
+      for (int g = 0; g < p.G; ++g) {
+        const float lse = lses[(int64_t)i * p.q_heads + g] * kLog2e;
+        if (lse == -INFINITY) continue;  // it saw nothing
+        const float4 x = *reinterpret_cast<const float4*>(first + ((int64_t)i * p.q_heads + g) * p.logits_s0 + pos);
+        w[0] += exp2_fast(x.x - lse);
+        w[1] += exp2_fast(x.y - lse);
+        w[2] += exp2_fast(x.z - lse);
+        w[3] += exp2_fast(x.w - lse);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (pos + e < un.to)
+        dst[pos + e] = pos + e >= old_end || sp.decay == 0.f ? w[e] : fmaf(sp.decay, dst[pos + e], w[e]);
+  }
+}
+
+// ---- from the keys --------------------------------------------------------------------------------------------
+
+constexpr int kOneTile = 1 << 30;  // query rows of an M tile of the plan: a unit's rows are all in one
+constexpr int kTokens = 128;
+constexpr int kColumns = 256;  // query rows at a time
+constexpr int kThreads = 320;
+constexpr int kCopyWarp = 8, kMmaWarp = 9;
+
+template <int D>
+struct Ring {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kHalf = kTokens * 128;
+  static constexpr int kSlot = kHalves * kHalf;
+  static constexpr int kSlots = 4;
+  static constexpr int kBytes = kSlots * kSlot;
+  static constexpr int kQueryHalf = kColumns * 128;
+  static constexpr int kQueries = kHalves * kQueryHalf;
+};
+
+template <int D>
+struct Tail {
+  uint64_t full[Ring<D>::kSlots], empty[Ring<D>::kSlots], q_full, s_full[2], s_free[2], drained;
+  uint32_t tmem;
+  int scratch[kThreads / 32 + 1];
+  alignas(16) float lse[kColumns];
+  alignas(16) int limit[kColumns];
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) score_kernel(const __grid_constant__ ScoreParams sp) {
+__global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constant__ ScoreParams sp) {
   using R = Ring<D>;
   const AttendParams& p = sp.a;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* queries = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* ring = queries + R::kQueries;
   Tail<D>& tail = *reinterpret_cast<Tail<D>*>(ring + R::kBytes);
   const Plan plan{reinterpret_cast<int*>(ring + R::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16), p.rows};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < R::kStages; ++s) {
+    for (int s = 0; s < R::kSlots; ++s) {
       mbar_init(&tail.full[s], 1);
-      mbar_init(&tail.empty[s], kMathWarps);
+      mbar_init(&tail.empty[s], 1);
     }
+    mbar_init(&tail.q_full, 256);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&tail.s_full[w], 1);
+      mbar_init(&tail.s_free[w], 128);
+    }
+    mbar_init(&tail.drained, 1);
     fence_mbar_init();
   }
   chain_wait();  // the attention's log-sum-exps
-  make_plan<false, kThreads>(p, plan, kOneTile, tail.scratch);
+  make_plan<false, kThreads, kTokens>(p, plan, kOneTile, tail.scratch);
   chain_release();
   const int W = plan.cum[plan.units];
   const int n = sharing_ctas(W, gridDim.x);
   if ((int)blockIdx.x >= n || W == 0) return;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tail.tmem;
   const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
-  const int per_tile = kTile >> p.block_shift;
+  const int per_tile = kTokens >> p.block_shift;
+  bool good = true;  // after a wait that gave up a role goes on without waiting, so that every role ends
 
-  if (warp == kMathWarps) {  // ---- the copy warp --------------------------------------------------------
+  if (warp == kCopyWarp) {
     const uint64_t policy = l2_evict_first_policy();
     const uint32_t block_bytes = (uint32_t)p.block_size * 128u;
-    int stage = 0, issued = 0;
+    int slot = 0, issued = 0;
     uint32_t phase = 0;
-    bool good = true;
     for (int t = begin; t < end && good;) {
-      const Item it = item_at<false>(p, plan, kOneTile, t, end);
+      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
       const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
       const int last_block = (it.un.to - 1) >> p.block_shift;
-      const bool mine = lane < per_tile;
-      int id = mine && lane + it.first * per_tile <= last_block ? ids[lane + it.first * per_tile] : -2;
-      for (int tile = it.first; tile < it.last && good; ++tile, ++t) {
-        const int b = lane + tile * per_tile;
-        const int next = tile + 1 < it.last && mine && b + per_tile <= last_block ? ids[b + per_tile] : -2;
-        if (issued >= R::kStages) good = mbar_wait_bounded(&tail.empty[stage], phase ^ 1, p.status);
-        good = __all_sync(kFullMask, good);
-        if (!good) break;
-        const bool ok = mine && b <= last_block && id >= 0 && (int64_t)id < p.pool_blocks;
-        const uint32_t which = __ballot_sync(kFullMask, ok);
-        if (lane == 0) {
-          tail.blocks[stage] = which;
-          mbar_arrive_expect_tx(&tail.full[stage], (uint32_t)__popc(which) * block_bytes * R::kHalves);
-        }
-        __syncwarp();
-        if (ok) {
-          const uint32_t at = smem_u32(ring) + stage * R::kStage + lane * block_bytes;
+      for (int m0 = 0; m0 < it.un.q.nq * p.G && good; m0 += kColumns) {
+        for (int tile = it.first; tile < it.last; ++tile) {
+          if (issued >= R::kSlots) good = mbar_wait_bounded(&tail.empty[slot], phase ^ 1, p.status);
+          good = __all_sync(kFullMask, good);
+          if (!good) break;
+          if (lane == 0) mbar_arrive_expect_tx(&tail.full[slot], R::kSlot);
+          __syncwarp();
+          if (lane < per_tile) {
+            const int b = tile * per_tile + lane;
+            int id = b <= last_block ? ids[b] : -2;
+            if (id < 0 || (int64_t)id >= p.pool_blocks) id = (int)p.pool_blocks;  // past the tensor: zeros
+            const uint32_t at = smem_u32(ring) + slot * R::kSlot + lane * block_bytes;
 #pragma unroll
-          for (int h = 0; h < R::kHalves; ++h)
-            tensor_copy_4d(at + h * (kTile * 128), &p.kmap, 64 * h, it.head, 0, id, &tail.full[stage], policy);
+            for (int h = 0; h < R::kHalves; ++h)
+              tensor_copy_4d(at + h * R::kHalf, &p.kmap, 64 * h, it.head, 0, id, &tail.full[slot], policy);
+          }
+          ++issued;
+          if (++slot == R::kSlots) slot = 0, phase ^= 1;
         }
-        id = next;
-        ++issued;
-        if (++stage == R::kStages) stage = 0, phase ^= 1;
       }
+      t += it.last - it.first;
     }
-    for (int s = 0; s < R::kStages; ++s) {  // no CTA leaves with copies in flight
-      const int uses = issued > s ? (issued - s - 1) / R::kStages + 1 : 0;
+    for (int s = 0; s < R::kSlots; ++s) {  // no CTA leaves with copies in flight
+      const int uses = issued > s ? (issued - s - 1) / R::kSlots + 1 : 0;
       if (uses > 0) mbar_wait_bounded(&tail.full[s], (uses - 1) & 1, p.status);
     }
-    return;
-  }
-
-  // ---- the math warps ---------------------------------------------------------------------------------------
-  const int quad = lane >> 2, pair = lane & 3;
-  int stage = 0;
-  uint32_t phase = 0;
-  bool good = true;
-  for (int t = begin; t < end;) {
-    const Item it = item_at<false>(p, plan, kOneTile, t, end);
-    const QueryRange uq = it.un.q;
-    const int to = it.un.to, M = uq.nq * p.G;
-    const int slot = slot_of(sp, it.unit, lane);
-    const int fresh = sp.fresh != nullptr ? sp.fresh[it.unit] : uq.nq;
-    const int old_end = to - max(fresh, 0);  // tokens from here on have no score yet
-    float* dst = sp.scores + (int64_t)max(slot, 0) * sp.s0 + (int64_t)it.head * sp.s1;
-    for (int tile = it.first; tile < it.last; ++tile, ++t) {
-      if (good) good = mbar_wait_bounded(&tail.full[stage], phase, p.status);
-      const uint32_t keys = smem_u32(ring) + stage * R::kStage;
-      const uint32_t blocks = tail.blocks[stage];
-      uint32_t kf[D / 16][4];
+  } else if (warp == kMmaWarp) {
+    const uint32_t tm = __shfl_sync(kFullMask, tmem, 0);
+    const uint32_t q_low = operand_low(smem_u32(queries), 16), ring_low = operand_low(smem_u32(ring), 16);
+    int slot = 0;
+    uint32_t phase = 0, q_uses = 0, uses[2] = {0, 0};
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (good) good = mbar_wait_bounded(bar, parity, p.status);
+      good = __all_sync(kFullMask, good);
+      tc_fence_after();
+    };
+    for (int t = begin; t < end;) {
+      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
+      const int M = it.un.q.nq * p.G;
+      for (int m0 = 0; m0 < M; m0 += kColumns) {
+        const uint32_t shape = mma_shape<std::is_same<T, __half>::value>((min(M - m0, kColumns) + 15) / 16 * 16, false);
+        wait(&tail.q_full, q_uses++ & 1);
+        for (int j = 0; j < it.last - it.first; ++j) {
+          const int w = j & 1;
+          wait(&tail.full[slot], phase);
+          if (uses[w] > 0) wait(&tail.s_free[w], (uses[w] - 1) & 1);
+          ++uses[w];
+          if (good && elect_one()) {
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        ldmatrix_x4(kf[k], keys + chunk_at(warp * 16 + (lane & 15), 2 * k + (lane >> 4)));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tail.empty[stage]);  // the keys are in registers
-      if (++stage == R::kStages) stage = 0, phase ^= 1;
-      const int pos[2] = {tile * kTile + warp * 16 + quad, tile * kTile + warp * 16 + quad + 8};
-      float w[2] = {0.f, 0.f};
-      for (int m0 = 0; m0 < M; m0 += 8) {
-        const int mq = m0 + quad;  // the query row of this lane's operand
-        const bool real = mq < M;
-        const T* src = static_cast<const T*>(p.q) + (int64_t)(uq.q0 + mq / p.G) * p.q_s0 +
-                       (int64_t)(it.head * p.G + mq % p.G) * p.q_s1 + 2 * pair;
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t b[2] = {real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u,
-                                 real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u};
-          Mma<T>::run(c, kf[k], b);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {  // this lane's two result columns
-          const int m = m0 + 2 * pair + e;
-          if (m >= M) continue;
-          const int i = m / p.G;
-          const float lse = p.lse[(int64_t)(uq.q0 + i) * p.q_heads + it.head * p.G + (m - i * p.G)];
-          if (lse == -INFINITY) continue;
-          const float base = lse * 1.4426950408889634f;
-          const int limit = to - uq.nq + i + 1;
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (pos[j] < limit) w[j] += exp2_fast(fmaf(c[2 * j + e], p.scale_log2, -base));
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(tm + w * kColumns, ring_low + slot * (R::kSlot >> 4) + (((uint32_t)(k >> 2) * R::kHalf + (k & 3) * 32) >> 4),
+                     q_low + (((uint32_t)(k >> 2) * R::kQueryHalf + (k & 3) * 32) >> 4), shape, k > 0);
+          }
+          if (elect_one()) tc_commit(&tail.s_full[w]);
+          if (elect_one()) tc_commit(&tail.empty[slot]);
+          if (++slot == R::kSlots) slot = 0, phase ^= 1;
         }
       }
+      t += it.last - it.first;
+    }
+    if (elect_one()) tc_commit(&tail.drained);
+    mbar_wait_bounded(&tail.drained, 0, p.status);
+  } else {  // ---- the warpgroups that add ----------------------------------------------------------------------
+    const int w = warp >> 2, token_lane = threadIdx.x & 127, column = threadIdx.x;  // column: the query row this thread loads
+    const uint32_t s_at = tmem + w * kColumns + ((uint32_t)(warp & 3) << 21);
+    uint32_t s_uses = 0;
+    for (int t = begin; t < end;) {
+      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
+      const QueryRange uq = it.un.q;
+      const int to = it.un.to, M = uq.nq * p.G;
+      const int slot = slot_of(sp, it.unit, lane);
+      const int fresh = sp.fresh != nullptr ? sp.fresh[it.unit] : uq.nq;
+      const int old_end = to - max(fresh, 0);  // tokens from here on have no score yet
+      float* dst = sp.scores + (int64_t)max(slot, 0) * sp.s0 + (int64_t)it.head * sp.s1;
+      const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
+      const int last_block = (to - 1) >> p.block_shift;
+      for (int m0 = 0; m0 < M; m0 += kColumns) {
+        const int count = min(M - m0, kColumns), padded = (count + 15) / 16 * 16;
+        named_barrier(1, 256);  // every product with the queries before is complete, and every read of their sums
+        if (column < padded) {
+          const int m = m0 + column, i = m / p.G, qhead = it.head * p.G + m - i * p.G;
+          const bool real = column < count;
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(uq.q0 + i) * p.q_s0 + (int64_t)qhead * p.q_s1);
+          const uint32_t at = smem_u32(queries) + column * 128;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        w[j] += __shfl_xor_sync(kFullMask, w[j], 1);
-        w[j] += __shfl_xor_sync(kFullMask, w[j], 2);
-        const int tk = warp * 16 + quad + 8 * j;
-        if (!((blocks >> (tk >> p.block_shift)) & 1u)) w[j] = 0.f;  // keys that were not read
-        if (pair == 0 && slot >= 0 && pos[j] < to)
-          dst[pos[j]] = pos[j] >= old_end || sp.decay == 0.f ? w[j] : fmaf(sp.decay, dst[pos[j]], w[j]);
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 v = real ? src[c] : make_uint4(0, 0, 0, 0);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (c >> 3) * R::kQueryHalf + (((c & 7) ^ (column & 7)) << 4)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                         : "memory");
+          }
+          const float lse = real ? p.lse[(int64_t)(uq.q0 + i) * p.q_heads + qhead] : -INFINITY;
+          tail.lse[column] = lse == -INFINITY ? INFINITY : lse * kLog2e;  // no weight from a query that saw nothing
+          tail.limit[column] = real ? to - uq.nq + i + 1 : 0;
+        }
+        proxy_fence_smem();
+        mbar_arrive(&tail.q_full);
+        named_barrier(1, 256);
+        for (int tile = it.first + w; tile < it.last; tile += 2) {
+          const int b = tile * per_tile + lane;
+          const int id = lane < per_tile && b <= last_block ? ids[b] : 0;
+          const uint32_t missing = __ballot_sync(kFullMask, id < 0 || (int64_t)id >= p.pool_blocks);
+          if (good) good = mbar_wait_bounded(&tail.s_full[w], s_uses & 1, p.status);
+          ++s_uses;
+          tc_fence_after();
+          __syncwarp();
+          const int pos = tile * kTokens + token_lane;
+          const bool inner = (tile + 1) * kTokens <= to - uq.nq + 1;  // every query token sees the whole tile
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int c = 0; c < count; c += 32) {
+            float s[32];
+            tmem_ld32(s, s_at + c);
+            tmem_wait_ld(s);
+            const float4* lse = reinterpret_cast<const float4*>(tail.lse + c);
+            if (inner && c + 32 <= count) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float4 v = lse[k];
+                sum[0] += exp2_fast(fmaf(s[4 * k], p.scale_log2, -v.x));
+                sum[1] += exp2_fast(fmaf(s[4 * k + 1], p.scale_log2, -v.y));
+                sum[2] += exp2_fast(fmaf(s[4 * k + 2], p.scale_log2, -v.z));
+                sum[3] += exp2_fast(fmaf(s[4 * k + 3], p.scale_log2, -v.w));
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const int at = min(c + k, kColumns - 1);
+                const float v = exp2_fast(fmaf(s[k], p.scale_log2, -tail.lse[at]));
+                if (c + k < count && pos < tail.limit[at]) sum[k & 3] += v;
+              }
+            }
+          }
+          tc_fence_before();
+          mbar_arrive(&tail.s_free[w]);
+          float weight = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          if (missing >> (token_lane >> p.block_shift) & 1u) weight = 0.f;  // keys that were not read
+          if (slot >= 0 && pos < to) {  // this thread's token in every round of query rows
+            const float old = m0 > 0 ? dst[pos] : (pos >= old_end || sp.decay == 0.f ? 0.f : sp.decay * dst[pos]);
+            dst[pos] = old + weight;
+          }
+        }
       }
+      t += it.last - it.first;
     }
   }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 template <typename T, int D>
-int launch_scores(const ScoreParams& p, int device, int sms, cudaStream_t s) {
-  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows);
-  auto kernel = score_kernel<T, D>;
+int launch_weigh(const ScoreParams& p, int device, int sms, cudaStream_t s) {
+  const size_t smem = 1024 + Ring<D>::kQueries + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows);
+  auto kernel = weigh_kernel<T, D>;
   static LaunchCache cache;
   int resident = 0;
-  const int rc = prepare_launch(cache, kernel, "score_kernel", device, kThreads, smem, &resident);
+  const int rc = prepare_launch(cache, kernel, "weigh_kernel", device, kThreads, std::max(smem, (size_t)120 * 1024), &resident);
   if (rc != EKV_OK) return rc;
-  launch_chained(kernel, dim3(min(resident * sms, kAttendMaxCtas)), dim3(kThreads), smem, s, p);
-  return check_launch("score_kernel");
+  // more than half of an SM's shared memory: one CTA an SM, which takes all of its tensor memory
+  launch_chained(kernel, dim3(sms), dim3(kThreads), std::max(smem, (size_t)120 * 1024), s, p);
+  return check_launch("weigh_kernel");
 }
 
 }  // namespace
@@ -208,9 +336,16 @@ int launch_scores(const ScoreParams& p, int device, int sms, cudaStream_t s) {
 int launch_score_kernel(const AttendParams& a, int dim, int dtype, float* scores, int64_t s0, int64_t s1,
                         const int32_t* slots, const int32_t* fresh, int n_slots, float decay, int device, int sms, cudaStream_t s) {
   const ScoreParams p{a, scores, s0, s1, slots, fresh, n_slots, decay};
+  if (a.logits != nullptr) {
+    // about eight CTAs an SM, or one for every 4 KB of a row's logits
+    const int64_t units = (int64_t)a.rows * a.heads, chunks = (a.logits_s0 + 4 * kAddThreads - 1) / (4 * kAddThreads);
+    const int64_t spread = std::min(chunks, std::max<int64_t>(1, 8ll * sms / units));
+    launch_chained(add_kernel, dim3((unsigned)units, (unsigned)std::min<int64_t>(spread, 65535)), dim3(kAddThreads), 0, s, p);
+    return check_launch("add_kernel");
+  }
   if (dtype == EKV_DTYPE_BF16)
-    return dim == 128 ? launch_scores<__nv_bfloat16, 128>(p, device, sms, s) : launch_scores<__nv_bfloat16, 64>(p, device, sms, s);
-  return dim == 128 ? launch_scores<__half, 128>(p, device, sms, s) : launch_scores<__half, 64>(p, device, sms, s);
+    return dim == 128 ? launch_weigh<__nv_bfloat16, 128>(p, device, sms, s) : launch_weigh<__nv_bfloat16, 64>(p, device, sms, s);
+  return dim == 128 ? launch_weigh<__half, 128>(p, device, sms, s) : launch_weigh<__half, 64>(p, device, sms, s);
 }
 
 }  // namespace ekv

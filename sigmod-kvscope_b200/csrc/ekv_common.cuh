@@ -27,6 +27,16 @@ constexpr int kMaxDevices = 64;  // per-device one-time kernel attributes
 // for an ordinal at or past kMaxDevices (the per-device caches of the entry points hold that many).
 int current_device(int* device);
 
+// The SMs of a device, asked once.
+inline int sm_count(int device, int* sms) {
+  static int known[kMaxDevices] = {};
+  if (known[device] == 0 &&
+      cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return check_launch("cudaDeviceGetAttribute");
+  *sms = known[device];
+  return EKV_OK;
+}
+
 inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 

@@ -2,16 +2,23 @@
 // moved to the front of the row's blocks.
 //
 // select_kernel. A token's rank is its score (float32; NaN as -inf), equal scores to the older token; a row's first
-// and newest tokens are kept whatever they score. One CTA per (row, KV head): the scores as order-preserving 32-bit
-// keys, four passes of an 8-bit digit each find the key of the last token kept and how many equal to it are
-// (a histogram in shared memory, counted in integers: no order matters), and one ordered pass writes the kept
-// positions, ascending, then -1.
+// and newest tokens are kept whatever they score. A cluster of CTAs per (row, KV head), each with a slice of the row and
+// each warp with a run of it: the scores become order-preserving 32-bit keys in registers (up to 32 a lane; longer rows
+// are read again for each pass), four passes of an 8-bit digit each find the key of the last token kept and how many
+// equal to it are, and the warps write the kept positions of their runs, ascending, then -1. Scores crowd into a few exponents, so every lane counts in its
+// own column of bins, which is a bank of its own (with one histogram for all lanes, or eight, the additions of the first
+// pass waited for one another: 8 us of 8 x 8 units of 65536 tokens). The CTAs' counts are added through distributed
+// shared memory, in integers: no order matters.
 //
 // compact: position j of a (row, head) takes the key, value and score of position kept[j] >= j, in place, in
 // chunks: a chunk's sources are all read before any of it is written, and later chunks only read positions past
 // it, so the copy that fills chunk k + 1 may run while chunk k is stored. check_kernel comes first: the list must ascend
 // strictly, from the identity on the protected first tokens, and no block the row writes may be another row's, or
 // occur twice in the row (each block a row holds is claimed once in an owner table); a row that fails is left as it was.
+#include <cooperative_groups.h>
+
+#include <mutex>
+
 #include "ekv_common.cuh"
 
 namespace ekv {
@@ -36,6 +43,8 @@ struct SelectParams {
 };
 
 constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
+static_assert(kSelectWarps == 16, "the last walk's sums over warps and CTAs");
 
 __device__ __forceinline__ uint32_t score_key(float x) {  // larger is better; -0 as 0
   if (isnan(x)) x = -INFINITY;
@@ -43,16 +52,29 @@ __device__ __forceinline__ uint32_t score_key(float x) {  // larger is better; -
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const __grid_constant__ SelectParams p) {
-  __shared__ int s_hist[256];
-  __shared__ int s_scan[kSelectThreads / 32 + 1];
+// KEYS: keys of a lane that stay in registers; 0: rows too long for that.
+template <int KEYS>
+__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_constant__ SelectParams p) {
+  namespace cg = cooperative_groups;
+  // few keys a lane: one histogram will do, and saves the step that adds the lanes' columns
+  constexpr bool kColumns = KEYS == 0 || KEYS > 8;
+  __shared__ int s_lanes[kColumns ? 256 : 1][32];
+  __shared__ int s_sum[256];
+  __shared__ __align__(16) int s_hist[2][256];
   __shared__ int s_pick[2];
+  __shared__ int s_count[2][kSelectWarps];  // per warp: tokens kept anyway or above, tokens equal to the last kept
+  __shared__ int s_total[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
   chain_release();
   chain_wait();
-  const int row = blockIdx.x / p.heads, head = blockIdx.x - row * p.heads;
+  const int unit = blockIdx.x / C;
+  const int row = unit / p.heads, head = unit - row * p.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n = max(p.lens[row], 0);
   int slot = p.slots != nullptr ? p.slots[row] : row;
-  if (threadIdx.x == 0 && head == 0) {
+  const bool reports = threadIdx.x == 0 && rank == 0 && head == 0;
+  if (reports) {
     if (n > p.capacity) set_status(p.status, EKV_STATUS_LEN_OVER_WIDTH);
     if (slot >= p.n_slots) set_status(p.status, EKV_STATUS_BAD_SLOT);
   }
@@ -62,69 +84,153 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(const __grid_con
   const int first = min(p.first, n), recent = min(p.recent, n - first);
   const int m = keep < 0 || keep >= n || slot < 0 ? n : max(keep, first + recent);
   int32_t* out = p.kept + (int64_t)row * p.k0 + (int64_t)head * p.k1;
-  if (threadIdx.x == 0 && head == 0) p.new_lens[row] = m;
-  if (m == n) {
-    for (int i = threadIdx.x; i < p.capacity; i += kSelectThreads) out[i] = i < n ? i : -1;
+  if (reports) p.new_lens[row] = m;
+  if (m == n) {  // the same for every CTA of the cluster
+    for (int i = rank * kSelectThreads + threadIdx.x; i < p.capacity; i += C * kSelectThreads) out[i] = i < n ? i : -1;
     return;
   }
   const float* scores = p.scores + (int64_t)slot * p.s0 + (int64_t)head * p.s1;
-  const int lo = first, hi = n - recent;  // the tokens to choose from
-  int want = m - first - recent;          // >= 0, < hi - lo
+  // a warp's run of tokens [from, to)
+  const int run = KEYS > 0 ? 32 * KEYS : (((n + C - 1) / C + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+  const int from = min(n, (rank * kSelectWarps + warp) * run), to = min(n, from + run);
+  // A token's key: what is kept anyway above every score, what is not the run's below.
+  auto key_of = [&](int i, float x) { return i >= to ? 0u : i < first || i >= n - recent ? 0xffffffffu : score_key(x); };
+  uint32_t keys[KEYS > 0 ? KEYS : 1];
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+      const int i = from + 32 * k + lane;
+      keys[k] = i < to ? __float_as_uint(scores[i]) : 0u;
+    }
+  }
+  for (int i = m + rank * kSelectThreads + threadIdx.x; i < p.capacity; i += C * kSelectThreads) out[i] = -1;
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) keys[k] = key_of(from + 32 * k + lane, __uint_as_float(keys[k]));
+  }
+  // visit(i, key) for the run's tokens, 32 at a time with the whole warp; i may lie behind `to`
+  auto walk = [&](auto visit) {
+    if constexpr (KEYS > 0) {
+#pragma unroll
+      for (int k = 0; k < KEYS; ++k) visit(from + 32 * k + lane, keys[k]);
+    } else {
+      for (int base = from; base < to; base += 32) visit(base + lane, key_of(base + lane, base + lane < to ? scores[base + lane] : 0.f));
+    }
+  };
+  int want = m;  // tokens above the one that is being found: fewer than there are
   uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) s_hist[i] = 0;
+  if (kColumns) {
+    for (int i = threadIdx.x; i < 256 * 32; i += kSelectThreads) (&s_lanes[0][0])[i] = 0;
+  } else {
+    for (int i = threadIdx.x; i < 512; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
+  }
+  __syncthreads();
+  for (int pass = 0; pass < 4; ++pass) {
+    const int shift = 24 - 8 * pass;
+    int* hist = s_hist[pass & 1];
+    walk([&](int, uint32_t key) {
+      const int digit = (key >> shift) & 255;
+      if ((key & mask) == prefix && key != 0u) atomicAdd(kColumns ? &s_lanes[digit][lane] : &hist[digit], 1);
+    });
     __syncthreads();
-    for (int i = lo + threadIdx.x; i < hi; i += kSelectThreads) {
-      const uint32_t key = score_key(scores[i]);
-      if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & 255], 1);
+#pragma unroll
+    for (int d = 0; kColumns && d < 256 / kSelectWarps; ++d) {
+      const int bin = warp * (256 / kSelectWarps) + d;
+      const int count = __reduce_add_sync(kFullMask, s_lanes[bin][lane]);
+      s_lanes[bin][lane] = 0;
+      if (lane == 0) hist[bin] = count;
+    }
+    cluster.sync();  // every CTA's histogram of this pass; the next pass fills the other one
+    if (threadIdx.x < 256) {
+      int count = 0;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < C) count += cluster.map_shared_rank(hist, c)[threadIdx.x];
+      s_sum[threadIdx.x] = count;
+    } else if (!kColumns) {
+      s_hist[(pass + 1) & 1][threadIdx.x - 256] = 0;  // read by every CTA before the barrier above
     }
     __syncthreads();
-    if (threadIdx.x < 32) {  // lane l holds digits [248 - 8 l, 256 - 8 l): from the largest down
-      const int top = 255 - 8 * threadIdx.x;
-      int sum = 0;
-      for (int d = 0; d < 8; ++d) sum += s_hist[top - d];
+    if (warp == 0) {  // lane l holds digits [248 - 8 l, 256 - 8 l): from the largest down
+      const int top = 255 - 8 * lane;
+      int count[8], sum = 0;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) sum += count[d] = s_sum[top - d];
       int incl = sum;
       for (int off = 1; off < 32; off <<= 1) {
         const int v = __shfl_up_sync(kFullMask, incl, off);
-        if ((int)threadIdx.x >= off) incl += v;
+        if (lane >= off) incl += v;
       }
       int before = incl - sum;
       // the digit in which the count of larger keys passes `want`: exactly one lane finds it
       if (before <= want && want < incl) {
-        int d = 0;
-        while (before + s_hist[top - d] <= want) before += s_hist[top - d++];
-        s_pick[0] = top - d;
-        s_pick[1] = want - before;
+        int digit = 0;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const bool here = before <= want && want < before + count[d];
+          if (here) {
+            digit = top - d;
+            s_pick[1] = want - before;
+          }
+          before += count[d];
+        }
+        s_pick[0] = digit;
       }
     }
     __syncthreads();
     prefix |= (uint32_t)s_pick[0] << shift;
     mask |= 255u << shift;
     want = s_pick[1];
-    __syncthreads();
+    __syncthreads();  // before s_pick is written again
   }
-  // keep every key above `prefix` and the `want` oldest equal to it
-  int at = 0, equal = 0;
-  for (int base = 0; base < n; base += kSelectThreads) {
-    const int i = base + threadIdx.x;
-    bool pin = false, above = false, same = false;
-    if (i < n) {
-      pin = i < lo || i >= hi;
-      const uint32_t key = pin ? 0u : score_key(scores[i]);
-      above = !pin && key > prefix;
-      same = !pin && key == prefix;
-    }
-    int same_total = 0, kept_total = 0;
-    const int rank = equal + block_exclusive_scan<kSelectThreads>(same ? 1 : 0, s_scan, &same_total);
-    const bool take = pin || above || (same && rank < want);
-    __syncthreads();
-    const int place = at + block_exclusive_scan<kSelectThreads>(take ? 1 : 0, s_scan, &kept_total);
-    if (take) out[place] = i;
-    at += kept_total;
-    equal += same_total;
-    __syncthreads();
+  // keep every key above `prefix` and the `want` oldest equal to it: counted per warp, then placed
+  int sure = 0, equal = 0;
+  walk([&](int, uint32_t key) {
+    sure += key > prefix;
+    equal += key == prefix;
+  });
+  sure = __reduce_add_sync(kFullMask, sure);
+  equal = __reduce_add_sync(kFullMask, equal);
+  if (lane == 0) {
+    s_count[0][warp] = sure;
+    s_count[1][warp] = equal;
   }
-  for (int i = m + threadIdx.x; i < p.capacity; i += kSelectThreads) out[i] = -1;
+  __syncthreads();
+  if (warp < 2) {
+    const int sum = __reduce_add_sync(kFullMask, lane < kSelectWarps ? s_count[warp][lane] : 0);
+    if (lane == 0) s_total[warp] = sum;
+  }
+  cluster.sync();
+  // lanes 0 to 15 add the warps before this one, lanes 16 to 23 the CTAs before
+  int sure_before = lane < warp ? s_count[0][lane & 15] : 0, equal_before = lane < warp ? s_count[1][lane & 15] : 0;
+  if (lane >= 16 && lane - 16 < rank) {
+    const int* remote = cluster.map_shared_rank(s_total, lane - 16);
+    sure_before = remote[0];
+    equal_before = remote[1];
+  }
+  sure_before = __reduce_add_sync(kFullMask, sure_before);
+  equal_before = __reduce_add_sync(kFullMask, equal_before);
+  const uint32_t below = lanes_below();
+  if (equal == 0) {  // nearly every run: no score equal to the last one kept
+    int place = sure_before + min(equal_before, want);
+    walk([&](int i, uint32_t key) {
+      const bool take = key > prefix;
+      const uint32_t takes = __ballot_sync(kFullMask, take);
+      if (take) out[place + __popc(takes & below)] = i;
+      place += __popc(takes);
+    });
+  } else {
+    walk([&](int i, uint32_t key) {
+      const bool is_sure = key > prefix, is_equal = key == prefix;  // prefix is a score's key: not 0
+      const uint32_t sures = __ballot_sync(kFullMask, is_sure), equals = __ballot_sync(kFullMask, is_equal);
+      const int tied = equal_before + __popc(equals & below);
+      const int place = sure_before + __popc(sures & below) + min(tied, want);
+      if (is_sure || (is_equal && tied < want)) out[place] = i;
+      sure_before += __popc(sures);
+      equal_before += __popc(equals);
+    });
+  }
+  cluster.sync();  // no CTA leaves while another reads its totals
 }
 
 // ---- compact -------------------------------------------------------------------------------------------------
@@ -215,66 +321,113 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveBytes = 32768;  // of a chunk
+constexpr int kMoveWarps = kMoveThreads / 32;
+constexpr int kMoveLoads = 4;  // 16-byte loads of a lane and chunk: 2 KB a warp, 16 KB a CTA, two chunks in flight
 
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const __grid_constant__ CompactParams p) {
-  extern __shared__ __align__(128) uint8_t s_chunk[];  // two chunks, and two of scores behind them
+// A cluster of CTAs per (row, KV head) takes C chunks at a time, one each. SPLIT: keys and values are units of their own.
+__global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_constant__ CompactParams p, int split) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = cluster.num_blocks(), rank = cluster.block_rank();
   chain_release();
   chain_wait();
-  const int row = blockIdx.x / p.heads, head = blockIdx.x - row * p.heads;
+  int unit = blockIdx.x / C;
+  const int only = split ? unit & 1 : 0;  // the part this unit moves
+  if (split) unit >>= 1;
+  const int row = unit / p.heads, head = unit - row * p.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n, m;
-  if (!row_moves(p, row, n, m)) return;
+  if (!row_moves(p, row, n, m)) return;  // as every CTA of the cluster does
   const int bad = p.bad[row];
   if (bad) {
-    if (threadIdx.x == 0 && head == 0)
+    if (threadIdx.x == 0 && rank == 0 && head == 0 && only == 0)
       set_status(p.status, (bad & kRowShared ? EKV_STATUS_BLOCK_SHARED : 0u) | (bad & kRowList ? EKV_STATUS_BAD_LIST : 0u) |
                                (bad & kRowBlock ? EKV_STATUS_BAD_BLOCK_ID : 0u) | (bad & kRowSlot ? EKV_STATUS_BAD_SLOT : 0u));
     return;
   }
-  const int32_t* list = p.kept + (int64_t)row * p.k0 + (int64_t)head * p.k1;
-  const int32_t* ids = p.table + (int64_t)row * p.table_s0;
-  const int slot = p.scores == nullptr ? -1 : (p.slots != nullptr ? p.slots[row] : row);
-  float* scores = slot < 0 ? nullptr : p.scores + (int64_t)slot * p.s0 + (int64_t)head * p.s1;
-  const int pieces = p.row_bytes / 16;          // 16-byte pieces of a key row
-  const int per = kMoveBytes / (2 * p.row_bytes);  // tokens of a chunk
-  float* s_scores = reinterpret_cast<float*>(s_chunk + 2 * kMoveBytes);
-  auto place = [&](int pos, int part, int piece) {
-    const int b = pos / p.block_size;
-    return p.kv + (int64_t)ids[b] * p.c_block + part * p.c_part + (int64_t)(pos - b * p.block_size) * p.c_pos +
-           (int64_t)head * p.c_head + 16 * piece;
-  };
-  auto load = [&](int j0, int buf) {
-    const int count = min(per, m - j0) * 2 * pieces;
-    for (int i = threadIdx.x; i < count; i += kMoveThreads) {
-      const int j = i / (2 * pieces), rest = i - j * 2 * pieces, part = rest / pieces;
-      cp_async16(s_chunk + buf * kMoveBytes + 16 * i, place(list[j0 + j], part, rest - part * pieces));
-    }
-    if (scores != nullptr)
-      for (int j = threadIdx.x; j < min(per, m - j0); j += kMoveThreads)
-        cp_async4(s_scores + buf * per + j, scores + list[j0 + j]);
-    cp_async_commit();
-  };
   const int start = p.hole[row * p.heads + head];
   if (start >= m) return;
-  load(start, 0);
+  const int32_t* list = p.kept + (int64_t)row * p.k0 + (int64_t)head * p.k1;
+  const int32_t* ids = p.table + (int64_t)row * p.table_s0;
+  const int slot = p.scores == nullptr || only == 1 ? -1 : (p.slots != nullptr ? p.slots[row] : row);
+  float* scores = slot < 0 ? nullptr : p.scores + (int64_t)slot * p.s0 + (int64_t)head * p.s1;
+  uint8_t* heads_at = p.kv + (int64_t)head * p.c_head + only * p.c_part;
+  const int pieces = p.row_bytes / 16, per_token = split ? pieces : 2 * pieces;  // 16-byte pieces
+  const int tw = min(32, kMoveLoads * 32 / per_token);                             // tokens of a warp's chunk
+  const uint32_t inverse = (65536 + per_token - 1) / per_token;                    // i / per_token for i < 128
+  const int step = C * kMoveWarps * tw;
+
+  // A lane's token of the warp's chunk at j0: its destination is position j0 + lane, its source list[j0 + lane]. Chunks
+  // run through a pipeline -- positions, then block ids and with them the bytes' places, then the bytes -- so that only the
+  // last step's latency is left at each chunk, and that one beside the chunk before.
+  struct Place {
+    int64_t source, target;
+    int from, to;
+  };
+  auto positions = [&](int j0, Place& a) {
+    const int j = j0 + lane;
+    const bool real = lane < tw && j < m;
+    a.to = real ? j : -1;
+    a.from = real ? list[j] : 0;
+  };
+  auto places = [&](Place& a) {
+    if (a.to < 0) return;
+    const int sb = a.from / p.block_size, tb = a.to / p.block_size;
+    a.source = (int64_t)ids[sb] * p.c_block + (int64_t)(a.from - sb * p.block_size) * p.c_pos;
+    a.target = (int64_t)ids[tb] * p.c_block + (int64_t)(a.to - tb * p.block_size) * p.c_pos;
+  };
+  auto piece = [&](int s, int& token) -> int64_t {  // where piece s * 32 + lane of the chunk lies in its token's rows
+    const uint32_t i = s * 32 + lane;
+    token = (int)(i * inverse >> 16);
+    const int rest = (int)i - token * per_token;
+    const int part = rest >= pieces;
+    return (int64_t)part * p.c_part + 16 * (rest - part * pieces);
+  };
+  auto load = [&](const Place& a, uint4 (&v)[kMoveLoads], float& score) {
+#pragma unroll
+    for (int s = 0; s < kMoveLoads; ++s) {
+      int token;
+      const int64_t at = piece(s, token);
+      const int64_t source = __shfl_sync(kFullMask, a.source, token & 31);
+      const int to = __shfl_sync(kFullMask, a.to, token & 31);
+      if (token < tw && to >= 0) v[s] = *reinterpret_cast<const uint4*>(heads_at + source + at);
+    }
+    if (scores != nullptr && a.to >= 0) score = scores[a.from];
+  };
+  auto store = [&](const Place& a, const uint4 (&v)[kMoveLoads], float score) {
+#pragma unroll
+    for (int s = 0; s < kMoveLoads; ++s) {
+      int token;
+      const int64_t at = piece(s, token);
+      const int64_t target = __shfl_sync(kFullMask, a.target, token & 31);
+      const int to = __shfl_sync(kFullMask, a.to, token & 31);
+      if (token < tw && to >= 0) *reinterpret_cast<uint4*>(heads_at + target + at) = v[s];
+    }
+    if (scores != nullptr && a.to >= 0) scores[a.to] = score;
+  };
+  const int j0 = start + (rank * kMoveWarps + warp) * tw;
+  Place now, next, after;
+  uint4 v[2][kMoveLoads];
+  float score[2];
+  positions(j0, now);
+  positions(j0 + step, next);
+  places(now);
+  load(now, v[0], score[0]);
+  places(next);
   int buf = 0;
-  for (int j0 = start; j0 < m; j0 += per, buf ^= 1) {
-    if (j0 + per < m) {
-      load(j0 + per, buf ^ 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncthreads();  // the whole chunk has been read
-    const int count = min(per, m - j0) * 2 * pieces;
-    for (int i = threadIdx.x; i < count; i += kMoveThreads) {
-      const int j = i / (2 * pieces), rest = i - j * 2 * pieces, part = rest / pieces;
-      *reinterpret_cast<uint4*>(place(j0 + j, part, rest - part * pieces)) =
-          *reinterpret_cast<const uint4*>(s_chunk + buf * kMoveBytes + 16 * i);
-    }
-    if (scores != nullptr)
-      for (int j = threadIdx.x; j < min(per, m - j0); j += kMoveThreads) scores[j0 + j] = s_scores[buf * per + j];
-    __syncthreads();  // before the buffer is filled again
+  // every chunk of the cluster's step is read before any of it is written; the steps after it read only positions past
+  // what this one writes
+#pragma unroll 2
+  for (int base = start; base < m; base += step) {
+    const int j = j0 + (base - start);
+    positions(j + 2 * step, after);
+    load(next, v[buf ^ 1], score[buf ^ 1]);
+    if (C > 1) cluster.sync(); else __syncthreads();
+    store(now, v[buf], score[buf]);
+    places(after);
+    now = next;
+    next = after;
+    buf ^= 1;
   }
 }
 
@@ -312,11 +465,24 @@ extern "C" int ekv_select_tokens(const float* scores, int64_t score_stride_slot,
     return fail(EKV_EINVAL, "a score stride is below the capacity");
   if (kept_stride_head < capacity || kept_stride_row < kept_stride_head)
     return fail(EKV_EINVAL, "a stride of the kept lists is below the capacity");
-  if ((int64_t)rows * heads > 0x7fffffffll || capacity > 0x7fffffff - 4096)
+  if ((int64_t)rows * heads > 0x7fffffffll / 8 || capacity > 0x7fffffff - 4096)
     return fail(EKV_ENOTSUP, "more than 2^31 - 1 rows x heads, or tokens of a row");
-  const SelectParams p{scores, score_stride_slot, score_stride_head, slots, n_slots, capacity, lens, keep, keep_all,
-                       first_tokens, recent_tokens, rows, heads, kept, kept_stride_row, kept_stride_head, new_lens, status};
-  launch_chained(select_kernel, dim3(rows * heads), dim3(kSelectThreads), 0, static_cast<cudaStream_t>(stream), p);
+  const SelectParams p{scores, score_stride_slot, score_stride_head, slots, n_slots, capacity, lens, keep, keep_all, first_tokens,
+                       recent_tokens, rows, heads, kept, kept_stride_row, kept_stride_head, new_lens, status};
+  int device = 0, sms = 0, rc;
+  if ((rc = current_device(&device)) != EKV_OK || (rc = sm_count(device, &sms)) != EKV_OK) return rc;
+  // The fewest CTAs a unit whose registers hold the row, then as many more as leave every CTA resident (two an SM) with a
+  // run of at least 4 keys a lane.
+  const int64_t units = (int64_t)rows * heads;
+  auto lane_keys = [&](int C) { return (int)(((int64_t)capacity + C * kSelectThreads - 1) / (C * kSelectThreads)); };
+  int C = 1;
+  while (C < 8 && lane_keys(C) > 32) C *= 2;
+  while (C < 8 && lane_keys(C) > 4 && units * C * 2 <= 2 * sms) C *= 2;
+  const int keys = lane_keys(C);
+  auto kernel = keys <= 4 ? select_kernel<4> : keys <= 8 ? select_kernel<8> : keys <= 16 ? select_kernel<16>
+                : keys <= 32 ? select_kernel<32> : select_kernel<0>;
+  launch_chained_cluster(kernel, dim3((unsigned)(units * C)), dim3(kSelectThreads), 0, static_cast<cudaStream_t>(stream),
+                         (unsigned)C, p);
   return check_launch("select_kernel");
 }
 
@@ -336,14 +502,14 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
   if (!kv || !table || !lens || !kept || !new_lens) return fail(EKV_EINVAL, "a required device pointer is NULL");
   if (rows <= 0 || width <= 0 || heads <= 0 || block_size <= 0 || pool_blocks <= 0 || columns <= 0)
     return fail(EKV_EINVAL, "rows, width, heads, block_size, columns and pool_blocks must be positive");
-  if (head_bytes <= 0 || (head_bytes & 15) || head_bytes > 4096)
-    return fail(EKV_ENOTSUP, "a head of %d bytes: this build moves 16 to 4096 in whole 16-byte units", head_bytes);
+  if (head_bytes <= 0 || (head_bytes & 15) || head_bytes > 1024)
+    return fail(EKV_ENOTSUP, "a head of %d bytes: this build moves 16 to 1024 in whole 16-byte units", head_bytes);
   if (((uintptr_t)kv & 15) || (kv_stride_block & 15) || (kv_stride_part & 15) || (kv_stride_pos & 15) || (kv_stride_head & 15))
     return fail(EKV_EINVAL, "the cache must be 16-byte aligned with strides of whole 16-byte units");
   if (table_stride < width) return fail(EKV_EINVAL, "the table's row stride is below the width");
   if (kept_stride_head < columns || kept_stride_row < 0) return fail(EKV_EINVAL, "a stride of the kept lists is below their length");
   if (first_tokens < 0) return fail(EKV_EINVAL, "first_tokens must not be negative");
-  if (pool_blocks > 0x7fffffffll || (int64_t)width * block_size > 0x7fffffffll - 65536 || (int64_t)rows * heads > 0x7fffffffll)
+  if (pool_blocks > 0x7fffffffll || (int64_t)width * block_size > 0x7fffffffll - 65536 || (int64_t)rows * heads > 0x7fffffffll / 16)
     return fail(EKV_ENOTSUP, "more than 2^31 - 1 blocks, tokens of a row, or rows x heads");
   if (scores) {
     if (n_slots <= 0 || (!slots && n_slots < rows)) return fail(EKV_EINVAL, "%d score slots for %d rows", n_slots, rows);
@@ -365,9 +531,13 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
   launch_chained(check_kernel, dim3(rows * heads), dim3(kCheckThreads), 0, s, p);
   int rc = check_launch("check_kernel");
   if (rc != EKV_OK) return rc;
-  const size_t smem = 2 * kMoveBytes + 2 * (kMoveBytes / (2 * (size_t)head_bytes)) * 4;
-  if (cudaFuncSetAttribute(move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return check_launch("cudaFuncSetAttribute(move_kernel)");
-  launch_chained(move_kernel, dim3(rows * heads), dim3(kMoveThreads), smem, s, p);
+  int device = 0, sms = 0;
+  if ((rc = current_device(&device)) != EKV_OK || (rc = sm_count(device, &sms)) != EKV_OK) return rc;
+  // Up to two CTAs an SM from clusters of the portable size, then with keys and values apart.
+  const int64_t units = (int64_t)rows * heads;
+  int C = 1;
+  while (C < 8 && units * C * 2 <= 2 * sms) C *= 2;
+  const int split = units * C * 2 <= 2 * sms;
+  launch_chained_cluster(move_kernel, dim3((unsigned)(units * C * (split ? 2 : 1))), dim3(kMoveThreads), 0, s, (unsigned)C, p, split);
   return check_launch("move_kernel");
 }

@@ -124,6 +124,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _i32, _i32, _i32, _f32, _i32, _p, _p, _i32,  # kv_heads D dtype scale groups group_start prefix common
          _p, _i64, _i64, _p, _p, _sz, _p, _p],  # out lse workspace bytes status stream
     ),
+    "ekv_attend_scored_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "ekv_attend_scored": (
         _i32,
         [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64,  # q and strides, kv and strides, pool_blocks

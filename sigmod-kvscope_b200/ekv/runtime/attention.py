@@ -201,7 +201,7 @@ def attend_scored(
     if tokens == 0 or rows == 0:
         return out, lse
     lib = _lib.load()
-    size = lib.ekv_attend_workspace_bytes(rows, tokens, 0, q_heads, kv_heads, dim)
+    size = lib.ekv_attend_scored_workspace_bytes(rows, tokens, width, block_size, q_heads, kv_heads, dim)
     with _lib.on_device(device) as stream:
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         rc = lib.ekv_attend_scored(

@@ -120,7 +120,7 @@ def test_select_tokens_refuses(lib, over, code):
     (dict(rows=0), L.EINVAL),
     (dict(columns=0), L.EINVAL),
     (dict(head_bytes=200), L.ENOTSUP),
-    (dict(head_bytes=8192), L.ENOTSUP),
+    (dict(head_bytes=1040), L.ENOTSUP),
     (dict(s2=520), L.EINVAL),
     (dict(kv=ctypes.c_void_p(0x1004)), L.EINVAL),
     (dict(ts=7), L.EINVAL),

@@ -184,6 +184,34 @@ def test_scores_gather_the_weights(cuda_lib, dtype, dim, block, queries):
     check(got, x, 0.1, dtype)
 
 
+@pytest.mark.parametrize("dtype, dim, block", [(torch.float16, 128, 16), (torch.bfloat16, 64, 64), (torch.float16, 64, 8)])
+def test_scores_from_windows_of_many_query_rows(cuda_lib, dtype, dim, block):
+    """From 8 to 512 query rows a KV head (two rounds of 256), rows that end inside a tile, a row of one tile, a missing block."""
+    lens = [1000, 130, 64, 640, 257]
+    x = make(31, lens, queries=[64, 33, 32, 1, 40], dim=dim, block=block, dtype=dtype, q_heads=16)
+    capacity = x["table"].shape[1] * block
+    scores = torch.rand(5, 2, capacity, generator=torch.Generator().manual_seed(2))
+    got = run_scored(x, on_device(x), 0.1, scores, fresh=[1000, 100, 70, 1, 0], decay=0.5)
+    check(got, x, 0.1, dtype)
+
+
+@pytest.mark.parametrize("queries", [1, 20])
+def test_scores_of_blocks_that_are_not_there(cuda_lib, queries):
+    from ekv.runtime.attention import attend_scored
+
+    x = make(32, [100, 300], queries=[queries] * 2)
+    ok = np.ones(tuple(x["table"].shape), dtype=bool)
+    x["table"][1, 4], ok[1, 4] = -3, False
+    d = on_device(x)
+    scores = torch.ones(2, 2, x["table"].shape[1] * 16, device="cuda")
+    attend_scored(d["query"], d["cache"], d["table"], d["lens"], 0.1, scores, query_start=d["start"], fresh=d["lens"])
+    _, _, w = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(), 0.1,
+                         x["start"].numpy(), ok)
+    for r, n in enumerate([100, 300]):
+        np.testing.assert_allclose(scores[r, :, :n].cpu().numpy(), w[r], rtol=1e-6, atol=4e-5 * w[r].max())
+    assert torch.all(scores[1, :, 64:80] == 0) and torch.all(scores[0, :, 100:] == 1)
+
+
 def test_a_prompt_with_no_scores_yet_and_scores_that_are_not_numbers(cuda_lib):
     x = make(7, [200, 50, 100], queries=[16, 5, 1])
     scores = torch.full((3, 2, x["table"].shape[1] * 16), float("nan"))
