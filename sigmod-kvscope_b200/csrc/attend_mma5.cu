@@ -10,10 +10,9 @@
 //     there is copied from past the pool, which the TMA engine reads as zeros).
 //   mma warp: S = Q K^T into tensor memory, then O += P V with P from tensor memory; one thread issues. S of the next
 //     tile follows O of this one, so a score's arrival also says that the output below it is at rest.
-//   softmax warpgroups: a row's 128 scores 32 at a time, once for their maximum and once for their exponentials (all 128
-//     in registers spilled); the running maximum is only raised when it grew by more than 2^8, so the output in tensor
-//     memory is rescaled a few times a row, by the same threads; probabilities go back to tensor memory over the scores
-//     already read, rounded to the values' type.
+//   softmax warpgroups: a row's 128 scores 32 at a time. The running maximum is only raised when it grew by more than 2^8,
+//     so most tiles need one pass over their scores, and the output in tensor memory is rescaled a few times a row, by the
+//     same threads; probabilities go back to tensor memory over the scores, rounded to the values' type.
 #include <type_traits>
 
 #include "attend.cuh"
@@ -70,6 +69,147 @@ struct Share {
 __device__ __forceinline__ Share share_of(const AttendParams& p, const Item& it) {
   const int rows = it.un.q.nq * p.G - it.mt * kWideRows;
   return {rows <= kSub, it.last - it.first};
+}
+
+// ---- one tile of one query row ----------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+
+struct SoftmaxTile {
+  uint32_t s_at, o_at;   // this thread's scores and output in tensor memory
+  int pos, limit;        // of the tile's first token, and of the first one the row does not see
+  uint32_t missing;      // blocks of the tile that are not there
+  int block_shift;
+  float scale_log2, grow;
+  bool later;            // the output holds earlier tiles
+};
+
+// Raises m to `top` in the lanes that ask for it and rescales l and the output to it; returns the new l. With the whole warp.
+template <int D>
+__device__ __forceinline__ float rescale(const SoftmaxTile& a, bool raise, float top, float& m, float l) {
+  const float f = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * a.scale_log2)) : 1.f;
+  if (raise) m = top;
+  if (a.later) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      float o[32];
+      tmem_ld32(o, a.o_at + c);
+      tmem_wait_ld(o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] *= f;
+      tmem_st32(a.o_at + c, reinterpret_cast<const uint32_t*>(o));
+    }
+  }
+  return l * f;  // the stores are waited for with the probabilities'
+}
+
+// A thread's row of 128 scores that the row sees: raises its running maximum m where it grew by more than `grow` (and then
+// rescales its sum l and the output), writes the probabilities over the scores and adds them to l. Two scores to an
+// instruction where the hardware has one. (One pass over the scores, against the maximum as it stood, with a second one
+// only where it had grown, measured slower: its 64 packed probabilities and 64 scores crowd the registers.)
+template <typename T, int D>
+__device__ __forceinline__ void seen_softmax(const SoftmaxTile& a, float& m, float& l) {
+  float s[2][32];
+  auto fetch = [&](int c) { tmem_ld32(s[c & 1], a.s_at + 32 * c); };
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  fetch(0);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {  // chunk c + 1 is on its way while chunk c is worked on
+    tmem_wait_ld(s[c & 1]);
+    if (c < 3) fetch(c + 1);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx[i & 3] = max3(mx[i & 3], s[c & 1][2 * i], s[c & 1][2 * i + 1]);
+  }
+  const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  const bool raise = top > m + a.grow;  // also a row's first scores: m is -inf
+  if (__any_sync(kFullMask, raise)) l = rescale<D>(a, raise, top, m, l);
+  const float from = m == -INFINITY ? 0.f : m * a.scale_log2;
+  const uint64_t scale2 = pair_of(a.scale_log2, a.scale_log2), from2 = pair_of(-from, -from);
+  uint64_t sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+  fetch(0);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_wait_ld(s[c & 1]);
+    if (c < 3) fetch(c + 1);
+    uint32_t u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x, y;
+      split(fma_pair(pair_of(s[c & 1][2 * i], s[c & 1][2 * i + 1]), scale2, from2), x, y);
+      x = exp2_fast(x);
+      y = exp2_fast(y);
+      sum[i & 1] = add_pair(sum[i & 1], pair_of(x, y));
+      u[i] = pack2<T>(x, y);
+    }
+    tmem_st16(a.s_at + 16 * c, u);
+  }
+  float x, y;
+  split(add_pair(sum[0], sum[1]), x, y);
+  l += x + y;
+}
+
+// The same where the row does not see the whole tile. Not inlined: its registers would be the common case's too. Returns
+// (m, l).
+template <typename T, int D>
+__device__ __noinline__ float2 full_softmax(const SoftmaxTile& a, float m, float l) {
+  const bool masked = a.missing != 0 || a.pos + kTokens > a.limit;
+  float s[32];
+  auto fetch = [&](int c) {
+    tmem_ld32(s, a.s_at + 32 * c);
+    tmem_wait_ld(s);
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (a.pos + 32 * c + i >= a.limit || (a.missing >> ((32 * c + i) >> a.block_shift) & 1u)) s[i] = -INFINITY;
+    }
+    __syncwarp();
+  };
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    fetch(c);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+  }
+  const bool raise = top > m + a.grow;  // also a row's first scores: m is -inf
+  if (__any_sync(kFullMask, raise)) l = rescale<D>(a, raise, top, m, l);
+  const float from = m == -INFINITY ? 0.f : m * a.scale_log2;
+  float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    fetch(c);
+    uint32_t u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = exp2_fast(fmaf(s[2 * i], a.scale_log2, -from)), y = exp2_fast(fmaf(s[2 * i + 1], a.scale_log2, -from));
+      sum[0] += x;
+      sum[1] += y;
+      u[i] = pack2<T>(x, y);
+    }
+    tmem_st16(a.s_at + 16 * c, u);  // over scores already read
+  }
+  tmem_wait_st();
+  return make_float2(m, l + (sum[0] + sum[1]));
 }
 
 template <typename T, int D, bool PREFIX>
@@ -291,13 +431,15 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       const int token = uq.q0 + mrow / p.G, qhead = it.head * p.G + mrow % p.G;
       float m = -INFINITY, l = 0.f;
       if (sh.of(w) > 0) {
-        // this thread's query row, into the subtile's swizzled rows
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 + (int64_t)qhead * p.q_s1);
-        const uint32_t dst = smem_u32(queries) + w * R::kSlot + row * 128;
+        // the warp's 32 query rows into the subtile's swizzled rows, D / 8 lanes a row
+        const int64_t mine = real ? (int64_t)token * p.q_s0 + (int64_t)qhead * p.q_s1 : -1;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 v = real ? src[c] : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * R::kHalf + (((c & 7) ^ (row & 7)) << 4)),
+        for (int i = 0; i < D / 8; ++i) {
+          const int r = i * (256 / D) + lane / (D / 8), c = lane % (D / 8), at = (warp & 3) * 32 + r;
+          const int64_t source = __shfl_sync(kFullMask, mine, r);
+          const uint4 v = source >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + source + 8 * c) : make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(queries) + w * R::kSlot + (c >> 3) * R::kHalf +
+                                                                       at * 128 + (((c & 7) ^ (at & 7)) << 4)),
                        "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                        : "memory");
         }
@@ -323,64 +465,14 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
           __syncwarp();
           const int pos = it.un.from + tile * kTokens;
           const bool masked = missing != 0 || __any_sync(kFullMask, pos + kTokens > limit);
-          float s[2][32];
-          // chunk c of the scores is waited for while chunk c + 1 is on its way
-          auto fetch = [&](int c) { tmem_ld32(s[c & 1], s_at + 32 * c); };
-          auto mask = [&](int c) {
-            if (!masked) return;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (pos + 32 * c + i >= limit || (missing >> ((32 * c + i) >> p.block_shift) & 1u)) s[c & 1][i] = -INFINITY;
-          };
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          fetch(0);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld(s[c & 1]);
-            if (c < 3) fetch(c + 1);
-            mask(c);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[c & 1][i]);
+          const SoftmaxTile st{s_at, o_at, pos, limit, missing, p.block_shift, p.scale_log2, grow, tile >= it.first + step};
+          if (!masked) {
+            seen_softmax<T, D>(st, m, l);
+          } else {
+            const float2 ml = full_softmax<T, D>(st, m, l);
+            m = ml.x;
+            l = ml.y;
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const bool raise = top > m + grow;  // also a row's first scores: m is -inf
-          if (__any_sync(kFullMask, raise)) {
-            const float f = raise ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * p.scale_log2)) : 1.f;
-            if (raise) m = top;
-            l *= f;
-            if (tile >= it.first + step) {  // the output holds earlier tiles
-#pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tmem_ld32(o, o_at + c);
-                tmem_wait_ld(o);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= f;
-                tmem_st32(o_at + c, reinterpret_cast<const uint32_t*>(o));
-              }
-              // waited for with the probabilities below
-            }
-          }
-          const float from = m == -INFINITY ? 0.f : m * p.scale_log2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          fetch(0);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld(s[c & 1]);
-            if (c < 3) fetch(c + 1);
-            mask(c);
-            uint32_t u[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float a = exp2_fast(fmaf(s[c & 1][2 * i], p.scale_log2, -from));
-              const float b = exp2_fast(fmaf(s[c & 1][2 * i + 1], p.scale_log2, -from));
-              sum[(2 * i) & 3] += a;
-              sum[(2 * i + 1) & 3] += b;
-              u[i] = pack2<T>(a, b);
-            }
-            tmem_st16(s_at + 16 * c, u);
-          }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&tail.p_ready[w]);
@@ -403,16 +495,26 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       }
       if (real) *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * p.scale_log2, l);
       if (sh.of(w) > 0) {
+        // The output by way of the queries' shared memory, whose products are complete, so that a store covers whole lines
+        // and not 16 bytes of each of 32 rows: 32 dims of the warp's rows at a time, a row's 16-byte pieces turned by its number.
+        float* stage = reinterpret_cast<float*>(queries + w * R::kSlot + (warp & 3) * 4096);
+        const int64_t to = real ? (int64_t)(dst - p.parts) : INT64_MIN;
         __syncwarp();
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
           tmem_ld32(o, o_at + c);
           tmem_wait_ld(o);
-          if (real) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(dst + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(stage + lane * 32 + 4 * (i ^ (lane & 7))) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3), k = lane & 7;
+            const int64_t target = __shfl_sync(kFullMask, to, r);
+            if (target != INT64_MIN)
+              *reinterpret_cast<float4*>(p.parts + target + c + 4 * k) = *reinterpret_cast<const float4*>(stage + r * 32 + 4 * (k ^ (r & 7)));
           }
           __syncwarp();
         }
