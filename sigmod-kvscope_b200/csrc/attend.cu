@@ -62,12 +62,22 @@ __device__ __forceinline__ uint32_t chunk_at(int t, int c) {
 // The shared memory behind the ring.
 template <int D, int WM, int WN>
 struct Tail {
+  static constexpr int kRows = WN > 1 ? 4 / WM : 1;  // query rows of each of the WM that join at a time
   uint64_t full[Ring<D>::kStages], empty[Ring<D>::kStages];
+  uint64_t item_full, item_empty;
   uint32_t blocks[Ring<D>::kStages];  // which of the stage's blocks were copied (bit b: the tile's block b)
   int scratch[kThreads / 32 + 1];
-  float m[WN > 1 ? WN : 1][16 * WM], l[WN > 1 ? WN : 1][16 * WM];
-  alignas(16) float o[WN > 1 ? WN / 2 : 1][16 * WM][WN > 1 ? D / 2 + 4 : 1];  // half the dims at a time
+  Item item;  // what the math warps take next
+  float m[2][WN > 1 ? WN : 1][16 * WM], l[2][WN > 1 ? WN : 1][16 * WM];  // of one item and of the next
+  alignas(16) float o[WN > 1 ? WM * WN * kRows : 1][WN > 1 ? D + 8 : 4];
+  alignas(16) uint8_t queries[WN > 1 ? 16 * WM * D * 2 : 16];  // the item's query rows, in 16-byte pieces turned by the row
 };
+
+// Where piece c of query row r lies in the shared queries.
+template <int D>
+__device__ __forceinline__ uint32_t query_at(int r, int c) {
+  return (uint32_t)r * (2 * D) + (uint32_t)((c & ~7) | ((c & 7) ^ (r & 7))) * 16;
+}
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ AttendParams p) {
@@ -87,6 +97,8 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       mbar_init(&tail.full[s], 1);
       mbar_init(&tail.empty[s], kMathWarps);
     }
+    mbar_init(&tail.item_full, 64);  // every lane of the copy warp, and its copies of queries
+    mbar_init(&tail.item_empty, kMathWarps);
     fence_mbar_init();
   }
   // The lengths, tables and caches may be the work of the launches before. A launch that follows a prefix launch
@@ -110,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool good = true;
-    for (int t = begin; t < end && good;) {
+    for (int t = begin, n_items = 0; t < end && good; ++n_items) {
       const Item it = item_at<PREFIX>(p, plan, MT, t, end);
       const int from = it.un.from, to = it.un.to;
       const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
@@ -144,8 +156,32 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         id = next;
         ++issued;
         if (++stage == R::kStages) stage = 0, phase ^= 1;
+        if (tile == it.first) {
+          // The item for the math warps, behind its first tile's copies and when they have taken the one before: they find
+          // it, and its queries, without a chain of loads of their own.
+          if (n_items > 0) good = mbar_wait_bounded(&tail.item_empty, (n_items - 1) & 1, p.status);
+          good = __all_sync(kFullMask, good);
+          if (!good) break;
+          if (lane == 0) tail.item = it;
+          if constexpr (WN > 1) {
+#pragma unroll 4
+            for (int i = lane; i < MT * D / 8; i += 32) {
+              const int r = i / (D / 8), c = i % (D / 8), mrow = it.mt * MT + r;
+              uint8_t* dst = tail.queries + query_at<D>(r, c);
+              if (mrow < it.un.q.nq * p.G)
+                cp_async16(dst, static_cast<const T*>(p.q) + (int64_t)(it.un.q.q0 + mrow / p.G) * p.q_s0 +
+                                    (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 8 * c);
+              else
+                *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&tail.item_full)) : "memory");
+          mbar_arrive(&tail.item_full);
+        }
       }
     }
+    // copies of queries that the math warps did not wait for have to land too
+    asm volatile("cp.async.wait_all;" ::: "memory");
     // no CTA leaves with copies in flight: the last phase of every stage that was used has to be complete
     for (int s = 0; s < R::kStages; ++s) {
       const int uses = issued > s ? (issued - s - 1) / R::kStages + 1 : 0;
@@ -161,8 +197,12 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   int stage = 0;
   uint32_t phase = 0;
   bool good = true;
-  for (int t = begin; t < end;) {
-    const Item it = item_at<PREFIX>(p, plan, MT, t, end);
+  for (int t = begin, n_items = 0; t < end; ++n_items) {
+    // after a wait that gave up the walk goes on without waiting, so that the warps' barriers stay paired
+    if (good) good = mbar_wait_bounded(&tail.item_full, n_items & 1, p.status);
+    good = __all_sync(kFullMask, good);
+    Item it;
+    if (good) it = tail.item; else it = item_at<PREFIX>(p, plan, MT, t, end);
     const QueryRange uq = it.un.q;
     const int from = it.un.from, to = it.un.to;
     // this lane's two query rows: the tokens they see, and their fragments
@@ -175,14 +215,23 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       const bool real = mrow < uq.nq * p.G;
       limit[j] = 0x7fffffff;
       if (real) limit[j] = token_limit<PREFIX>(p, it.un, token);
-      const T* src = static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 +
-                     (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 2 * pair;
+      if constexpr (WN == 1) {
+        const T* src = static_cast<const T*>(p.q) + (int64_t)token * p.q_s0 +
+                       (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 2 * pair;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][j] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-        qf[k][j + 2] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][j] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+          qf[k][j + 2] = real ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+        }
       }
     }
+    if constexpr (WN > 1) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        ldmatrix_x4(qf[k], smem_u32(tail.queries) + query_at<D>(wm * 16 + (lane & 15), 2 * k + (lane >> 4)));
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tail.item_empty);
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < D / 8; ++d)
@@ -190,7 +239,6 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       for (int j = 0; j < 4; ++j) o[d][j] = 0.f;
 
     for (int tile = it.first; tile < it.last; ++tile, ++t) {
-      // after a wait that gave up the walk goes on without waiting, so that the warps' barriers stay paired
       if (good) good = mbar_wait_bounded(&tail.full[stage], phase, p.status);
       const uint32_t keys = smem_u32(ring) + stage * R::kStage, values = keys + R::kPart;
       const uint32_t blocks = tail.blocks[stage];
@@ -318,93 +366,106 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       l[j] += __shfl_xor_sync(kFullMask, l[j], 1);
       l[j] += __shfl_xor_sync(kFullMask, l[j], 2);
     }
-    if (WN > 1) {
+    const bool complete = it.first == 0 && it.last == it.tiles;
+    const bool final = complete && p.groups == 0;  // nothing else joins: the output itself
+    // where row mrow's part goes: its dims, and its maximum and sum
+    auto part_at = [&](int mrow, int token, int head, float*& dst, float*& ml) {
+      if (complete) {
+        const int64_t at = (int64_t)token * p.q_heads + head;
+        dst = p.whole + at * D;
+        ml = p.whole + (int64_t)p.tokens * p.q_heads * D + 2 * at;
+      } else {
+        const int64_t at = (int64_t)(2 * blockIdx.x + (it.first == 0 ? 1 : 0)) * MT + (mrow - it.mt * MT);
+        dst = p.parts + at * D;
+        ml = p.parts + (int64_t)2 * p.max_ctas * MT * D + 2 * at;
+      }
+    };
+    if constexpr (WN > 1) {
+      // The WN warps of a row join through shared memory, a few rows at a time, in the warps' order: each scales its part to
+      // the common maximum, and then every thread adds four dims of a row and writes them, a row's lanes side by side.
+      constexpr int kRows = TailT::kRows, kPer = 8 / kRows;
+      float(&ms)[WN][16 * WM] = tail.m[n_items & 1], (&ls)[WN][16 * WM] = tail.l[n_items & 1];
       if (pair == 0) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          tail.m[wn][wm * 16 + quad + 8 * j] = m[j];
-          tail.l[wn][wm * 16 + quad + 8 * j] = l[j];
+          ms[wn][wm * 16 + quad + 8 * j] = m[j];
+          ls[wn][wm * 16 + quad + 8 * j] = l[j];
         }
       }
       named_barrier(1, kMathWarps * 32);
       float f[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int row = wm * 16 + quad + 8 * j;
         float top = -INFINITY;
-        for (int w = 0; w < WN; ++w) top = fmaxf(top, tail.m[w][row]);
+        for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][wm * 16 + quad + 8 * j]);
         f[j] = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - top);
-        float sum = 0.f;
-        for (int w = 0; w < WN; ++w) sum += tail.m[w][row] == -INFINITY ? 0.f : tail.l[w][row] * exp2_fast(tail.m[w][row] - top);
-        m[j] = top;
-        l[j] = sum;
       }
+      const int rows = min(16, uq.nq * p.G - it.mt * MT);  // of the first of the WM: the others have no more
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        o[d][0] *= f[0];
-        o[d][1] *= f[0];
-        o[d][2] *= f[1];
-        o[d][3] *= f[1];
-      }
+      for (int round = 0; round < 16 / kRows; ++round) {
+        if (round * kRows >= rows) break;
+        if (round > 0) named_barrier(1, kMathWarps * 32);
+        constexpr int kQuads = kRows;
+        const int j = round / kPer;  // constant in the unrolled loop
+        if (quad / kQuads == round % kPer) {
+          float* dst = tail.o[(wm * WN + wn) * kRows + quad % kQuads] + 2 * pair;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {
+          for (int d = 0; d < D / 8; ++d)
+            *reinterpret_cast<float2*>(dst + 8 * d) =
+                f[j] == 0.f ? make_float2(0.f, 0.f) : make_float2(o[d][2 * j] * f[j], o[d][2 * j + 1] * f[j]);
+        }
+        named_barrier(1, kMathWarps * 32);
+        const int i = wn * 32 + lane, r = i / (D / 4), c = i % (D / 4);  // this thread's row of the round and its four dims
+        const int tile_row = wm * 16 + round * kRows + r, mrow = it.mt * MT + tile_row;
+        if (r < kRows && mrow < uq.nq * p.G) {
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          float top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int half = WN / 2; half >= 1; half /= 2) {  // a tree, so the order of the additions is fixed
-          if (wn >= half && wn < 2 * half) {
+          for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][tile_row]);
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              const float(&v)[4] = o[part * (D / 16) + d];
-              float* dst = &tail.o[wn - half][wm * 16 + quad][8 * d + 2 * pair];
-              *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
-              *reinterpret_cast<float2*>(dst + 8 * (D / 2 + 4)) = make_float2(v[2], v[3]);
-            }
+          for (int w = 0; w < WN; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(tail.o[(wm * WN + w) * kRows + r] + 4 * c);
+            const float mw = ms[w][tile_row];
+            total += mw == -INFINITY ? 0.f : ls[w][tile_row] * exp2_fast(mw - top);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
           }
-          named_barrier(1, kMathWarps * 32);
-          if (wn < half) {
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              float(&v)[4] = o[part * (D / 16) + d];
-              const float* src = &tail.o[wn][wm * 16 + quad][8 * d + 2 * pair];
-              const float2 a = *reinterpret_cast<const float2*>(src);
-              const float2 b = *reinterpret_cast<const float2*>(src + 8 * (D / 2 + 4));
-              v[0] += a.x;
-              v[1] += a.y;
-              v[2] += b.x;
-              v[3] += b.y;
-            }
+          const int token = uq.q0 + mrow / p.G, head = it.head * p.G + mrow % p.G;
+          if (final) {
+            const float inv = 1.f / total;
+            uint2 v;
+            v.x = total == 0.f ? 0u : pack2<T>(sum.x * inv, sum.y * inv);
+            v.y = total == 0.f ? 0u : pack2<T>(sum.z * inv, sum.w * inv);
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)head * p.out_s1 + 4 * c) = v;
+            if (p.lse != nullptr && c == 0)
+              p.lse[(int64_t)token * p.q_heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+          } else {
+            float *dst, *ml;
+            part_at(mrow, token, head, dst, ml);
+            *reinterpret_cast<float4*>(dst + 4 * c) = sum;
+            if (c == 0) *reinterpret_cast<float2*>(ml) = make_float2(top, total);
           }
-          named_barrier(1, kMathWarps * 32);
         }
       }
-    }
-    if (wn == 0) {
-      const bool complete = it.first == 0 && it.last == it.tiles;
+    } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int mrow = it.mt * MT + wm * 16 + quad + 8 * j;
         if (mrow >= uq.nq * p.G) continue;
         const int token = uq.q0 + mrow / p.G, head = it.head * p.G + mrow % p.G;
-        if (complete && p.groups == 0) {
-          const float inv = l[j] > 0.f ? 1.f / l[j] : (l[j] == 0.f ? 0.f : l[j]);
+        if (final) {
+          const float inv = 1.f / l[j];
           T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)head * p.out_s1 + 2 * pair;
 #pragma unroll
-          for (int d = 0; d < D / 8; ++d) {
-            const float x = l[j] == 0.f ? 0.f : o[d][2 * j] * inv, y = l[j] == 0.f ? 0.f : o[d][2 * j + 1] * inv;
-            *reinterpret_cast<uint32_t*>(dst + 8 * d) = pack2<T>(x, y);
-          }
+          for (int d = 0; d < D / 8; ++d)
+            *reinterpret_cast<uint32_t*>(dst + 8 * d) = l[j] == 0.f ? 0u : pack2<T>(o[d][2 * j] * inv, o[d][2 * j + 1] * inv);
           if (p.lse != nullptr && pair == 0)
             p.lse[(int64_t)token * p.q_heads + head] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * kLn2;
         } else {
           float *dst, *ml;
-          if (complete) {
-            const int64_t at = (int64_t)token * p.q_heads + head;
-            dst = p.whole + at * D;
-            ml = p.whole + (int64_t)p.tokens * p.q_heads * D + 2 * at;
-          } else {
-            const int64_t at = (int64_t)(2 * blockIdx.x + (it.first == 0 ? 1 : 0)) * MT + (mrow - it.mt * MT);
-            dst = p.parts + at * D;
-            ml = p.parts + (int64_t)2 * p.max_ctas * MT * D + 2 * at;
-          }
+          part_at(mrow, token, head, dst, ml);
 #pragma unroll
           for (int d = 0; d < D / 8; ++d)
             *reinterpret_cast<float2*>(dst + 8 * d + 2 * pair) = make_float2(o[d][2 * j], o[d][2 * j + 1]);
@@ -508,21 +569,40 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
     for (int k = 0; k < 2; ++k) {
-#pragma unroll 4
-      for (int i = 0; i < lists[k].count; ++i) {
-        const int64_t at = part_row(lists[k], i);
-        const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
-        const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-        float o[D / 32];
-        if constexpr (D == 128)
-          *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(lists[k].o + at * D + lane * 4);
-        else
-          *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(lists[k].o + at * D + lane * 2);
-        l += ml.x == -INFINITY ? 0.f : ml.y * f;
+      for (int base = 0; base < lists[k].count; base += 32) {
+        // a lane a part: its factor (0: nothing of it is read), then the outputs, eight loads in flight
+        float f = 0.f;
+        int64_t at = 0;
+        if (base + lane < lists[k].count) {
+          at = part_row(lists[k], base + lane);
+          const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
+          f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
+          if (f != 0.f) l += ml.y * f;
+        }
+        const int count = min(32, lists[k].count - base);
+        for (int i0 = 0; i0 < count; i0 += 8) {
+          float o[8][D / 32], fs[8];
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d) acc[d] = ml.x == -INFINITY ? acc[d] : fmaf(o[d], f, acc[d]);
+          for (int i = 0; i < 8; ++i) {
+            fs[i] = __shfl_sync(kFullMask, f, i0 + i);
+            const int64_t row_at = __shfl_sync(kFullMask, at, i0 + i);
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) o[i][d] = 0.f;
+            if (fs[i] != 0.f) {  // lanes behind the last part have a factor of 0
+              if constexpr (D == 128)
+                *reinterpret_cast<float4*>(o[i]) = *reinterpret_cast<const float4*>(lists[k].o + row_at * D + lane * 4);
+              else
+                *reinterpret_cast<float2*>(o[i]) = *reinterpret_cast<const float2*>(lists[k].o + row_at * D + lane * 2);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) acc[d] = fmaf(o[i][d], fs[i], acc[d]);
+        }
       }
     }
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
     const float inv = 1.f / l;
     T* dst = static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)qhead * p.out_s1 + lane * (D / 32);
 #pragma unroll
