@@ -66,7 +66,7 @@ struct Tail {
   uint64_t full[Ring<D>::kStages], empty[Ring<D>::kStages];
   uint64_t item_full, item_empty;
   uint32_t blocks[Ring<D>::kStages];  // which of the stage's blocks were copied (bit b: the tile's block b)
-  int scratch[kThreads / 32 + 1];
+  int scratch[kThreads / 32 + 1], found[2];
   Item item;  // what the math warps take next
   float m[2][WN > 1 ? WN : 1][16 * WM], l[2][WN > 1 ? WN : 1][16 * WM];  // of one item and of the next
   alignas(16) float o[WN > 1 ? WM * WN * kRows : 1][WN > 1 ? D + 8 : 4];
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   TailT& tail = *reinterpret_cast<TailT*>(ring + R::kBytes);
-  const Plan plan{reinterpret_cast<int*>(ring + R::kBytes + (sizeof(TailT) + 15) / 16 * 16), PREFIX ? p.groups : p.rows};
+  const int units = PREFIX ? p.groups : p.rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -105,15 +105,13 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   // starts after that one has waited for them, reads nothing that it writes, and so runs beside its last CTAs; it
   // waits at its end, so that what follows finds both complete.
   if (!p.follows) chain_wait();
-  make_plan<PREFIX, kThreads>(p, plan, MT, tail.scratch);
-  const int W = plan.cum[plan.units];
-  const int n = sharing_ctas(W, gridDim.x);
+  const Deal dealt = deal<PREFIX, kThreads>(p, units, MT, tail.scratch, tail.found);
+  const int begin = dealt.begin, end = dealt.end;
   chain_release();
-  if ((int)blockIdx.x >= n || W == 0) {
+  if (begin >= end) {
     if (p.follows) chain_wait();
     return;
   }
-  const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
   const int per_tile = kTile >> p.block_shift;  // blocks of a tile
 
   if (warp == kMathWarps) {  // ---- the copy warp ------------------------------------------------------
@@ -122,8 +120,9 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool good = true;
+    Walk<PREFIX> walk(p, dealt, units, MT);
     for (int t = begin, n_items = 0; t < end && good; ++n_items) {
-      const Item it = item_at<PREFIX>(p, plan, MT, t, end);
+      const Item it = walk.at(p, t, end);
       const int from = it.un.from, to = it.un.to;
       const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
       const int last_block = (to - 1) >> p.block_shift;
@@ -164,15 +163,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
           if (!good) break;
           if (lane == 0) tail.item = it;
           if constexpr (WN > 1) {
+            constexpr int kStep = 256 / D;  // rows that the warp's 32 pieces cover
+            const int piece = lane % (D / 8);
+            int r = lane / (D / 8), i = (it.mt * MT + r) / p.G, g = it.mt * MT + r - i * p.G;
 #pragma unroll 4
-            for (int i = lane; i < MT * D / 8; i += 32) {
-              const int r = i / (D / 8), c = i % (D / 8), mrow = it.mt * MT + r;
-              uint8_t* dst = tail.queries + query_at<D>(r, c);
-              if (mrow < it.un.q.nq * p.G)
-                cp_async16(dst, static_cast<const T*>(p.q) + (int64_t)(it.un.q.q0 + mrow / p.G) * p.q_s0 +
-                                    (int64_t)(it.head * p.G + mrow % p.G) * p.q_s1 + 8 * c);
+            for (; r < MT; r += kStep) {
+              uint8_t* dst = tail.queries + query_at<D>(r, piece);
+              if (i < it.un.q.nq)
+                cp_async16(dst, static_cast<const T*>(p.q) + (int64_t)(it.un.q.q0 + i) * p.q_s0 +
+                                    (int64_t)(it.head * p.G + g) * p.q_s1 + 8 * piece);
               else
                 *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+              for (g += kStep; g >= p.G; g -= p.G) ++i;
             }
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&tail.item_full)) : "memory");
@@ -198,11 +200,11 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   uint32_t phase = 0;
   bool good = true;
   for (int t = begin, n_items = 0; t < end; ++n_items) {
-    // after a wait that gave up the walk goes on without waiting, so that the warps' barriers stay paired
+    // after a wait that gave up the warps go on to the item's end without waiting, where their barriers are, and leave together
     if (good) good = mbar_wait_bounded(&tail.item_full, n_items & 1, p.status);
-    good = __all_sync(kFullMask, good);
-    Item it;
-    if (good) it = tail.item; else it = item_at<PREFIX>(p, plan, MT, t, end);
+    good = named_barrier_and(2, kMathWarps * 32, good);
+    if (!good) break;
+    const Item it = tail.item;
     const QueryRange uq = it.un.q;
     const int from = it.un.from, to = it.un.to;
     // this lane's two query rows: the tokens they see, and their fragments
@@ -494,40 +496,38 @@ struct CombineParams {
 
 constexpr int kCombineThreads = 128;
 
-// The parts of one (query token, query head) in one phase: those of CTAs [c0, c1], or the one finished item. A wide
-// launch leaves an item of at most kWideRows / 2 query rows in two halves, over alternate tiles.
+// The parts of an M tile's query rows in one phase: those of a run of CTAs, or the one finished item. A wide launch leaves an
+// item of at most kWideRows / 2 query rows in two halves, over alternate tiles.
 struct PartList {
   const float *o, *ml;
-  int count;
-  int halves;
-  int64_t first, rest, step, half;  // rows of the first CTA's part, of the second's, from there on, and of the other half
+  int count, halves;
+  bool whole;
+  int64_t first, rest, step, half;  // where the first CTA's part begins, the second's, one more, and the other half
 };
 
-__device__ __forceinline__ PartList list_parts(const AttendParams& p, const PhaseOut& ph, int unit, int nq, int m, int head,
-                                               int token, int qhead, int D) {
-  PartList out{nullptr, nullptr, 0, 1, 0, 0, 0, 0};
-  const int W = ph.cum[ph.units], n = sharing_ctas(W, ph.ctas);
+__device__ __forceinline__ PartList list_parts(const AttendParams& p, const PhaseOut& ph, int unit, int nq, int mt, int head, int D) {
+  PartList out{nullptr, nullptr, 0, 1, false, 0, 0, 0, 0};
+  const int W = ph.cum[ph.units], start = ph.cum[unit], span = ph.cum[unit + 1] - start;
   const int mts = (nq * p.G + ph.MT - 1) / ph.MT;
-  const int span = ph.cum[unit + 1] - ph.cum[unit];
   if (span == 0 || mts == 0) return out;
-  const int tiles = span / (mts * p.heads), mt = m / ph.MT;
-  const int a = ph.cum[unit] + (head * mts + mt) * tiles, b = a + tiles;
+  const int n = sharing_ctas(W, ph.ctas);
+  const int tiles = span / (mts * p.heads);
+  const int a = start + (head * mts + mt) * tiles, b = a + tiles;
   const int c0 = cta_of(a, W, n), c1 = cta_of(b - 1, W, n);
   const int64_t all = (int64_t)p.tokens * p.q_heads;
   if (ph.MT == kWideRows && nq * p.G - mt * ph.MT <= kWideRows / 2) out.halves = 2;
-  if (c0 == c1) {
+  out.whole = c0 == c1;
+  if (out.whole) {
     out.o = ph.whole;
     out.ml = ph.whole + all * (ph.MT == kWideRows ? 2 : 1) * D;
     out.count = 1;
-    out.first = (int64_t)token * p.q_heads + qhead;
     out.half = all;
   } else {
     out.o = ph.parts;
     out.ml = ph.parts + (int64_t)2 * ph.max_ctas * ph.MT * D;
     out.count = c1 - c0 + 1;
-    const int mi = m - mt * ph.MT;
-    out.first = (int64_t)(2 * c0 + 1) * ph.MT + mi;
-    out.rest = (int64_t)(2 * c0 + 2) * ph.MT + mi;
+    out.first = (int64_t)(2 * c0 + 1) * ph.MT;
+    out.rest = (int64_t)(2 * c0 + 2) * ph.MT;
     out.step = 2 * ph.MT;
     out.half = kWideRows / 2;
   }
@@ -535,14 +535,15 @@ __device__ __forceinline__ PartList list_parts(const AttendParams& p, const Phas
   return out;
 }
 
-__device__ __forceinline__ int64_t part_row(const PartList& l, int i) {
+// Part i's row; `at`: the query row's place in an M tile's part, or among all query rows where the list is whole.
+__device__ __forceinline__ int64_t part_row(const PartList& l, int i, int64_t at) {
   const int c = l.halves == 2 ? i >> 1 : i;
-  return (c == 0 ? l.first : l.rest + (c - 1) * l.step) + (l.halves == 2 && (i & 1) ? l.half : 0);
+  return at + (c == 0 ? l.first : l.rest + (c - 1) * l.step) + (l.halves == 2 && (i & 1) ? l.half : 0);
 }
 
-// CTAs per (row, KV head), a warp per query row in turn; every lane holds D / 32 dims. The parts are added in order.
+// CTAs per (row, KV head), a warp for each `run` query rows in turn; every lane holds D / 32 dims. The parts are added in order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineParams c) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ CombineParams c, int run) {
   const AttendParams& p = c.p;
   chain_release();
   chain_wait();
@@ -551,19 +552,37 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
   const Unit un = unit_at<false>(p, row, false);
   const int group = p.groups > 0 ? p.row_group[row] : -1;
   const int4 gi = group >= 0 ? p.group_info[group] : make_int4(0, 0, 0, 0);
-  for (int m0 = blockIdx.y * (kCombineThreads / 32) + (threadIdx.x >> 5); m0 < un.q.nq * p.G;
-       m0 += gridDim.y * (kCombineThreads / 32)) {
-    const int token = un.q.q0 + m0 / p.G, qhead = head * p.G + m0 % p.G;
-    PartList lists[2];
-    lists[0] = list_parts(p, c.own, row, un.q.nq, m0, head, token, qhead, D);
-    lists[1].count = 0;
-    if (group >= 0 && token >= gi.x && token < gi.x + gi.y)
-      lists[1] = list_parts(p, c.prefix, group, gi.y, (token - gi.x) * p.G + m0 % p.G, head, token, qhead, D);
-    else if (lists[0].count == 1 && p.groups == 0 && c.own.MT != kWideRows)
-      continue;  // the attention kernel wrote it
+  const int M = un.q.nq * p.G, lead = (un.q.q0 - gi.x) * p.G;  // the group's query rows before this row's
+  const int warps = gridDim.y * (kCombineThreads / 32), warp = blockIdx.y * (kCombineThreads / 32) + (threadIdx.x >> 5);
+  PartList lists[2];
+  lists[0].count = lists[1].count = 0;
+  int have[2] = {-1, -1};
+  int i = -1, g = 0;
+  for (int m0 = warp * run, in_run = 0; m0 < M; in_run + 1 < run ? (++in_run, ++m0) : (in_run = 0, m0 += (warps - 1) * run + 1)) {
+    if (in_run == 0) {
+      i = m0 / p.G;
+      g = m0 - i * p.G;
+    } else if (++g == p.G) {
+      g = 0;
+      ++i;
+    }
+    const int token = un.q.q0 + i, qhead = head * p.G + g;
+    const int64_t all = (int64_t)token * p.q_heads + qhead;
+    const int own_mt = m0 / c.own.MT;
+    if (own_mt != have[0]) lists[0] = list_parts(p, c.own, row, un.q.nq, have[0] = own_mt, head, D);
+    if (group >= 0 && lead + m0 >= 0 && lead + m0 < gi.y * p.G) {
+      const int prefix_mt = (lead + m0) / c.prefix.MT;
+      if (prefix_mt != have[1]) lists[1] = list_parts(p, c.prefix, group, gi.y, have[1] = prefix_mt, head, D);
+    } else {
+      lists[1].count = 0;
+      have[1] = -1;
+      if (p.groups == 0 && lists[0].count == 1 && c.own.MT != kWideRows) continue;  // the attention kernel wrote it
+    }
+    const int64_t place[2] = {lists[0].whole ? all : m0 - own_mt * c.own.MT,
+                              lists[1].whole ? all : lead + m0 - have[1] * c.prefix.MT};
     float m = -INFINITY;
     for (int k = 0; k < 2; ++k)
-      for (int i = lane; i < lists[k].count; i += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], i)]);
+      for (int j = lane; j < lists[k].count; j += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], j, place[k])]);
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
     float acc[D / 32], l = 0.f;
 #pragma unroll
@@ -574,7 +593,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
         float f = 0.f;
         int64_t at = 0;
         if (base + lane < lists[k].count) {
-          at = part_row(lists[k], base + lane);
+          at = part_row(lists[k], base + lane, place[k]);
           const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
           f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
           if (f != 0.f) l += ml.y * f;
@@ -743,8 +762,7 @@ int pick_mt(int64_t tokens, int units, int G) {
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
 int launch_attend(const AttendParams& p, int device, int sms, int* ctas, cudaStream_t s) {
-  const int units = PREFIX ? p.groups : p.rows;
-  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16 + plan_bytes(units);
+  const size_t smem = 1024 + Ring<D>::kBytes + (sizeof(Tail<D, WM, WN>) + 15) / 16 * 16;
   auto kernel = attend_kernel<T, D, WM, WN, PREFIX>;
   static LaunchCache cache;
   int resident = 0;
@@ -796,9 +814,11 @@ int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, 
     if (rc != EKV_OK) return rc;
   }
   c.p = p;
-  // warps for a row's average of query rows
-  const int per = kCombineThreads / 32, spread = (int)std::min<int64_t>(64, ((int64_t)p.tokens * p.G / p.rows + per - 1) / per);
-  launch_chained(combine_kernel<T, D>, dim3(p.rows * p.heads, max(spread, 1)), dim3(kCombineThreads), 0, s, c);
+  // warps for a row's average of query rows, several rows each where there are many: an M tile's list is made once for them
+  const int64_t average = std::max<int64_t>(1, (int64_t)p.tokens * p.G / p.rows);
+  const int per = kCombineThreads / 32, run = average >= 32 ? 4 : 1;
+  const int spread = (int)std::min<int64_t>(64, (average + per * run - 1) / (per * run));
+  launch_chained(combine_kernel<T, D>, dim3(p.rows * p.heads, spread), dim3(kCombineThreads), 0, s, c, run);
   return check_launch("combine_kernel");
 }
 

@@ -6,7 +6,7 @@
 // query rows are cut into M tiles, its tokens into tiles of kTile; the launch's tiles, numbered unit by
 // unit, KV head, M tile, token tile, are dealt evenly: CTA c of n takes tiles [c W / n, (c + 1) W / n). The units'
 // running tile counts come from the lengths on the device, so no plan travels through the host: without
-// groups every CTA scans them itself (one level of loads), with groups a one-CTA kernel goes ahead, since what a
+// groups every CTA adds them up itself (one level of loads), with groups a one-CTA kernel goes ahead, since what a
 // row shares takes a chain of dependent loads that would otherwise stand at the start of every CTA of every launch.
 //
 // Parts. A CTA that covers a whole (unit, KV head, M tile) finishes it; one that covers some of its tiles
@@ -124,72 +124,129 @@ __device__ __forceinline__ int token_limit(const AttendParams& p, const Unit& un
   return PREFIX ? p.limits[t] : un.to - un.q.nq + (t - un.q.q0) + 1;
 }
 
-// The running tile counts, in shared memory.
-struct Plan {
-  int* cum;  // [units + 1]
-  int units;
-};
-
-__host__ __device__ inline size_t plan_bytes(int units) { return ((size_t)(units + 1) * 4 + 15) / 16 * 16; }
-
-// Fills the plan with every thread of the CTA (THREADS of them); `scratch` holds THREADS / 32 + 1 ints.
-template <bool PREFIX, int THREADS, int TOKENS = kTile>
-__device__ __forceinline__ void make_plan(const AttendParams& p, const Plan& plan, int MT, int* scratch) {
-  if (PREFIX || p.groups > 0) {
-    for (int u = threadIdx.x; u <= plan.units; u += THREADS) plan.cum[u] = __ldcg(p.cum + u);
-    __syncthreads();
-    return;
-  }
-  const bool report = blockIdx.x == 0;
-  int carry = 0;
-  for (int base = 0; base < plan.units; base += THREADS) {
-    const int u = base + threadIdx.x;
-    int n = 0;
-    if (u < plan.units) {
-      const Unit un = unit_at<PREFIX>(p, u, report);
-      n = un.template tiles<TOKENS>() * p.heads * un.m_tiles(p, MT);
-    }
-    int total = 0;
-    const int before = block_exclusive_scan<THREADS>(n, scratch, &total);
-    if (u < plan.units) plan.cum[u] = carry + before;
-    carry += total;
-  }
-  if (threadIdx.x == 0) plan.cum[plan.units] = carry;
-  __syncthreads();
-  if (report && p.cum != nullptr)  // for the combine kernel
-    for (int u = threadIdx.x; u <= plan.units; u += THREADS) p.cum[u] = plan.cum[u];
-}
-
 // The tiles of CTA c when n CTAs share W, and the CTA that holds tile t.
 __device__ __forceinline__ int first_tile(int c, int W, int n) { return (int)((int64_t)c * W / n); }
-__device__ __forceinline__ int cta_of(int t, int W, int n) { return (int)((((int64_t)t + 1) * n - 1) / W); }
+__device__ __forceinline__ int cta_of(int t, int W, int n) {  // floor(((t + 1) n - 1) / W), by an estimate put right
+  const int64_t x = ((int64_t)t + 1) * n - 1;
+  int c = (int)((float)x / (float)W);
+  while ((int64_t)(c + 1) * W <= x) ++c;
+  while ((int64_t)c * W > x) --c;
+  return c;
+}
 __device__ __forceinline__ int sharing_ctas(int W, int ctas) { return W < ctas ? (W > 0 ? W : 1) : ctas; }
 
-// One item of a CTA's range: (unit, KV head, M tile) and its tiles [first, last) that the CTA covers.
+// A unit's tiles over all KV heads and M tiles.
+template <int TOKENS>
+__device__ __forceinline__ int unit_tiles(const AttendParams& p, const Unit& un, int MT) {
+  return un.template tiles<TOKENS>() * p.heads * un.m_tiles(p, MT);
+}
+
+// What a CTA is dealt: tiles [begin, end) of W, the first of them in unit `unit`, whose tiles start at `base`.
+struct Deal {
+  int begin, end, W, unit, base;
+};
+
+// With every thread of the CTA (THREADS of them); scratch holds THREADS / 32 + 1 ints, found 2. Without groups CTA 0 also
+// leaves the running counts for the combine kernel.
+template <bool PREFIX, int THREADS, int TOKENS = kTile>
+__device__ __forceinline__ Deal deal(const AttendParams& p, int units, int MT, int* scratch, int* found) {
+  Deal d;
+  const bool report = blockIdx.x == 0;
+  int mine = 0, before = 0;  // of the last THREADS units looked at
+  if (PREFIX || p.groups > 0) {
+    d.W = __ldcg(p.cum + units);
+  } else {
+    d.W = 0;
+    for (int base = 0; base < units; base += THREADS) {
+      const int u = base + threadIdx.x;
+      mine = u < units ? unit_tiles<TOKENS>(p, unit_at<PREFIX>(p, u, report), MT) : 0;
+      int total = 0;
+      before = d.W + block_exclusive_scan<THREADS>(mine, scratch, &total);
+      d.W += total;
+    }
+  }
+  const int n = sharing_ctas(d.W, gridDim.x);
+  if (threadIdx.x == 0) found[0] = found[1] = 0;
+  __syncthreads();
+  d.begin = (int)blockIdx.x < n ? first_tile(blockIdx.x, d.W, n) : d.W;
+  d.end = (int)blockIdx.x < n ? first_tile(blockIdx.x + 1, d.W, n) : d.W;
+  int carry = 0;
+  for (int base = 0; base < units; base += THREADS) {
+    const int u = base + threadIdx.x;
+    if (PREFIX || p.groups > 0) {
+      before = u < units ? __ldcg(p.cum + u) : d.W;
+      mine = u < units ? __ldcg(p.cum + u + 1) - before : 0;
+    } else if (units > THREADS) {
+      mine = u < units ? unit_tiles<TOKENS>(p, unit_at<PREFIX>(p, u, false), MT) : 0;
+      int total = 0;
+      before = carry + block_exclusive_scan<THREADS>(mine, scratch, &total);
+      carry += total;
+    }
+    if (u < units && before <= d.begin && d.begin < before + mine) {  // one thread at most
+      found[0] = u;
+      found[1] = before;
+    }
+    if (!PREFIX && p.groups == 0 && report && p.cum != nullptr && u < units) p.cum[u] = before;
+  }
+  if (!PREFIX && p.groups == 0 && report && p.cum != nullptr && threadIdx.x == 0) p.cum[units] = d.W;
+  __syncthreads();
+  d.unit = found[0];
+  d.base = found[1];
+  return d;
+}
+
+// One item of a CTA's tiles: (unit, KV head, M tile) and its tiles [first, last) that the CTA covers.
 struct Item {
   Unit un;
   int unit, head, mt, first, last, tiles;
 };
 
+// A warp's walk through the units from the one its CTA starts in, 32 of them in its lanes at a time, so that the next item
+// costs a vote and some shuffles and not a chain of loads.
 template <bool PREFIX, int TOKENS = kTile>
-__device__ __forceinline__ Item item_at(const AttendParams& p, const Plan& plan, int MT, int t, int end) {
-  int lo = 0, hi = plan.units;  // the last unit that starts at or before t (units without tiles never hold one)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (plan.cum[mid] <= t) lo = mid; else hi = mid;
+struct Walk {
+  Unit un;           // this lane's unit
+  int unit, start, count;
+  int MT, units;
+  __device__ __forceinline__ void load(const AttendParams& p, int first, int base) {
+    unit = first + (int)(threadIdx.x & 31);
+    un = Unit{{0, 0}, 0, 0, 0};
+    if (unit < units) un = unit_at<PREFIX>(p, unit, false);
+    count = unit_tiles<TOKENS>(p, un, MT);
+    int incl = count;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(kFullMask, incl, off);
+      if ((int)(threadIdx.x & 31) >= off) incl += v;
+    }
+    start = base + incl - count;
   }
-  Item it;
-  it.unit = lo;
-  it.un = unit_at<PREFIX>(p, lo, false);
-  it.tiles = it.un.template tiles<TOKENS>();
-  const int mts = it.un.m_tiles(p, MT);
-  const int rem = t - plan.cum[lo], hm = rem / it.tiles;
-  it.head = hm / mts;
-  it.mt = hm - it.head * mts;
-  it.first = rem - hm * it.tiles;
-  it.last = min(it.tiles, it.first + end - t);
-  return it;
-}
+  __device__ __forceinline__ Walk(const AttendParams& p, const Deal& d, int units_, int MT_) : MT(MT_), units(units_) { load(p, d.unit, d.base); }
+  // The item that tile t (at or past the one before's) starts or continues; with the whole warp.
+  __device__ __forceinline__ Item at(const AttendParams& p, int t, int end) {
+    uint32_t here;
+    while ((here = __ballot_sync(kFullMask, start <= t && t < start + count)) == 0) {
+      const int next = __shfl_sync(kFullMask, unit, 31) + 1, base = __shfl_sync(kFullMask, start + count, 31);
+      if (next >= units) break;  // no tile is past the last unit
+      load(p, next, base);
+    }
+    const int l = here ? __ffs(here) - 1 : 0;
+    Item it;
+    it.un.q.q0 = __shfl_sync(kFullMask, un.q.q0, l);
+    it.un.q.nq = __shfl_sync(kFullMask, un.q.nq, l);
+    it.un.row = __shfl_sync(kFullMask, un.row, l);
+    it.un.from = __shfl_sync(kFullMask, un.from, l);
+    it.un.to = __shfl_sync(kFullMask, un.to, l);
+    it.unit = __shfl_sync(kFullMask, unit, l);
+    it.tiles = max(it.un.template tiles<TOKENS>(), 1);
+    const int mts = max(it.un.m_tiles(p, MT), 1);
+    const int rem = t - __shfl_sync(kFullMask, start, l), hm = rem / it.tiles;
+    it.head = hm / mts;
+    it.mt = hm - it.head * mts;
+    it.first = rem - hm * it.tiles;
+    it.last = min(it.tiles, it.first + end - t);
+    return it;
+  }
+};
 
 // ---- copies ------------------------------------------------------------------------------------------------
 
@@ -203,6 +260,16 @@ __device__ __forceinline__ void tensor_copy_4d(uint32_t dst, const CUtensorMap* 
 }
 
 __device__ __forceinline__ void proxy_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Whether `ok` holds for all `threads` that meet at the barrier.
+__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(all)
+               : "r"(id), "r"(threads), "r"((uint32_t)ok)
+               : "memory");
+  return all != 0;
+}
 
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

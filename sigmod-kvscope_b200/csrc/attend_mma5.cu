@@ -42,7 +42,7 @@ struct WideTail {
   uint64_t full[Wide<D>::kSlots], empty[Wide<D>::kSlots];
   uint64_t q_full[2], s_full[2], p_ready[2], o_full[2], o_free[2], drained;
   uint32_t tmem;
-  int scratch[kThreads / 32 + 1];
+  int scratch[kThreads / 32 + 1], found[2];
 };
 
 template <typename T>
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   uint8_t* queries = base;              // [2] subtiles
   uint8_t* ring = base + 2 * R::kSlot;  // [kSlots]
   WideTail<D>& tail = *reinterpret_cast<WideTail<D>*>(ring + R::kRing);
-  const Plan plan{reinterpret_cast<int*>(ring + R::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16), PREFIX ? p.groups : p.rows};
+  const int units = PREFIX ? p.groups : p.rows;
   const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < R::kSlots; ++s) {
@@ -238,11 +238,10 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     fence_mbar_init();
   }
   chain_wait();
-  make_plan<PREFIX, kThreads, kTokens>(p, plan, kWideRows, tail.scratch);
-  const int W = plan.cum[plan.units];
-  const int n = sharing_ctas(W, gridDim.x);
+  const Deal dealt = deal<PREFIX, kThreads, kTokens>(p, units, kWideRows, tail.scratch, tail.found);
+  const int begin = dealt.begin, end = dealt.end;
   chain_release();
-  if ((int)blockIdx.x >= n || W == 0) return;
+  if (begin >= end) return;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem)), "r"(kColumns)
                  : "memory");
@@ -252,8 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tail.tmem;
-  const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
   const int per_tile = kTokens >> p.block_shift;  // blocks of a tile
+  Walk<PREFIX, kTokens> walk(p, dealt, units, kWideRows);
   bool good = true;  // after a wait that gave up a role goes on without waiting, so that every role ends
 
   if (warp == kCopyWarp) {
@@ -262,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     int slot = 0, issued = 0;
     uint32_t phase = 0;
     for (int t = begin; t < end && good;) {
-      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const Item it = walk.at(p, t, end);
       const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
       const int block0 = it.un.from >> p.block_shift, last_block = (it.un.to - 1) >> p.block_shift;
       const int tiles = it.last - it.first;
@@ -353,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       __syncwarp();
     };
     for (int t = begin; t < end;) {
-      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const Item it = walk.at(p, t, end);
       const Share sh = share_of(p, it);
       int ks = take();
       if (sh.single) {
@@ -423,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     uint32_t s_uses = 0, o_uses = 0;
     const float grow = 8.f / p.scale_log2;
     for (int t = begin; t < end;) {
-      const Item it = item_at<PREFIX, kTokens>(p, plan, kWideRows, t, end);
+      const Item it = walk.at(p, t, end);
       const Share sh = share_of(p, it);
       const QueryRange uq = it.un.q;
       const int mi = sh.single ? row : w * kSub + row, mrow = it.mt * kWideRows + mi;
@@ -532,8 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
 
 template <typename T, int D, bool PREFIX>
 int launch(const AttendParams& p, int device, int sms, int* ctas, cudaStream_t s) {
-  const int units = PREFIX ? p.groups : p.rows;
-  const size_t smem = 1024 + 2 * Wide<D>::kSlot + Wide<D>::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16 + plan_bytes(units);
+  const size_t smem = 1024 + 2 * Wide<D>::kSlot + Wide<D>::kRing + (sizeof(WideTail<D>) + 15) / 16 * 16;
   auto kernel = wide_kernel<T, D, PREFIX>;
   static LaunchCache cache;
   int resident = 0;

@@ -111,7 +111,7 @@ template <int D>
 struct Tail {
   uint64_t full[Ring<D>::kSlots], empty[Ring<D>::kSlots], q_full, s_full[2], s_free[2], drained;
   uint32_t tmem;
-  int scratch[kThreads / 32 + 1];
+  int scratch[kThreads / 32 + 1], found[2];
   alignas(16) float lse[kColumns];
   alignas(16) int limit[kColumns];
 };
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
   uint8_t* queries = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* ring = queries + R::kQueries;
   Tail<D>& tail = *reinterpret_cast<Tail<D>*>(ring + R::kBytes);
-  const Plan plan{reinterpret_cast<int*>(ring + R::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16), p.rows};
+  const int units = p.rows;
   const int warp = __shfl_sync(kFullMask, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < R::kSlots; ++s) {
@@ -140,11 +140,10 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     fence_mbar_init();
   }
   chain_wait();  // the attention's log-sum-exps
-  make_plan<false, kThreads, kTokens>(p, plan, kOneTile, tail.scratch);
+  const Deal dealt = deal<false, kThreads, kTokens>(p, units, kOneTile, tail.scratch, tail.found);
+  const int begin = dealt.begin, end = dealt.end;
   chain_release();
-  const int W = plan.cum[plan.units];
-  const int n = sharing_ctas(W, gridDim.x);
-  if ((int)blockIdx.x >= n || W == 0) return;
+  if (begin >= end) return;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem)), "r"(512)
                  : "memory");
@@ -154,8 +153,8 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tail.tmem;
-  const int begin = first_tile(blockIdx.x, W, n), end = first_tile(blockIdx.x + 1, W, n);
   const int per_tile = kTokens >> p.block_shift;
+  Walk<false, kTokens> walk(p, dealt, units, kOneTile);
   bool good = true;  // after a wait that gave up a role goes on without waiting, so that every role ends
 
   if (warp == kCopyWarp) {
@@ -164,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     int slot = 0, issued = 0;
     uint32_t phase = 0;
     for (int t = begin; t < end && good;) {
-      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
+      const Item it = walk.at(p, t, end);
       const int32_t* ids = p.table + (int64_t)it.un.row * p.table_s0;
       const int last_block = (it.un.to - 1) >> p.block_shift;
       for (int m0 = 0; m0 < it.un.q.nq * p.G && good; m0 += kColumns) {
@@ -204,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
       tc_fence_after();
     };
     for (int t = begin; t < end;) {
-      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
+      const Item it = walk.at(p, t, end);
       const int M = it.un.q.nq * p.G;
       for (int m0 = 0; m0 < M; m0 += kColumns) {
         const uint32_t shape = mma_shape<std::is_same<T, __half>::value>((min(M - m0, kColumns) + 15) / 16 * 16, false);
@@ -234,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
     const uint32_t s_at = tmem + w * kColumns + ((uint32_t)(warp & 3) << 21);
     uint32_t s_uses = 0;
     for (int t = begin; t < end;) {
-      const Item it = item_at<false, kTokens>(p, plan, kOneTile, t, end);
+      const Item it = walk.at(p, t, end);
       const QueryRange uq = it.un.q;
       const int to = it.un.to, M = uq.nq * p.G;
       const int slot = slot_of(sp, it.unit, lane);
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
 
 template <typename T, int D>
 int launch_weigh(const ScoreParams& p, int device, int sms, cudaStream_t s) {
-  const size_t smem = 1024 + Ring<D>::kQueries + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16 + plan_bytes(p.a.rows);
+  const size_t smem = 1024 + Ring<D>::kQueries + Ring<D>::kBytes + (sizeof(Tail<D>) + 15) / 16 * 16;
   auto kernel = weigh_kernel<T, D>;
   static LaunchCache cache;
   int resident = 0;
