@@ -62,13 +62,16 @@ __device__ __forceinline__ uint32_t chunk_at(int t, int c) {
 // The shared memory behind the ring.
 template <int D, int WM, int WN>
 struct Tail {
-  static constexpr int kRows = WN > 1 ? 4 / WM : 1;  // query rows of each of the WM that join at a time
+  // query rows of each of the WM that join at a time: all where they fit beside two CTAs' rings, else a few
+  static constexpr int kRows = WN == 1 ? 1 : D == 64 ? 16 : 4 / WM;
   uint64_t full[Ring<D>::kStages], empty[Ring<D>::kStages];
   uint64_t item_full, item_empty;
   uint32_t blocks[Ring<D>::kStages];  // which of the stage's blocks were copied (bit b: the tile's block b)
   int scratch[kThreads / 32 + 1], found[2];
   Item item;  // what the math warps take next
   float m[2][WN > 1 ? WN : 1][16 * WM], l[2][WN > 1 ? WN : 1][16 * WM];  // of one item and of the next
+  float inverse[16 * WM];   // of a row's sum, or 1 where the part is not the row's last
+  int64_t target[16 * WM];  // where a row's output goes, or -1
   alignas(16) float o[WN > 1 ? WM * WN * kRows : 1][WN > 1 ? D + 8 : 4];
   alignas(16) uint8_t queries[WN > 1 ? 16 * WM * D * 2 : 16];  // the item's query rows, in 16-byte pieces turned by the row
 };
@@ -383,9 +386,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       }
     };
     if constexpr (WN > 1) {
-      // The WN warps of a row join through shared memory, a few rows at a time, in the warps' order: each scales its part to
-      // the common maximum, and then every thread adds four dims of a row and writes them, a row's lanes side by side.
-      constexpr int kRows = TailT::kRows, kPer = 8 / kRows;
+      // The WN warps of a row join through shared memory in the warps' order: a thread a row finds the row's maximum, its sum
+      // and its place; each warp scales its part to the maximum; then every thread adds four dims of a row and writes them, a
+      // row's lanes side by side.
+      constexpr int kRows = TailT::kRows;
       float(&ms)[WN][16 * WM] = tail.m[n_items & 1], (&ls)[WN][16 * WM] = tail.l[n_items & 1];
       if (pair == 0) {
 #pragma unroll
@@ -395,10 +399,36 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         }
       }
       named_barrier(1, kMathWarps * 32);
+      if (threadIdx.x < MT) {
+        const int mrow = it.mt * MT + threadIdx.x;
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][threadIdx.x]);
+#pragma unroll
+        for (int w = 0; w < WN; ++w)
+          total += ms[w][threadIdx.x] == -INFINITY ? 0.f : ls[w][threadIdx.x] * exp2_fast(ms[w][threadIdx.x] - top);
+        int64_t target = -1;
+        if (mrow < uq.nq * p.G) {
+          const int i = mrow / p.G, token = uq.q0 + i, head = it.head * p.G + mrow - i * p.G;
+          if (final) {
+            target = (int64_t)token * p.out_s0 + (int64_t)head * p.out_s1;
+            if (p.lse != nullptr)
+              p.lse[(int64_t)token * p.q_heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+          } else {
+            float *dst, *ml;
+            part_at(mrow, token, head, dst, ml);
+            target = dst - p.parts;
+            *reinterpret_cast<float2*>(ml) = make_float2(top, total);
+          }
+        }
+        tail.target[threadIdx.x] = target;
+        tail.inverse[threadIdx.x] = final ? (total == 0.f ? 0.f : 1.f / total) : 1.f;
+      }
       float f[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float top = -INFINITY;
+#pragma unroll
         for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][wm * 16 + quad + 8 * j]);
         f[j] = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - top);
       }
@@ -407,47 +437,39 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       for (int round = 0; round < 16 / kRows; ++round) {
         if (round * kRows >= rows) break;
         if (round > 0) named_barrier(1, kMathWarps * 32);
-        constexpr int kQuads = kRows;
-        const int j = round / kPer;  // constant in the unrolled loop
-        if (quad / kQuads == round % kPer) {
-          float* dst = tail.o[(wm * WN + wn) * kRows + quad % kQuads] + 2 * pair;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if ((quad + 8 * j) / kRows != round) continue;
+          float* dst = tail.o[(wm * WN + wn) * kRows + (quad + 8 * j) % kRows] + 2 * pair;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d)
             *reinterpret_cast<float2*>(dst + 8 * d) =
                 f[j] == 0.f ? make_float2(0.f, 0.f) : make_float2(o[d][2 * j] * f[j], o[d][2 * j + 1] * f[j]);
         }
         named_barrier(1, kMathWarps * 32);
-        const int i = wn * 32 + lane, r = i / (D / 4), c = i % (D / 4);  // this thread's row of the round and its four dims
-        const int tile_row = wm * 16 + round * kRows + r, mrow = it.mt * MT + tile_row;
-        if (r < kRows && mrow < uq.nq * p.G) {
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          float top = -INFINITY, total = 0.f;
 #pragma unroll
-          for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][tile_row]);
+        for (int at = 0; at < kRows * D / 4; at += WN * 32) {
+          const int i = at + wn * 32 + lane, r = i / (D / 4), c = i % (D / 4);  // a row of the round and four of its dims
+          const int tile_row = wm * 16 + round * kRows + r;
+          const int64_t target = r < kRows ? tail.target[tile_row] : -1;
+          if (target < 0) continue;
+          const float inv = tail.inverse[tile_row];
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < WN; ++w) {
             const float4 v = *reinterpret_cast<const float4*>(tail.o[(wm * WN + w) * kRows + r] + 4 * c);
-            const float mw = ms[w][tile_row];
-            total += mw == -INFINITY ? 0.f : ls[w][tile_row] * exp2_fast(mw - top);
             sum.x += v.x;
             sum.y += v.y;
             sum.z += v.z;
             sum.w += v.w;
           }
-          const int token = uq.q0 + mrow / p.G, head = it.head * p.G + mrow % p.G;
-          if (final) {
-            const float inv = 1.f / total;
+          if (final) {  // a row that saw nothing has an inverse of 0
             uint2 v;
-            v.x = total == 0.f ? 0u : pack2<T>(sum.x * inv, sum.y * inv);
-            v.y = total == 0.f ? 0u : pack2<T>(sum.z * inv, sum.w * inv);
-            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (int64_t)token * p.out_s0 + (int64_t)head * p.out_s1 + 4 * c) = v;
-            if (p.lse != nullptr && c == 0)
-              p.lse[(int64_t)token * p.q_heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+            v.x = inv == 0.f ? 0u : pack2<T>(sum.x * inv, sum.y * inv);
+            v.y = inv == 0.f ? 0u : pack2<T>(sum.z * inv, sum.w * inv);
+            *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + target + 4 * c) = v;
           } else {
-            float *dst, *ml;
-            part_at(mrow, token, head, dst, ml);
-            *reinterpret_cast<float4*>(dst + 4 * c) = sum;
-            if (c == 0) *reinterpret_cast<float2*>(ml) = make_float2(top, total);
+            *reinterpret_cast<float4*>(p.parts + target + 4 * c) = sum;
           }
         }
       }
@@ -580,45 +602,62 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
     }
     const int64_t place[2] = {lists[0].whole ? all : m0 - own_mt * c.own.MT,
                               lists[1].whole ? all : lead + m0 - have[1] * c.prefix.MT};
-    float m = -INFINITY;
-    for (int k = 0; k < 2; ++k)
-      for (int j = lane; j < lists[k].count; j += 32) m = fmaxf(m, lists[k].ml[2 * part_row(lists[k], j, place[k])]);
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
-    float acc[D / 32], l = 0.f;
+    // Parts 32 at a time, a lane each for its maximum and sum; their outputs are asked for before those arrive (a part that
+    // holds nothing has a factor of 0 and its loads are not used), eight at a time and the next eight beside them.
+    const int total = lists[0].count + lists[1].count;
+    float m = -INFINITY, l = 0.f, acc[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
-    for (int k = 0; k < 2; ++k) {
-      for (int base = 0; base < lists[k].count; base += 32) {
-        // a lane a part: its factor (0: nothing of it is read), then the outputs, eight loads in flight
-        float f = 0.f;
-        int64_t at = 0;
-        if (base + lane < lists[k].count) {
-          at = part_row(lists[k], base + lane, place[k]);
-          const float2 ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
-          f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - m);
-          if (f != 0.f) l += ml.y * f;
-        }
-        const int count = min(32, lists[k].count - base);
-        for (int i0 = 0; i0 < count; i0 += 8) {
-          float o[8][D / 32], fs[8];
+    for (int base = 0; base < total; base += 32) {
+      const int j = base + lane, k = j < lists[0].count ? 0 : 1;
+      const float* src = nullptr;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (j < total) {
+        const int64_t at = part_row(lists[k], k == 0 ? j : j - lists[0].count, place[k]);
+        src = lists[k].o + at * D;
+        ml = *reinterpret_cast<const float2*>(lists[k].ml + 2 * at);
+      }
+      const int count = min(32, total - base);
+      float o[2][8][D / 32];
+      auto ask = [&](int i0, float(&to)[8][D / 32]) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            fs[i] = __shfl_sync(kFullMask, f, i0 + i);
-            const int64_t row_at = __shfl_sync(kFullMask, at, i0 + i);
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) o[i][d] = 0.f;
-            if (fs[i] != 0.f) {  // lanes behind the last part have a factor of 0
-              if constexpr (D == 128)
-                *reinterpret_cast<float4*>(o[i]) = *reinterpret_cast<const float4*>(lists[k].o + row_at * D + lane * 4);
-              else
-                *reinterpret_cast<float2*>(o[i]) = *reinterpret_cast<const float2*>(lists[k].o + row_at * D + lane * 2);
-            }
+        for (int i = 0; i < 8; ++i) {
+          const float* from = reinterpret_cast<const float*>(__shfl_sync(kFullMask, reinterpret_cast<unsigned long long>(src), i0 + i));
+          if (i0 + i < count) {
+            if constexpr (D == 128)
+              *reinterpret_cast<float4*>(to[i]) = *reinterpret_cast<const float4*>(from + lane * 4);
+            else
+              *reinterpret_cast<float2*>(to[i]) = *reinterpret_cast<const float2*>(from + lane * 2);
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) acc[d] = fmaf(o[i][d], fs[i], acc[d]);
         }
+      };
+      ask(0, o[0]);
+      float top = ml.x;
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+      top = fmaxf(top, m);
+      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
+      const float keep = m == -INFINITY ? 0.f : exp2_fast(m - top);
+      m = top;
+      l = l * keep + (f == 0.f ? 0.f : f * ml.y);
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) acc[d] *= keep;
+      auto add = [&](int i0, const float(&from)[8][D / 32]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float fi = __shfl_sync(kFullMask, f, i0 + i);
+          if (fi != 0.f) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) acc[d] = fmaf(from[i][d], fi, acc[d]);
+          }
+        }
+      };
+#pragma unroll
+      for (int i0 = 0; i0 < 32; i0 += 16) {
+        if (i0 >= count) break;
+        if (i0 + 8 < count) ask(i0 + 8, o[1]);
+        add(i0, o[0]);
+        if (i0 + 16 < count) ask(i0 + 16, o[0]);
+        if (i0 + 8 < count) add(i0 + 8, o[1]);
       }
     }
     for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
@@ -678,6 +717,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
   }
   __syncthreads();
+  bool more = false;
   const int own_tokens = pp.mt_own == kWideRows ? 2 * kTile : kTile;
   running_sum(pp.cum_own, p.rows, scratch, [&](int r) {
     const QueryRange q = row_queries(p, r, true);
@@ -693,12 +733,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     p.row_info[r] = make_int4(q.q0, q.nq, from, to);
     p.row_group[r] = in ? lo : -1;
     for (int i = 0; i < min(q.nq, 8); ++i) p.limits[q.q0 + i] = min(to - q.nq + i + 1, from);
+    more |= q.nq > 8;
     return to > from && q.nq > 0 ? (to - from + own_tokens - 1) / own_tokens * p.heads * ((q.nq * p.G + pp.mt_own - 1) / pp.mt_own)
                                  : 0;
   });
-  __syncthreads();
+  more = __syncthreads_or(more);
   // rows of many query tokens: their limits by a warp
-  for (int r = threadIdx.x >> 5; r < p.rows && p.tokens > 8; r += kPlanThreads / 32) {
+  for (int r = threadIdx.x >> 5; r < p.rows && more; r += kPlanThreads / 32) {
     const int4 v = p.row_info[r];
     for (int i = 8 + lane; i < v.y; i += 32) p.limits[v.x + i] = min(v.w - v.y + i + 1, v.z);
   }
@@ -816,7 +857,7 @@ int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, 
   c.p = p;
   // warps for a row's average of query rows, several rows each where there are many: an M tile's list is made once for them
   const int64_t average = std::max<int64_t>(1, (int64_t)p.tokens * p.G / p.rows);
-  const int per = kCombineThreads / 32, run = average >= 32 ? 4 : 1;
+  const int per = kCombineThreads / 32, run = average >= 128 ? 4 : average >= 32 ? 2 : 1;
   const int spread = (int)std::min<int64_t>(64, (average + per * run - 1) / (per * run));
   launch_chained(combine_kernel<T, D>, dim3(p.rows * p.heads, spread), dim3(kCombineThreads), 0, s, c, run);
   return check_launch("combine_kernel");
