@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import sys
 
 LIB_NAME = "libekv_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
@@ -203,15 +204,12 @@ class on_device:
         self.index = device.index
 
     def __enter__(self) -> int:
-        import torch
-
-        self.before = torch._C._cuda_getDevice()
+        c = sys.modules["torch"]._C
+        self.before = c._cuda_getDevice()
         if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+            c._cuda_setDevice(self.index)
+        return c._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *_) -> None:
         if self.before != self.index:
-            import torch
-
-            torch.cuda.set_device(self.before)
+            sys.modules["torch"]._C._cuda_setDevice(self.before)

@@ -27,41 +27,47 @@ def _index(name: str, t: torch.Tensor | None, size: int, device: torch.device) -
     """The address of an int32 index array of at least ``size`` entries on the call's device."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < size or t.device != device or (size > 1 and t.stride(0) != 1):
+    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) < size or t.device != device or (size > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a contiguous int32 tensor of at least {size} entries on {device}")
     return t.data_ptr()
 
 
-def _check_batch(query: torch.Tensor, kv_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> None:
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2:
-        raise ValueError(f"expected a KV cache [blocks, 2, block, heads, dim], got {tuple(kv_cache.shape)}")
-    if query.dim() != 3 or query.shape[2] != kv_cache.shape[4]:
-        raise ValueError(f"expected a query [tokens, heads, {kv_cache.shape[4]}], got {tuple(query.shape)}")
-    if query.dtype not in _DTYPES or kv_cache.dtype != query.dtype:
+def _batch(query: torch.Tensor, kv_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> tuple:
+    """What a call passes on of its batch, checked: each tensor's shape and strides are asked for once."""
+    q_shape, kv_shape, table_shape = query.shape, kv_cache.shape, table.shape
+    if len(kv_shape) != 5 or kv_shape[1] != 2:
+        raise ValueError(f"expected a KV cache [blocks, 2, block, heads, dim], got {tuple(kv_shape)}")
+    if len(q_shape) != 3 or q_shape[2] != kv_shape[4]:
+        raise ValueError(f"expected a query [tokens, heads, {kv_shape[4]}], got {tuple(q_shape)}")
+    dtype = _DTYPES.get(query.dtype)
+    if dtype is None or kv_cache.dtype is not query.dtype:
         raise ValueError(f"query and cache must both be float16 or bfloat16, got {query.dtype}, {kv_cache.dtype}")
-    if query.stride(2) != 1 or kv_cache.stride(4) != 1:
+    q_stride, kv_stride = query.stride(), kv_cache.stride()
+    if q_stride[2] != 1 or kv_stride[4] != 1:
         raise ValueError("the head dimension of the query and the cache must be contiguous")
-    if table.dtype != torch.int32 or lens.dtype != torch.int32:
+    if table.dtype is not torch.int32 or lens.dtype is not torch.int32:
         raise ValueError("the block table and the lengths must be int32")
-    if table.dim() != 2 or lens.dim() != 1 or lens.shape[0] < table.shape[0]:
+    if len(table_shape) != 2 or lens.dim() != 1 or len(lens) < table_shape[0]:
         raise ValueError("the block table must be [rows, width] with a length per row")
-    if (table.shape[1] > 1 and table.stride(1) != 1) or (lens.shape[0] > 1 and lens.stride(0) != 1):
+    table_stride = table.stride()
+    if (table_shape[1] > 1 and table_stride[1] != 1) or (table_shape[0] > 1 and lens.stride(0) != 1):
         raise ValueError("the block table's rows and the lengths must be contiguous")
     device = query.device
     if device.type != "cuda":
         raise ValueError("the attention runs on the device: the query must be a CUDA tensor")
     if kv_cache.device != device or table.device != device or lens.device != device:
         raise ValueError(f"the cache, the block table and the lengths must be on the query's device {device}")
+    return device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride[0]
 
 
 def _outputs(query: torch.Tensor, out: torch.Tensor | None, lse: torch.Tensor | None):
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or out.stride(2) != 1:
+        out = torch.empty_like(query)
+    elif out.shape != query.shape or out.dtype is not query.dtype or out.device != query.device or out.stride(2) != 1:
         raise ValueError("out must match the query's shape, dtype and device, its head dimension contiguous")
     if lse is None:
-        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
-    elif lse.shape != query.shape[:2] or lse.dtype != torch.float32 or lse.device != query.device or not lse.is_contiguous():
+        lse = query.new_empty(query.shape[:2], dtype=torch.float32)
+    elif lse.shape != query.shape[:2] or lse.dtype is not torch.float32 or lse.device != query.device or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous float32 {tuple(query.shape[:2])} tensor on the query's device")
     return out, lse
 
@@ -69,7 +75,7 @@ def _outputs(query: torch.Tensor, out: torch.Tensor | None, lse: torch.Tensor | 
 def _status(status: torch.Tensor | None, device: torch.device) -> int | None:
     if status is None:
         return None
-    if status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+    if status.dtype is not torch.int32 or status.numel() != 1 or status.device != device:
         raise ValueError(f"status must be one int32 on {device}")
     return status.data_ptr()
 
@@ -104,11 +110,10 @@ def attend(
     token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
     in the tables, which the kernels skip. The call runs on the current stream of the query's device.
     """
-    _check_batch(query, kv_cache, table, lens)
-    device = query.device
-    tokens, q_heads, dim = query.shape
-    rows, width = table.shape
-    blocks, _, block_size, kv_heads, _ = kv_cache.shape
+    device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride = _batch(query, kv_cache, table, lens)
+    tokens, q_heads, dim = q_shape
+    rows, width = table_shape
+    blocks, _, block_size, kv_heads, _ = kv_shape
     groups = common = 0
     prefix = None
     if isinstance(prefix_blocks, torch.Tensor):
@@ -131,29 +136,32 @@ def attend(
     out, lse = _outputs(query, out, lse)
     if tokens == 0 or rows == 0:
         return out, lse
+    out_stride = out.stride()
     lib = _lib.load()
     size = lib.ekv_attend_workspace_bytes(rows, tokens, groups, q_heads, kv_heads, dim)
     with _lib.on_device(device) as stream:
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = query.new_empty(size, dtype=torch.uint8)
         rc = lib.ekv_attend(
-            query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
-            kv_cache.stride(1), kv_cache.stride(2), kv_cache.stride(3), blocks, table.data_ptr(), table.stride(0),
-            lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
-            scale, groups, members, prefix, common, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+            query.data_ptr(), q_stride[0], q_stride[1], kv_cache.data_ptr(), kv_stride[0], kv_stride[1], kv_stride[2],
+            kv_stride[3], blocks, table.data_ptr(), table_stride, lens.data_ptr(), starts, tokens, rows, width, block_size,
+            q_heads, kv_heads, dim, dtype,
+            scale, groups, members, prefix, common, out.data_ptr(), out_stride[0], out_stride[1], lse.data_ptr(),
             workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_attend")
     return out, lse
 
 
-def check_scores(scores: torch.Tensor, heads: int, tokens: int, device: torch.device) -> None:
-    """A score table [slots, heads, >= tokens] float32 on ``device``, each head's scores contiguous."""
-    if scores.dtype != torch.float32 or scores.dim() != 3 or scores.device != device:
+def check_scores(scores: torch.Tensor, heads: int, tokens: int, device: torch.device) -> tuple:
+    """The strides of a score table [slots, heads, >= tokens] float32 on ``device``, each head's scores contiguous."""
+    shape, stride = scores.shape, scores.stride()
+    if scores.dtype is not torch.float32 or len(shape) != 3 or scores.device != device:
         raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor on {device}")
-    if scores.shape[1] != heads or scores.shape[2] < tokens:
-        raise ValueError(f"scores of {heads} heads and at least {tokens} tokens are needed, got {tuple(scores.shape)}")
-    if scores.stride(2) != 1:
+    if shape[1] != heads or shape[2] < tokens:
+        raise ValueError(f"scores of {heads} heads and at least {tokens} tokens are needed, got {tuple(shape)}")
+    if stride[2] != 1:
         raise ValueError("the scores of a head must be contiguous")
+    return stride
 
 
 def attend_scored(
@@ -183,12 +191,11 @@ def attend_scored(
 
     The other arguments, and the ``(out, lse)`` returned, are ``attend``'s.
     """
-    _check_batch(query, kv_cache, table, lens)
-    device = query.device
-    tokens, q_heads, dim = query.shape
-    rows, width = table.shape
-    blocks, _, block_size, kv_heads, _ = kv_cache.shape
-    check_scores(scores, kv_heads, width * block_size, device)
+    device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride = _batch(query, kv_cache, table, lens)
+    tokens, q_heads, dim = q_shape
+    rows, width = table_shape
+    blocks, _, block_size, kv_heads, _ = kv_shape
+    score_stride = check_scores(scores, kv_heads, width * block_size, device)
     starts = _index("query_start", query_start, rows + 1, device)
     places = _index("slots", slots, rows, device)
     new = _index("fresh", fresh, rows, device)
@@ -200,17 +207,17 @@ def attend_scored(
     out, lse = _outputs(query, out, lse)
     if tokens == 0 or rows == 0:
         return out, lse
+    out_stride = out.stride()
     lib = _lib.load()
     size = lib.ekv_attend_scored_workspace_bytes(rows, tokens, width, block_size, q_heads, kv_heads, dim)
     with _lib.on_device(device) as stream:
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = query.new_empty(size, dtype=torch.uint8)
         rc = lib.ekv_attend_scored(
-            query.data_ptr(), query.stride(0), query.stride(1), kv_cache.data_ptr(), kv_cache.stride(0),
-            kv_cache.stride(1), kv_cache.stride(2), kv_cache.stride(3), blocks, table.data_ptr(), table.stride(0),
-            lens.data_ptr(), starts, tokens, rows, width, block_size, q_heads, kv_heads, dim, _DTYPES[query.dtype],
-            scale, scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[0], places, new, decay,
-            out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), workspace.data_ptr(), size, word,
-            stream,
+            query.data_ptr(), q_stride[0], q_stride[1], kv_cache.data_ptr(), kv_stride[0], kv_stride[1], kv_stride[2],
+            kv_stride[3], blocks, table.data_ptr(), table_stride, lens.data_ptr(), starts, tokens, rows, width, block_size,
+            q_heads, kv_heads, dim, dtype,
+            scale, scores.data_ptr(), score_stride[0], score_stride[1], len(scores), places, new, decay,
+            out.data_ptr(), out_stride[0], out_stride[1], lse.data_ptr(), workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_attend_scored")
     return out, lse

@@ -40,7 +40,7 @@ def select_tokens(
     if scores.dim() != 3:
         raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor, got {tuple(scores.shape)}")
     n_slots, heads, capacity = scores.shape
-    check_scores(scores, heads, 1, device)
+    stride = check_scores(scores, heads, 1, device)
     if device.type != "cuda":
         raise ValueError("the selection runs on the device: scores must be a CUDA tensor")
     if lens.dim() != 1:
@@ -54,20 +54,21 @@ def select_tokens(
         raise ValueError("first_tokens and recent_tokens must not be negative")
     counts, count = (_index("keep", keep, rows, device), 0) if isinstance(keep, torch.Tensor) else (None, int(keep))
     if kept is None:
-        kept = torch.empty(rows, heads, capacity, dtype=torch.int32, device=device)
-    elif kept.shape != (rows, heads, capacity) or kept.dtype != torch.int32 or kept.device != device or kept.stride(2) != 1:
+        kept = scores.new_empty((rows, heads, capacity), dtype=torch.int32)
+    elif kept.shape != (rows, heads, capacity) or kept.dtype is not torch.int32 or kept.device != device or kept.stride(2) != 1:
         raise ValueError(f"kept must be an int32 [{rows}, {heads}, {capacity}] tensor on {device}")
     if new_lens is None:
-        new_lens = torch.empty(rows, dtype=torch.int32, device=device)
+        new_lens = lens.new_empty(rows)
     new = _index("new_lens", new_lens, rows, device)
     word = _status(status, device)
     if rows == 0:
         return kept, new_lens
+    kept_stride = kept.stride()
     with _lib.on_device(device) as stream:
         rc = _lib.load().ekv_select_tokens(
-            scores.data_ptr(), scores.stride(0), scores.stride(1), n_slots, capacity, places, length, counts,
+            scores.data_ptr(), stride[0], stride[1], n_slots, capacity, places, length, counts,
             max(min(count, 0x7FFFFFFF), -1), min(first_tokens, capacity), min(recent_tokens, capacity), rows, heads,
-            kept.data_ptr(), kept.stride(0), kept.stride(1), new, word, stream,
+            kept.data_ptr(), kept_stride[0], kept_stride[1], new, word, stream,
         )
     _lib.check(rc, "ekv_select_tokens")
     return kept, new_lens
@@ -102,16 +103,17 @@ def compact_tokens(
     if device.type != "cuda":
         raise ValueError("the cache is compacted on the device: it must be a CUDA tensor")
     blocks, _, block_size, heads, dim = kv_cache.shape
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != device or (table.shape[1] > 1 and table.stride(1) != 1):
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.device != device or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"the block table must be an int32 [rows, width] tensor on {device} with contiguous rows")
     rows, width = table.shape
     length = _index("lens", lens, rows, device)
     new = _index("new_lens", new_lens, rows, device)
     places = _index("slots", slots, rows, device)
-    if kept.dtype != torch.int32 or kept.dim() != 3 or kept.shape[:2] != (rows, heads) or kept.device != device or kept.stride(2) != 1:
+    if kept.dtype is not torch.int32 or kept.dim() != 3 or kept.shape[:2] != (rows, heads) or kept.device != device or kept.stride(2) != 1:
         raise ValueError(f"kept must be an int32 [{rows}, {heads}, tokens] tensor on {device}")
+    score_stride = (0, 0)
     if scores is not None:
-        check_scores(scores, heads, width * block_size, device)
+        score_stride = check_scores(scores, heads, width * block_size, device)
         if slots is None and scores.shape[0] < rows:
             raise ValueError(f"{scores.shape[0]} score slots for {rows} rows")
     elif slots is not None:
@@ -124,14 +126,15 @@ def compact_tokens(
     lib = _lib.load()
     size = lib.ekv_compact_tokens_workspace_bytes(rows, heads, blocks)
     item = kv_cache.element_size()
+    s_block, s_part, s_pos, s_head, _ = kv_cache.stride()
+    kept_stride = kept.stride()
     with _lib.on_device(device) as stream:
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = kv_cache.new_empty(size, dtype=torch.uint8)
         rc = lib.ekv_compact_tokens(
-            kv_cache.data_ptr(), kv_cache.stride(0) * item, kv_cache.stride(1) * item, kv_cache.stride(2) * item,
-            kv_cache.stride(3) * item, blocks, dim * item, table.data_ptr(), table.stride(0), length, rows, width, heads,
-            block_size, kept.data_ptr(), kept.stride(0), kept.stride(1), kept.shape[2], new,
-            min(first_tokens, width * block_size), _lib.ptr(scores), scores.stride(0) if scores is not None else 0,
-            scores.stride(1) if scores is not None else 0, scores.shape[0] if scores is not None else 0, places,
+            kv_cache.data_ptr(), s_block * item, s_part * item, s_pos * item, s_head * item, blocks, dim * item,
+            table.data_ptr(), table.stride(0), length, rows, width, heads, block_size, kept.data_ptr(), kept_stride[0],
+            kept_stride[1], kept.shape[2], new, min(first_tokens, width * block_size), _lib.ptr(scores),
+            score_stride[0], score_stride[1], len(scores) if scores is not None else 0, places,
             workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_compact_tokens")
