@@ -551,7 +551,7 @@ size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_t pool_bloc
  * list, ascending strictly, below lens[r]); what lies behind new_lens[r] stays as it was. The lists keep the first
  * first_tokens positions in place, so blocks wholly among them may be shared between rows; every other block a
  * moving row holds must be its own. A row whose lists, blocks or slot break this is left as it was, with
- * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. One memset and two kernels, no host synchronisation.
+ * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. Two kernels, with a memset before them for tables of more than 512 entries; no host synchronisation.
  */
 int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
                        int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,

@@ -82,6 +82,20 @@ __device__ __forceinline__ uint32_t query_at(int r, int c) {
   return (uint32_t)r * (2 * D) + (uint32_t)((c & ~7) | ((c & 7) ^ (r & 7))) * 16;
 }
 
+// The output of an item with no tokens: its query rows saw nothing.
+template <typename T, int D>
+__device__ __noinline__ void empty_item(const AttendParams& p, int unit, int number, int MT) {
+  const Unit un = unit_at<false>(p, unit, false);
+  const int mts = un.m_tiles(p, MT), head = number / mts, m0 = (number - head * mts) * MT;
+  for (int i = threadIdx.x; i < MT * (D / 2); i += kThreads) {
+    const int mrow = m0 + i / (D / 2), c = i % (D / 2);
+    if (mrow >= un.q.nq * p.G) break;
+    const int64_t token = un.q.q0 + mrow / p.G, qhead = head * p.G + mrow % p.G;
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + token * p.out_s0 + qhead * p.out_s1 + 2 * c) = 0u;
+    if (c == 0 && p.lse != nullptr) p.lse[token * p.q_heads + qhead] = -INFINITY;
+  }
+}
+
 template <typename T, int D, int WM, int WN, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ AttendParams p) {
   using R = Ring<D>;
@@ -113,6 +127,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   chain_release();
   if (begin >= end) {
     if (p.follows) chain_wait();
+    if (!PREFIX && p.item_each && dealt.unit >= 0) empty_item<T, D>(p, dealt.unit, dealt.base, MT);
     return;
   }
   const int per_tile = kTile >> p.block_shift;  // blocks of a tile
@@ -809,7 +824,7 @@ int launch_attend(const AttendParams& p, int device, int sms, int* ctas, cudaStr
   int resident = 0;
   const int rc = prepare_launch(cache, kernel, "attend_kernel", device, kThreads, smem, &resident);
   if (rc != EKV_OK) return rc;
-  *ctas = min(sms * resident, p.max_ctas);
+  *ctas = p.item_each ? p.item_each : min(sms * resident, p.max_ctas);
   launch_chained(kernel, dim3(*ctas), dim3(kThreads), smem, s, p);
   return check_launch("attend_kernel");
 }
@@ -823,10 +838,20 @@ int launch_phase(const AttendParams& p, int device, int sms, int* ctas, cudaStre
   }
 }
 
+// The CTAs of a launch that gives each item one, or 0 where the tiles are dealt evenly. Rows of at most 512 tokens in at
+// most one item an SM: splitting their tiles over CTAs saves as much of the kernel as the launch that joins them takes (one
+// row of 333 tokens: 10.4 us whole, 10.0 us split), and that launch costs the host 2.5 us more.
+int whole_items(const AttendParams& p, int mt, int sms) {
+  const int64_t items = ((int64_t)p.rows + (int64_t)p.tokens * p.G / mt) * p.heads;  // at most
+  return p.groups == 0 && mt != kWideRows && (int64_t)p.width * p.block_size <= 8 * kTile && p.rows <= kThreads && items <= sms
+             ? (int)items : 0;
+}
+
 template <typename T, int D>
 int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, int device, int sms, cudaStream_t s) {
   CombineParams c{};
   const int phases = p.groups > 0 ? 2 : 1;
+  p.item_each = whole_items(p, mt[0], sms);
   const int type = std::is_same<T, __half>::value ? EKV_DTYPE_F16 : EKV_DTYPE_BF16;
   if (p.groups > 0) {
     p.row_info = reinterpret_cast<int4*>(ws + w.row_info);
@@ -854,6 +879,7 @@ int attend(AttendParams p, const Workspace& w, const int (&mt)[2], uint8_t* ws, 
                             : launch_phase<T, D, false>(p, device, sms, ctas, s);
     if (rc != EKV_OK) return rc;
   }
+  if (p.item_each) return EKV_OK;
   c.p = p;
   // warps for a row's average of query rows, several rows each where there are many: an M tile's list is made once for them
   const int64_t average = std::max<int64_t>(1, (int64_t)p.tokens * p.G / p.rows);

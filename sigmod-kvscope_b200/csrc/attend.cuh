@@ -60,6 +60,7 @@ struct AttendParams {
   float* whole;   // [tokens * q_heads][D] and [tokens * q_heads][2]: finished items when another phase joins (twice that
                   // in a wide launch, whose items of few query rows end in two halves)
   int follows;    // the launch before this one is the same call's prefix launch
+  int item_each;  // a CTA an item, however long: nothing is left in parts, and no launch joins them
   int mt_rows;    // query rows of an M tile
   int max_ctas;
 };
@@ -147,11 +148,37 @@ struct Deal {
 };
 
 // With every thread of the CTA (THREADS of them); scratch holds THREADS / 32 + 1 ints, found 2. Without groups CTA 0 also
-// leaves the running counts for the combine kernel.
+// leaves the running counts for the combine kernel. With item_each, CTA c's tiles are all of item c's, and base is 0; an
+// item without a tile has begin == end and its number in unit and base.
 template <bool PREFIX, int THREADS, int TOKENS = kTile>
 __device__ __forceinline__ Deal deal(const AttendParams& p, int units, int MT, int* scratch, int* found) {
   Deal d;
   const bool report = blockIdx.x == 0;
+  if (!PREFIX && p.item_each) {  // at most THREADS units
+    const int u = threadIdx.x;
+    int items = 0, tiles = 0, total = 0;
+    if (u < units) {
+      const Unit un = unit_at<false>(p, u, report);
+      items = p.heads * un.m_tiles(p, MT);
+      tiles = un.template tiles<TOKENS>();
+    }
+    const int first = block_exclusive_scan<THREADS>(items, scratch, &total), c = blockIdx.x;
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    if (first <= c && c < first + items) {
+      found[0] = u;
+      found[1] = c - first;
+      scratch[0] = tiles;
+    }
+    __syncthreads();
+    d.unit = found[0];
+    const int span = d.unit < 0 ? 0 : scratch[0];
+    d.base = span > 0 ? 0 : found[1];
+    d.begin = span > 0 ? found[1] * span : 0;
+    d.end = d.begin + span;
+    d.W = total;
+    return d;
+  }
   int mine = 0, before = 0;  // of the last THREADS units looked at
   if (PREFIX || p.groups > 0) {
     d.W = __ldcg(p.cum + units);

@@ -254,8 +254,9 @@ struct CompactParams {
   const int32_t* slots;
   int n_slots;
   int rows, width, heads, block_size, first, row_bytes;
-  int32_t* owner;  // [pool_blocks], 0: nobody's
-  int32_t* bad;    // [rows] kRow* bits
+  int32_t* owner;  // [pool_blocks], 0: nobody's; NULL: few blocks, compared with one another
+  int32_t* bad;    // [rows] kRow* bits that rows find in each other, with an owner table
+  int32_t* flags;  // [rows][heads] kRow* bits
   int32_t* hole;   // [rows][heads] the first position that takes another's token
   uint32_t* status;
 };
@@ -271,28 +272,59 @@ __device__ __forceinline__ bool row_moves(const CompactParams& p, int row, int& 
   return m >= 0 && m < n;
 }
 
+// Tables of up to this many entries have each moving row's blocks compared with every entry instead: no owner table to
+// clear, which is a launch less (four rows of 44 blocks: see ekv_compact_tokens).
+constexpr int kFewBlocks = 512;
+
+// The blocks [from, to) of a row that must be its own: all that it holds, but for those a moving row's protected tokens fill.
+__device__ __forceinline__ void own_blocks(const CompactParams& p, int row, int& from, int& to) {
+  int n, m;
+  from = row_moves(p, row, n, m) ? p.first / p.block_size : 0;
+  to = (n + p.block_size - 1) / p.block_size;
+}
+
 __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_constant__ CompactParams p) {
-  __shared__ int s_hole;
+  __shared__ int s_hole, s_flags;
+  __shared__ int s_ids[kFewBlocks];
   chain_release();
   chain_wait();
   const int row = blockIdx.x / p.heads, head = blockIdx.x - row * p.heads;
   int n, m;
   const bool moves = row_moves(p, row, n, m);
+  if (threadIdx.x == 0) {
+    s_hole = m;
+    s_flags = 0;
+  }
+  __syncthreads();
   if (head == 0) {
     const int64_t most = (int64_t)p.width * p.block_size;
     if (threadIdx.x == 0 && p.lens[row] > most) set_status(p.status, EKV_STATUS_LEN_OVER_WIDTH);
-    const int blocks = (n + p.block_size - 1) / p.block_size;
+    const int blocks = (n + p.block_size - 1) / p.block_size, own = moves ? p.first / p.block_size : 0;
     for (int b = threadIdx.x; b < blocks; b += kCheckThreads) {
       const int id = p.table[(int64_t)row * p.table_s0 + b];
-      if (id < 0 || id >= p.pool_blocks) {
-        if (moves) atomicOr(&p.bad[row], kRowBlock);
-        continue;
+      const bool bad = id < 0 || id >= p.pool_blocks;
+      if (bad && moves) atomicOr(&s_flags, kRowBlock);
+      if (p.owner == nullptr) {
+        s_ids[b] = id;
+      } else if (!bad && b >= own) {
+        const int other = atomicCAS(&p.owner[id], 0, row + 1);
+        if (other != 0) {  // claimed before, by another row or by this one
+          atomicOr(&p.bad[row], kRowShared);
+          atomicOr(&p.bad[other - 1], kRowShared);
+        }
       }
-      if (moves && b < p.first / p.block_size) continue;  // protected: read and written by nobody
-      const int other = atomicCAS(&p.owner[id], 0, row + 1);
-      if (other != 0) {  // claimed before, by another row or by this one
-        atomicOr(&p.bad[row], kRowShared);
-        atomicOr(&p.bad[other - 1], kRowShared);
+    }
+    if (p.owner == nullptr && moves) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.rows * p.width; i += kCheckThreads) {
+        const int r = i / p.width, b = i - r * p.width;
+        int from, to;
+        own_blocks(p, r, from, to);
+        if (b < from || b >= to) continue;
+        const int id = p.table[(int64_t)r * p.table_s0 + b];
+        bool shared = false;
+        for (int mine = own; mine < blocks; ++mine) shared |= s_ids[mine] == id && (r != row || mine != b);
+        if (shared) atomicOr(&s_flags, kRowShared);
       }
     }
     if (moves && p.scores != nullptr) {
@@ -300,12 +332,10 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
       bool bad = slot >= p.n_slots;
       if (slot >= 0 && p.slots != nullptr)
         for (int i = threadIdx.x; i < p.rows; i += kCheckThreads) bad |= i != row && p.slots[i] == slot;
-      if (bad) atomicOr(&p.bad[row], kRowSlot);
+      if (bad) atomicOr(&s_flags, kRowSlot);
     }
   }
   if (!moves) return;
-  if (threadIdx.x == 0) s_hole = m;
-  __syncthreads();
   const int32_t* list = p.kept + (int64_t)row * p.k0 + (int64_t)head * p.k1;
   bool ok = m <= p.columns;
   if (ok) {
@@ -315,9 +345,12 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
       if (v != j) atomicMin(&s_hole, j);
     }
   }
-  if (!ok) atomicOr(&p.bad[row], kRowList);
+  if (!ok) atomicOr(&s_flags, kRowList);
   __syncthreads();
-  if (threadIdx.x == 0) p.hole[row * p.heads + head] = s_hole;
+  if (threadIdx.x == 0) {
+    p.hole[row * p.heads + head] = s_hole;
+    p.flags[row * p.heads + head] = s_flags;
+  }
 }
 
 constexpr int kMoveThreads = 256;
@@ -338,7 +371,9 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n, m;
   if (!row_moves(p, row, n, m)) return;  // as every CTA of the cluster does
-  const int bad = p.bad[row];
+  int bad = 0;  // a row is moved whole or not at all
+  for (int h = lane; h < p.heads; h += 32) bad |= p.flags[row * p.heads + h];
+  bad = __reduce_or_sync(kFullMask, bad) | (p.owner != nullptr ? p.bad[row] : 0);
   if (bad) {
     if (threadIdx.x == 0 && rank == 0 && head == 0 && only == 0)
       set_status(p.status, (bad & kRowShared ? EKV_STATUS_BLOCK_SHARED : 0u) | (bad & kRowList ? EKV_STATUS_BAD_LIST : 0u) |
@@ -432,14 +467,15 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_cons
 }
 
 struct CompactLayout {
-  size_t owner, bad, hole, total;
+  size_t owner, bad, flags, hole, total;
 };
 
 CompactLayout compact_layout(int rows, int heads, int64_t pool_blocks) {
   CompactLayout w{};
   w.owner = 0;
   w.bad = (size_t)pool_blocks * 4;
-  w.hole = w.bad + (size_t)rows * 4;
+  w.flags = w.bad + (size_t)rows * 4;
+  w.hole = w.flags + (size_t)rows * heads * 4;
   w.total = round_up(w.hole + (size_t)rows * heads * 4, 256);
   return w;
 }
@@ -522,12 +558,13 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(ws, 0, w.hole, s) != cudaSuccess) return check_launch("cudaMemsetAsync(block owners)");
+  const bool few = (int64_t)rows * width <= kFewBlocks;
+  if (!few && cudaMemsetAsync(ws, 0, w.flags, s) != cudaSuccess) return check_launch("cudaMemsetAsync(block owners)");
   const CompactParams p{static_cast<uint8_t*>(kv), kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, pool_blocks,
                         table, table_stride, lens, kept, kept_stride_row, kept_stride_head, columns, new_lens, scores,
                         score_stride_slot, score_stride_head, slots, n_slots, rows, width, heads, block_size, first_tokens,
-                        head_bytes, reinterpret_cast<int32_t*>(ws + w.owner), reinterpret_cast<int32_t*>(ws + w.bad),
-                        reinterpret_cast<int32_t*>(ws + w.hole), status};
+                        head_bytes, few ? nullptr : reinterpret_cast<int32_t*>(ws + w.owner), reinterpret_cast<int32_t*>(ws + w.bad),
+                        reinterpret_cast<int32_t*>(ws + w.flags), reinterpret_cast<int32_t*>(ws + w.hole), status};
   launch_chained(check_kernel, dim3(rows * heads), dim3(kCheckThreads), 0, s, p);
   int rc = check_launch("check_kernel");
   if (rc != EKV_OK) return rc;

@@ -16,11 +16,23 @@ the score by which ``eviction`` decides which tokens of a bounded cache to keep.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
 
 _DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(*sizes: int) -> int:
+    return _lib.load().ekv_attend_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _scored_workspace(*sizes: int) -> int:
+    return _lib.load().ekv_attend_scored_workspace_bytes(*sizes)
 
 
 def _index(name: str, t: torch.Tensor | None, size: int, device: torch.device) -> int | None:
@@ -138,7 +150,7 @@ def attend(
         return out, lse
     out_stride = out.stride()
     lib = _lib.load()
-    size = lib.ekv_attend_workspace_bytes(rows, tokens, groups, q_heads, kv_heads, dim)
+    size = _workspace(rows, tokens, groups, q_heads, kv_heads, dim)
     with _lib.on_device(device) as stream:
         workspace = query.new_empty(size, dtype=torch.uint8)
         rc = lib.ekv_attend(
@@ -209,7 +221,7 @@ def attend_scored(
         return out, lse
     out_stride = out.stride()
     lib = _lib.load()
-    size = lib.ekv_attend_scored_workspace_bytes(rows, tokens, width, block_size, q_heads, kv_heads, dim)
+    size = _scored_workspace(rows, tokens, width, block_size, q_heads, kv_heads, dim)
     with _lib.on_device(device) as stream:
         workspace = query.new_empty(size, dtype=torch.uint8)
         rc = lib.ekv_attend_scored(

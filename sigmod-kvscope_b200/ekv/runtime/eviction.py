@@ -9,10 +9,17 @@ then the engine's to reuse. Keys carry their rotation when they are cached, so a
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
 from .attention import _index, _status, check_scores
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(*sizes: int) -> int:
+    return _lib.load().ekv_compact_tokens_workspace_bytes(*sizes)
 
 
 def select_tokens(
@@ -124,7 +131,7 @@ def compact_tokens(
     if rows == 0:
         return
     lib = _lib.load()
-    size = lib.ekv_compact_tokens_workspace_bytes(rows, heads, blocks)
+    size = _workspace(rows, heads, blocks)
     item = kv_cache.element_size()
     s_block, s_part, s_pos, s_head, _ = kv_cache.stride()
     kept_stride = kept.stride()

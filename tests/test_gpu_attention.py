@@ -67,6 +67,17 @@ def test_decode_rows_of_every_length(cuda_lib, dtype, dim, block):
     check(got, x, 1 / math.sqrt(dim), dtype, start=False)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_short_rows_with_and_without_a_wide_table(cuda_lib, wide):
+    """Rows of at most 512 tokens in few items get a CTA each; a table that could hold longer ones has their tiles dealt."""
+    from ekv.runtime.attention import attend
+
+    x = make(33, [333, 0, 512, 1, 64], queries=[1, 3, 2, 0, 9], width=33 if wide else 32)
+    d = on_device(x)
+    out, lse = torch.full_like(d["query"], 7.0), torch.full(tuple(d["query"].shape[:2]), 7.0, device="cuda")
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], out=out, lse=lse), x, 0.1, torch.bfloat16)
+
+
 @pytest.mark.parametrize("q_heads, kv_heads", [(2, 2), (10, 2), (16, 1), (32, 1), (12, 3), (48, 1)])
 def test_head_groups(cuda_lib, q_heads, kv_heads):
     from ekv.runtime.attention import attend
@@ -293,7 +304,6 @@ def test_strided_tensors_and_a_wider_table(cuda_lib):
 
     x = make(12, [90, 33], q_heads=4, kv_heads=2)
     d = on_device(x)
-    want = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1)
     q = torch.zeros(2, 6, 256, dtype=torch.bfloat16, device="cuda")[:, 1:5, 128:]
     q.copy_(d["query"])
     blocks, _, block, heads, dim = d["cache"].shape
@@ -303,6 +313,8 @@ def test_strided_tensors_and_a_wider_table(cuda_lib):
     table[:, : d["table"].shape[1]] = d["table"]
     out = torch.zeros(2, 4, 256, dtype=torch.bfloat16, device="cuda")[:, :, :128]
     got = attend(q, cache, table, d["lens"], 0.1, out=out)
+    want = attend(d["query"], d["cache"], table.contiguous(), d["lens"], 0.1)
+    check(got, x, 0.1, torch.bfloat16, start=False)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 

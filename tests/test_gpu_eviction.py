@@ -132,10 +132,15 @@ def test_compact_one_token_fewer(cuda_lib):
 
 
 def refused(status_name, cache, table, lens, kept, new, first=0, scores=None, slots=None, moved=()):
-    """The status, and that every row but those in `moved` is left as it was."""
+    """The status, and that every row but those in `moved` is left as it was: with a small table, and with one so wide that its
+    blocks are not compared with one another."""
     import ekv._lib as L
     from ekv.runtime.eviction import compact_tokens
 
+    if table.shape[1] < 300 and scores is None:
+        wide = torch.full((len(table), 300), -1, dtype=torch.int32)
+        wide[:, : table.shape[1]] = table
+        refused(status_name, cache, wide, lens, kept, new, first, moved=moved)
     got = cache.cuda()
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     extra = {} if scores is None else dict(scores=scores, slots=slots)
