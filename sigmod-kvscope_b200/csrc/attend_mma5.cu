@@ -432,14 +432,19 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       if (sh.of(w) > 0) {
         // the warp's 32 query rows into the subtile's swizzled rows, D / 8 lanes a row
         const int64_t mine = real ? (int64_t)token * p.q_s0 + (int64_t)qhead * p.q_s1 : -1;
+        uint4 v[D / 8];
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-          const int r = i * (256 / D) + lane / (D / 8), c = lane % (D / 8), at = (warp & 3) * 32 + r;
-          const int64_t source = __shfl_sync(kFullMask, mine, r);
-          const uint4 v = source >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + source + 8 * c) : make_uint4(0, 0, 0, 0);
+          const int64_t source = __shfl_sync(kFullMask, mine, i * (256 / D) + lane / (D / 8));
+          v[i] = source >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + source + 8 * (lane % (D / 8)))
+                             : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const int c = lane % (D / 8), at = (warp & 3) * 32 + i * (256 / D) + lane / (D / 8);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(queries) + w * R::kSlot + (c >> 3) * R::kHalf +
                                                                        at * 128 + (((c & 7) ^ (at & 7)) << 4)),
-                       "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                       "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
                        : "memory");
         }
         proxy_fence_smem();

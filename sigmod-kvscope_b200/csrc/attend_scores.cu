@@ -245,18 +245,26 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
       for (int m0 = 0; m0 < M; m0 += kColumns) {
         const int count = min(M - m0, kColumns), padded = (count + 15) / 16 * 16;
         named_barrier(1, 256);  // every product with the queries before is complete, and every read of their sums
-        if (column < padded) {
-          const int m = m0 + column, i = m / p.G, qhead = it.head * p.G + m - i * p.G;
-          const bool real = column < count;
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(uq.q0 + i) * p.q_s0 + (int64_t)qhead * p.q_s1);
-          const uint32_t at = smem_u32(queries) + column * 128;
+        const int m = m0 + column, i = m / p.G, qhead = it.head * p.G + m - i * p.G;
+        const bool real = column < count;
+        const int64_t mine = real ? (int64_t)(uq.q0 + i) * p.q_s0 + (int64_t)qhead * p.q_s1 : -1;
+        uint4 v[D / 8];
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 v = real ? src[c] : make_uint4(0, 0, 0, 0);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (c >> 3) * R::kQueryHalf + (((c & 7) ^ (column & 7)) << 4)),
-                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+        for (int k = 0; k < D / 8; ++k) {  // the warp's 32 query rows, D / 8 lanes a row
+          const int64_t source = __shfl_sync(kFullMask, mine, k * (256 / D) + lane / (D / 8));
+          v[k] = source >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + source + 8 * (lane % (D / 8)))
+                             : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const int c = lane % (D / 8), at = warp * 32 + k * (256 / D) + lane / (D / 8);
+          if (at < padded)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(queries) + (c >> 3) * R::kQueryHalf + at * 128 +
+                                                                         (((c & 7) ^ (at & 7)) << 4)),
+                         "r"(v[k].x), "r"(v[k].y), "r"(v[k].z), "r"(v[k].w)
                          : "memory");
-          }
+        }
+        if (column < padded) {
           const float lse = real ? p.lse[(int64_t)(uq.q0 + i) * p.q_heads + qhead] : -INFINITY;
           tail.lse[column] = lse == -INFINITY ? INFINITY : lse * kLog2e;  // no weight from a query that saw nothing
           tail.limit[column] = real ? to - uq.nq + i + 1 : 0;

@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_cons
       const int64_t at = piece(s, token);
       const int64_t source = __shfl_sync(kFullMask, a.source, token & 31);
       const int to = __shfl_sync(kFullMask, a.to, token & 31);
-      if (token < tw && to >= 0) v[s] = *reinterpret_cast<const uint4*>(heads_at + source + at);
+      if (token < tw && to >= 0) v[s] = __ldcg(reinterpret_cast<const uint4*>(heads_at + source + at));
     }
     if (scores != nullptr && a.to >= 0) score = scores[a.from];
   };
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_cons
       const int64_t at = piece(s, token);
       const int64_t target = __shfl_sync(kFullMask, a.target, token & 31);
       const int to = __shfl_sync(kFullMask, a.to, token & 31);
-      if (token < tw && to >= 0) *reinterpret_cast<uint4*>(heads_at + target + at) = v[s];
+      if (token < tw && to >= 0) __stcg(reinterpret_cast<uint4*>(heads_at + target + at), v[s]);
     }
     if (scores != nullptr && a.to >= 0) scores[a.to] = score;
   };
