@@ -1068,9 +1068,9 @@ extern "C" int ekv_attend_scored(const void* q, int64_t q_stride_token, int64_t 
                                  size_t workspace_bytes, uint32_t* status, void* stream) {
   clear_error();
   if (!scores || !lse) return fail(EKV_EINVAL, "a required device pointer is NULL");
-  if (n_slots <= 0 || score_stride_slot < 0 || score_stride_head < (int64_t)width * block_size ||
-      (n_slots > 1 && score_stride_slot < score_stride_head))
-    return fail(EKV_EINVAL, "scores must hold a slot's heads of at least width * block_size tokens each");
+  const int64_t most = (int64_t)width * block_size;
+  if (n_slots <= 0 || (kv_heads > 1 && score_stride_head < most) || (n_slots > 1 && score_stride_slot < most))
+    return fail(EKV_EINVAL, "scores must hold at least width * block_size tokens for every slot and head");
   if (!slots && n_slots < rows) return fail(EKV_EINVAL, "%d score slots for %d rows", n_slots, rows);
   if (!(decay >= 0.f && decay <= 1.f)) return fail(EKV_EINVAL, "the decay must lie in [0, 1]");
   AttendCall c{};

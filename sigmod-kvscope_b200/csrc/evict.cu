@@ -497,9 +497,9 @@ extern "C" int ekv_select_tokens(const float* scores, int64_t score_stride_slot,
     return fail(EKV_EINVAL, "rows, heads, capacity and slots must be positive");
   if (!slots && n_slots < rows) return fail(EKV_EINVAL, "%d score slots for %d rows", n_slots, rows);
   if (first_tokens < 0 || recent_tokens < 0) return fail(EKV_EINVAL, "first_tokens and recent_tokens must not be negative");
-  if (score_stride_head < capacity || score_stride_slot < 0 || (n_slots > 1 && score_stride_slot < score_stride_head))
+  if ((heads > 1 && score_stride_head < capacity) || (n_slots > 1 && score_stride_slot < capacity))
     return fail(EKV_EINVAL, "a score stride is below the capacity");
-  if (kept_stride_head < capacity || kept_stride_row < kept_stride_head)
+  if ((heads > 1 && kept_stride_head < capacity) || (rows > 1 && kept_stride_row < capacity))
     return fail(EKV_EINVAL, "a stride of the kept lists is below the capacity");
   if ((int64_t)rows * heads > 0x7fffffffll / 8 || capacity > 0x7fffffff - 4096)
     return fail(EKV_ENOTSUP, "more than 2^31 - 1 rows x heads, or tokens of a row");
@@ -543,15 +543,15 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
   if (((uintptr_t)kv & 15) || (kv_stride_block & 15) || (kv_stride_part & 15) || (kv_stride_pos & 15) || (kv_stride_head & 15))
     return fail(EKV_EINVAL, "the cache must be 16-byte aligned with strides of whole 16-byte units");
   if (table_stride < width) return fail(EKV_EINVAL, "the table's row stride is below the width");
-  if (kept_stride_head < columns || kept_stride_row < 0) return fail(EKV_EINVAL, "a stride of the kept lists is below their length");
+  if ((heads > 1 && kept_stride_head < columns) || (rows > 1 && kept_stride_row < columns)) return fail(EKV_EINVAL, "a stride of the kept lists is below their length");
   if (first_tokens < 0) return fail(EKV_EINVAL, "first_tokens must not be negative");
   if (pool_blocks > 0x7fffffffll || (int64_t)width * block_size > 0x7fffffffll - 65536 || (int64_t)rows * heads > 0x7fffffffll / 16)
     return fail(EKV_ENOTSUP, "more than 2^31 - 1 blocks, tokens of a row, or rows x heads");
   if (scores) {
     if (n_slots <= 0 || (!slots && n_slots < rows)) return fail(EKV_EINVAL, "%d score slots for %d rows", n_slots, rows);
-    if (score_stride_head < (int64_t)width * block_size || score_stride_slot < 0 ||
-        (n_slots > 1 && score_stride_slot < score_stride_head))
-      return fail(EKV_EINVAL, "scores must hold a slot's heads of at least width * block_size tokens each");
+    const int64_t most = (int64_t)width * block_size;
+    if ((heads > 1 && score_stride_head < most) || (n_slots > 1 && score_stride_slot < most))
+      return fail(EKV_EINVAL, "scores must hold at least width * block_size tokens for every slot and head");
   }
   const CompactLayout w = compact_layout(rows, heads, pool_blocks);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))

@@ -204,6 +204,69 @@ def test_compact_refuses_blocks_and_slots_outside_their_tables(cuda_lib):
     refused("STATUS_BAD_SLOT", cache, table, [100, 100], kept, [50, 50], scores=scores.cuda(), slots=ints([1, 1]))
 
 
+def test_tables_with_the_heads_outermost_and_a_strided_cache(cuda_lib):
+    from ekv.runtime.eviction import compact_tokens, select_tokens
+
+    lens = [100, 333, 50]
+    cache, scores, table = batch(7, lens, heads=3)
+    slots = [2, 0, 3]
+    outer = scores.permute(1, 0, 2).contiguous().cuda().permute(1, 0, 2)
+    kept = torch.empty(3, 3, scores.shape[2] + 5, dtype=torch.int32, device="cuda").permute(1, 0, 2)[..., 2:-3]
+    got, new = select_tokens(outer, ints(lens), 40, first_tokens=1, recent_tokens=7, slots=ints(slots), kept=kept)
+    want = oat.select(scores.numpy(), np.array(lens), [40] * 3, 1, 7, slots)
+    np.testing.assert_array_equal(got.cpu().numpy(), want[0])
+    blocks, _, block, heads, dim = cache.shape
+    strided = torch.empty(blocks, heads, block, 2, dim + 8, dtype=cache.dtype, device="cuda").permute(0, 3, 2, 1, 4)[..., 8:]
+    strided.copy_(cache)
+    compact_tokens(strided, table.cuda(), ints(lens), got, new, first_tokens=1, scores=outer, slots=ints(slots))
+    moved, moved_scores = oat.compact(cache.view(torch.uint8).numpy(), scores.numpy(), table.numpy(), lens, want[0], want[1], slots)
+    np.testing.assert_array_equal(strided.contiguous().cpu().view(torch.uint8).numpy(), moved)
+    np.testing.assert_array_equal(outer.cpu().numpy(), moved_scores)
+
+
+def test_eviction_in_a_replayed_graph_and_on_another_stream(cuda_lib):
+    from ekv.runtime.eviction import compact_tokens, select_tokens
+
+    lens = [500, 64, 0, 700]
+    cache, scores, table = batch(8, lens)
+    dev_cache, dev_scores, dev_lens, tab = cache.cuda(), scores.cuda(), ints(lens), table.cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = select_tokens(dev_scores, dev_lens, 100, first_tokens=4, recent_tokens=8)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, new = select_tokens(dev_scores, dev_lens, 100, first_tokens=4, recent_tokens=8)
+        compact_tokens(dev_cache, tab, dev_lens, kept, new, first_tokens=4, scores=dev_scores)
+    for shift in (0, 37):  # the graph again, on another batch
+        now = [max(n - shift, 0) for n in lens]
+        dev_cache.copy_(cache)
+        dev_scores.copy_(scores)
+        dev_lens.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        want = oat.select(scores.numpy(), np.array(now), [100] * 4, 4, 8, [0, 1, 2, 3])
+        np.testing.assert_array_equal(kept.cpu().numpy(), want[0])
+        if shift == 0:
+            np.testing.assert_array_equal(first[0].cpu().numpy(), want[0])
+        moved, moved_scores = oat.compact(cache.view(torch.uint8).numpy(), scores.numpy(), table.numpy(), now, want[0], want[1], [0, 1, 2, 3])
+        np.testing.assert_array_equal(dev_cache.cpu().view(torch.uint8).numpy(), moved)
+        np.testing.assert_array_equal(dev_scores.cpu().numpy(), moved_scores)
+
+
+def test_one_long_row(cuda_lib):
+    """Clusters of CTAs over one row, keys and values apart, and positions past 2^16."""
+    lens = [70001]
+    cache, scores, table = batch(9, lens, heads=1, dim=64)
+    gen = torch.Generator().manual_seed(1)
+    drop = torch.randperm(70001, generator=gen)[:9000]
+    keep = torch.ones(70001, dtype=torch.bool)
+    keep[drop] = False
+    keep[:100] = True
+    kept = torch.nonzero(keep)[:, 0].to(torch.int32).view(1, 1, -1)
+    check_compact(cache, scores, table, lens, kept, torch.tensor([kept.shape[2]], dtype=torch.int32), [1], first=100)
+
+
 def test_a_bounded_cache_over_many_steps(cuda_lib):
     """Attend, add the weights up, and at 96 tokens cut the row to 64: the cache as a serving loop uses it, against the
     same loop in float64 over lists of tokens."""
