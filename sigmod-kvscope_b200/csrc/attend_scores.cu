@@ -112,7 +112,7 @@ struct Tail {
   uint64_t full[Ring<D>::kSlots], empty[Ring<D>::kSlots], q_full, s_full[2], s_free[2], drained;
   uint32_t tmem;
   int scratch[kThreads / 32 + 1], found[2];
-  alignas(16) float lse[kColumns];
+  alignas(16) float lse[kColumns];  // minus it, in powers of two
   alignas(16) int limit[kColumns];
 };
 
@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
   } else {  // ---- the warpgroups that add ----------------------------------------------------------------------
     const int w = warp >> 2, token_lane = threadIdx.x & 127, column = threadIdx.x;  // column: the query row this thread loads
     const uint32_t s_at = tmem + w * kColumns + ((uint32_t)(warp & 3) << 21);
+    const uint64_t scale2 = pair_of(p.scale_log2, p.scale_log2);
     uint32_t s_uses = 0;
     for (int t = begin; t < end;) {
       const Item it = walk.at(p, t, end);
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
         }
         if (column < padded) {
           const float lse = real ? p.lse[(int64_t)(uq.q0 + i) * p.q_heads + qhead] : -INFINITY;
-          tail.lse[column] = lse == -INFINITY ? INFINITY : lse * kLog2e;  // no weight from a query that saw nothing
+          tail.lse[column] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;  // no weight from a query that saw nothing
           tail.limit[column] = real ? to - uq.nq + i + 1 : 0;
         }
         proxy_fence_smem();
@@ -282,33 +283,44 @@ __global__ void __launch_bounds__(kThreads, 1) weigh_kernel(const __grid_constan
           __syncwarp();
           const int pos = tile * kTokens + token_lane;
           const bool inner = (tile + 1) * kTokens <= to - uq.nq + 1;  // every query token sees the whole tile
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int c = 0; c < count; c += 32) {
-            float s[32];
-            tmem_ld32(s, s_at + c);
-            tmem_wait_ld(s);
-            const float4* lse = reinterpret_cast<const float4*>(tail.lse + c);
-            if (inner && c + 32 <= count) {
+          uint64_t sums[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+          float sum = 0.f;
+          float s[2][32];
+          tmem_ld32(s[0], s_at);
+          // 64 columns in turn through the two buffers: one chunk is on its way while the other is worked on
+          for (int c0 = 0; c0 < count; c0 += 64) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float4 v = lse[k];
-                sum[0] += exp2_fast(fmaf(s[4 * k], p.scale_log2, -v.x));
-                sum[1] += exp2_fast(fmaf(s[4 * k + 1], p.scale_log2, -v.y));
-                sum[2] += exp2_fast(fmaf(s[4 * k + 2], p.scale_log2, -v.z));
-                sum[3] += exp2_fast(fmaf(s[4 * k + 3], p.scale_log2, -v.w));
-              }
-            } else {
+            for (int half = 0; half < 2; ++half) {
+              const int c = c0 + 32 * half;
+              if (c >= count) break;
+              tmem_wait_ld(s[half]);
+              if (c + 32 < count) tmem_ld32(s[half ^ 1], s_at + c + 32);
+              if (inner && c + 32 <= count) {
+                const float4* lse = reinterpret_cast<const float4*>(tail.lse + c);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const int at = min(c + k, kColumns - 1);
-                const float v = exp2_fast(fmaf(s[k], p.scale_log2, -tail.lse[at]));
-                if (c + k < count && pos < tail.limit[at]) sum[k & 3] += v;
+                for (int k = 0; k < 8; ++k) {
+                  const float4 v = lse[k];  // minus the log-sum-exps
+                  float a, b, d, e;
+                  split(fma_pair(pair_of(s[half][4 * k], s[half][4 * k + 1]), scale2, pair_of(v.x, v.y)), a, b);
+                  split(fma_pair(pair_of(s[half][4 * k + 2], s[half][4 * k + 3]), scale2, pair_of(v.z, v.w)), d, e);
+                  sums[0] = add_pair(sums[0], pair_of(exp2_fast(a), exp2_fast(b)));
+                  sums[1] = add_pair(sums[1], pair_of(exp2_fast(d), exp2_fast(e)));
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  const int at = min(c + k, kColumns - 1);
+                  const float v = exp2_fast(fmaf(s[half][k], p.scale_log2, tail.lse[at]));
+                  if (c + k < count && pos < tail.limit[at]) sum += v;
+                }
               }
             }
           }
           tc_fence_before();
           mbar_arrive(&tail.s_free[w]);
-          float weight = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float x, y;
+          split(add_pair(sums[0], sums[1]), x, y);
+          float weight = (x + y) + sum;
           if (missing >> (token_lane >> p.block_shift) & 1u) weight = 0.f;  // keys that were not read
           if (slot >= 0 && pos < to) {  // this thread's token in every round of query rows
             const float old = m0 > 0 ? dst[pos] : (pos >= old_end || sp.decay == 0.f ? 0.f : sp.decay * dst[pos]);

@@ -181,11 +181,19 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
     prefix |= (uint32_t)s_pick[0] << shift;
     mask |= 255u << shift;
     want = s_pick[1];
-    __syncthreads();  // before s_pick is written again
+    if (want == 0) break;  // nothing that begins like this is kept: its further digits do not matter
+    __syncthreads();       // before s_pick is written again
   }
-  // keep every key above `prefix` and the `want` oldest equal to it: counted per warp, then placed
+  if constexpr (KEYS > 0) {
+    if (mask != 0xffffffffu) {
+#pragma unroll
+      for (int k = 0; k < KEYS; ++k) keys[k] &= mask;
+    }
+  }
+  // keep every key above `prefix` (in the digits found) and the `want` oldest equal to it: counted per warp, then placed
   int sure = 0, equal = 0;
   walk([&](int, uint32_t key) {
+    if (KEYS == 0) key &= mask;
     sure += key > prefix;
     equal += key == prefix;
   });
@@ -214,14 +222,15 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const __grid_
   if (equal == 0) {  // nearly every run: no score equal to the last one kept
     int place = sure_before + min(equal_before, want);
     walk([&](int i, uint32_t key) {
-      const bool take = key > prefix;
+      const bool take = (KEYS == 0 ? key & mask : key) > prefix;
       const uint32_t takes = __ballot_sync(kFullMask, take);
       if (take) out[place + __popc(takes & below)] = i;
       place += __popc(takes);
     });
   } else {
     walk([&](int i, uint32_t key) {
-      const bool is_sure = key > prefix, is_equal = key == prefix;  // prefix is a score's key: not 0
+      if (KEYS == 0) key &= mask;
+      const bool is_sure = key > prefix, is_equal = key == prefix;  // where some are kept, `prefix` is a score's whole key: not 0
       const uint32_t sures = __ballot_sync(kFullMask, is_sure), equals = __ballot_sync(kFullMask, is_equal);
       const int tied = equal_before + __popc(equals & below);
       const int place = sure_before + __popc(sures & below) + min(tied, want);

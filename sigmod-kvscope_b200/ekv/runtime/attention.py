@@ -39,7 +39,8 @@ def _index(name: str, t: torch.Tensor | None, size: int, device: torch.device) -
     """The address of an int32 index array of at least ``size`` entries on the call's device."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.dim() != 1 or len(t) < size or t.device != device or (size > 1 and t.stride(0) != 1):
+    if (t.dtype is not torch.int32 or t.dim() != 1 or len(t) < size or t.get_device() != device.index
+            or (size > 1 and t.stride(0) != 1)):
         raise ValueError(f"{name} must be a contiguous int32 tensor of at least {size} entries on {device}")
     return t.data_ptr()
 
@@ -67,7 +68,8 @@ def _batch(query: torch.Tensor, kv_cache: torch.Tensor, table: torch.Tensor, len
     device = query.device
     if device.type != "cuda":
         raise ValueError("the attention runs on the device: the query must be a CUDA tensor")
-    if kv_cache.device != device or table.device != device or lens.device != device:
+    index = device.index
+    if kv_cache.get_device() != index or table.get_device() != index or lens.get_device() != index:
         raise ValueError(f"the cache, the block table and the lengths must be on the query's device {device}")
     return device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride[0]
 
@@ -167,7 +169,7 @@ def attend(
 def check_scores(scores: torch.Tensor, heads: int, tokens: int, device: torch.device) -> tuple:
     """The strides of a score table [slots, heads, >= tokens] float32 on ``device``, each head's scores contiguous."""
     shape, stride = scores.shape, scores.stride()
-    if scores.dtype is not torch.float32 or len(shape) != 3 or scores.device != device:
+    if scores.dtype is not torch.float32 or len(shape) != 3 or scores.get_device() != device.index:
         raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor on {device}")
     if shape[1] != heads or shape[2] < tokens:
         raise ValueError(f"scores of {heads} heads and at least {tokens} tokens are needed, got {tuple(shape)}")

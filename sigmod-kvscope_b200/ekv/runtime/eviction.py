@@ -47,9 +47,9 @@ def select_tokens(
     if scores.dim() != 3:
         raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor, got {tuple(scores.shape)}")
     n_slots, heads, capacity = scores.shape
-    stride = check_scores(scores, heads, 1, device)
-    if device.type != "cuda":
+    if device.type != "cuda" and scores.dtype is torch.float32:
         raise ValueError("the selection runs on the device: scores must be a CUDA tensor")
+    stride = check_scores(scores, heads, 1, device)
     if lens.dim() != 1:
         raise ValueError("lens must be [rows]")
     rows = lens.shape[0]
