@@ -810,10 +810,28 @@ Workspace workspace_layout(int rows, int tokens, int groups, int q_heads, int di
   return w;
 }
 
-// Query rows of an M tile: the smallest variant that holds a unit's average in one tile.
-int pick_mt(int64_t tokens, int units, int G) {
+// Query rows of an M tile: the smallest variant that holds a unit's average in one tile. Above 64 the tcgen05 kernel, whose
+// tensor cores are twice as fast and whose items cost some 10 us each to begin and end (queries in, 128 KB of sums out):
+// from 12 of its 128-token tiles an item, as far as `span`, the most tokens of a unit, tells, and 500 tiles of 256 query rows
+// and 128 dims in all. (128 query rows, 8 heads, one prefix of 8000, 16000 and 32000 tokens: 52, 47 and 58 us there, 45,
+// 58 and 86 us here; 64 rows of 1000 tokens, 256 query rows a head: 372 there, 297 here; of 4096: 502 there, 769 here.)
+int pick_mt(int64_t tokens, int units, int G, int heads, int dim, int64_t span) {
   const int64_t m = (tokens + units - 1) / units * G;
-  return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : kWideRows;
+  if (m <= 64) return m <= 16 ? 16 : m <= 32 ? 32 : 64;
+  const int64_t tiles = (span + 2 * kTile - 1) / (2 * kTile), items = (int64_t)units * heads * ((m + kWideRows - 1) / kWideRows);
+  return tiles >= 12 && items * tiles * std::min<int64_t>(m, kWideRows) * dim >= 500ll * kWideRows * 128 ? kWideRows : 64;
+}
+
+// The bytes for any `span`: where both variants may be picked, of the larger one.
+size_t workspace_bytes(int rows, int tokens, int groups, int q_heads, int kv_heads, int dim, int64_t logits) {
+  const int G = q_heads / kv_heads;
+  size_t most = 0;
+  for (int pick = 0; pick < 4; ++pick) {
+    const int mt[2] = {pick_mt(tokens, rows, G, kv_heads, dim, pick & 1 ? 0x7fffffff : 0),
+                       groups > 0 ? pick_mt(tokens, groups, G, kv_heads, dim, pick & 2 ? 0x7fffffff : 0) : 0};
+    most = std::max(most, workspace_layout(rows, tokens, groups, q_heads, dim, mt, logits).total);
+  }
+  return most;
 }
 
 template <typename T, int D, int WM, int WN, bool PREFIX>
@@ -936,7 +954,7 @@ namespace {
 int64_t logits_row(int width, int block_size) { return ((int64_t)width * block_size + kTile - 1) / kTile * kTile; }
 int64_t kept_logits(int tokens, int rows, int width, int block_size, int q_heads, int kv_heads) {
   const int64_t n = (int64_t)tokens * q_heads * logits_row(width, block_size);
-  return pick_mt(tokens, rows, q_heads / kv_heads) == 16 && n <= (1ll << 28) ? n : 0;
+  return pick_mt(tokens, rows, q_heads / kv_heads, kv_heads, 128, 0) == 16 && n <= (1ll << 28) ? n : 0;
 }
 
 struct AttendCall {
@@ -988,8 +1006,9 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
       ((int64_t)rows + (int64_t)tokens * G / 16) * kv_heads * tiles > 0x7fffffffll)
     return fail(EKV_ENOTSUP, "a launch of more than 2^31 - 1 tiles (rows x heads x tokens)");
   if ((int64_t)tokens * q_heads > 0x7fffffffll / 4) return fail(EKV_ENOTSUP, "more than 2^29 query rows");
-  c.mt[0] = pick_mt(tokens, rows, G);
-  c.mt[1] = groups > 0 ? pick_mt(tokens, groups, G) : 0;
+  const int64_t span = (int64_t)width * block_size;
+  c.mt[0] = pick_mt(tokens, rows, G, kv_heads, head_dim, span);
+  c.mt[1] = groups > 0 ? pick_mt(tokens, groups, G, kv_heads, head_dim, prefix_blocks ? span : std::min(span, (int64_t)prefix_common * block_size)) : 0;
   const int64_t logits = scored ? kept_logits(tokens, rows, width, block_size, q_heads, kv_heads) : 0;
   const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, c.mt, logits);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
@@ -1027,17 +1046,14 @@ int run(const AttendCall& c, int head_dim, int dtype, cudaStream_t s) {
 
 extern "C" size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads, int kv_heads, int head_dim) {
   if (rows <= 0 || tokens <= 0 || groups < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
-  const int G = q_heads / kv_heads;
-  const int mt[2] = {pick_mt(tokens, rows, G), groups > 0 ? pick_mt(tokens, groups, G) : 0};
-  return workspace_layout(rows, tokens, groups, q_heads, head_dim, mt, 0).total;
+  return workspace_bytes(rows, tokens, groups, q_heads, kv_heads, head_dim, 0);
 }
 
 extern "C" size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,
                                                     int head_dim) {
   if (rows <= 0 || tokens <= 0 || width <= 0 || block_size <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads)
     return 0;
-  const int mt[2] = {pick_mt(tokens, rows, q_heads / kv_heads), 0};
-  return workspace_layout(rows, tokens, 0, q_heads, head_dim, mt, kept_logits(tokens, rows, width, block_size, q_heads, kv_heads)).total;
+  return workspace_bytes(rows, tokens, 0, q_heads, kv_heads, head_dim, kept_logits(tokens, rows, width, block_size, q_heads, kv_heads));
 }
 
 extern "C" int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,

@@ -37,6 +37,13 @@ def make(seed, lens, queries=None, q_heads=8, kv_heads=2, dim=128, block=16, dty
     return dict(query=query, cache=cache, table=table, lens=torch.tensor(lens, dtype=torch.int32), start=start)
 
 
+def widen(x, tokens=1 << 16):
+    """The same rows in a table that could hold many more tokens, which is what the kernel for many query rows is picked by."""
+    block = x["cache"].shape[2]
+    more = torch.full((len(x["table"]), tokens // block - x["table"].shape[1]), -1, dtype=torch.int32)
+    return dict(x, table=torch.cat([x["table"], more], 1))
+
+
 def on_device(x):
     return {k: v.cuda() for k, v in x.items()}
 
@@ -87,11 +94,13 @@ def test_head_groups(cuda_lib, q_heads, kv_heads):
     check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.09), x, 0.09, torch.bfloat16, start=False)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("queries", [[1, 4, 2, 1], [0, 7, 0, 3], [33, 1, 20, 64], [5, 5, 5, 5]])
-def test_several_query_tokens_a_row(cuda_lib, queries):
+def test_several_query_tokens_a_row(cuda_lib, queries, wide):
     from ekv.runtime.attention import attend
 
     x = make(3, [100, 64, 33, 200], queries=queries, dtype=torch.float16)
+    x = widen(x) if wide else x
     d = on_device(x)
     got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"])
     check(got, x, 0.1, torch.float16)
@@ -119,6 +128,11 @@ def test_shared_prefixes(cuda_lib, dim, queries, groups):
     got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=prefix,
                  group_start=group_start)
     check(got, x, 0.1, torch.bfloat16)
+    wide = widen(x)
+    d = on_device(wide)
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=prefix,
+                 group_start=group_start), wide, 0.1, torch.bfloat16)
+    d = on_device(x)
     if len(groups) == 1:
         again = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=groups[0][2])
         assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
@@ -135,9 +149,11 @@ def test_prefixes_of_many_query_rows(cuda_lib, dtype, dim, block, rows, q_heads,
     for blocks in (1, 3, 1000 // block, 5000 // block):
         x = make(20 + blocks, [blocks * block + 1 + r % 37 + queries for r in range(rows)], queries=[queries] * rows, dim=dim,
                  block=block, dtype=dtype, q_heads=q_heads, groups=[(0, rows, blocks)], width=blocks + -(-50 // block))
-        d = on_device(x)
-        got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=blocks)
-        check(got, x, 0.1, dtype)
+        prefix = torch.tensor([blocks], dtype=torch.int32, device="cuda")
+        for y in (x, widen(x, 1 << 17)):
+            d = on_device(y)
+            got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=prefix)
+            check(got, y, 0.1, dtype)
 
 
 def test_wide_rows_with_gaps_and_growing_scores(cuda_lib):
@@ -156,11 +172,13 @@ def test_wide_rows_with_gaps_and_growing_scores(cuda_lib):
     ok = np.ones(tuple(x["table"].shape), dtype=bool)
     for r, b, bad in [(0, 2, -1), (0, 40, 10**9), (1, 0, x["cache"].shape[0]), (1, 30, -7)]:
         x["table"][r, b], ok[r, b] = bad, False
-    d = on_device(x)
-    status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], status=status)
-    check(got, x, 0.1, torch.float16, pool_ok=ok)
-    assert int(status) == L.STATUS_BAD_BLOCK_ID
+    for y in (x, widen(x)):
+        d = on_device(y)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], status=status)
+        more = np.ones((4, y["table"].shape[1] - ok.shape[1]), dtype=bool)
+        check(got, y, 0.1, torch.float16, pool_ok=np.concatenate([ok, more], 1))
+        assert int(status) == L.STATUS_BAD_BLOCK_ID
 
 
 # ---- weights accumulated per token -------------------------------------------------------------------
