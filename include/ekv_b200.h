@@ -1,6 +1,6 @@
 /*
  * ekv_b200.h -- C ABI of libekv_b200.so, the sm_100a implementation of KVScope's attention-share
- * audit and block-table view path.
+ * audit and block-table view path, and of the attention and token eviction over the same paged cache.
  *
  * Every entry point takes plain device pointers, element strides and sizes, and a CUDA stream given
  * as `void*` (a cudaStream_t; NULL is the legacy default stream). None allocates device memory, none
@@ -478,7 +478,8 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  *          a row (tokens == rows). Token i of a row's n sees the positions below lens[r] - n + i + 1.
  * out [tokens][q_heads][head_dim] (element strides) receives softmax(scale q K^T) V and lse (may be NULL;
  * float32 [tokens][q_heads]) the natural log of the sum of exp(scale q.k); a query token that sees nothing gets
- * 0 and -inf. Tokens of no row keep what they have.
+ * 0 and -inf. Tokens of no row keep what they have. What lies behind a row may hold anything; values at positions that one of
+ * a row's query tokens sees and another does not must be finite.
  *
  * groups > 0: the rows [group_start[g], group_start[g + 1]) (int32 [groups + 1]; NULL with groups = 1: every row)
  * share their first prefix_blocks[g] blocks (int32 [groups]; NULL with groups = 1: prefix_common blocks): their
@@ -487,7 +488,7 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  * A table entry outside [0, pool_blocks) is skipped with EKV_STATUS_BAD_BLOCK_ID, a length past the table
  * clamped with EKV_STATUS_LEN_OVER_WIDTH, a row whose query tokens are not tokens of the batch skipped with
  * EKV_STATUS_BAD_QROW. Supported: head_dim 64 and 128, block_size 8, 16, 32 and 64, rows <= 2048, scale > 0, base
- * addresses and strides in whole 16-byte units. Two kernels (three with groups), no host synchronisation.
+ * addresses and strides in whole 16-byte units. One or two kernels (four with groups), no host synchronisation.
  */
 int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,
                int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos, int64_t kv_stride_head,
@@ -507,8 +508,8 @@ int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, con
  * w = sum of exp(scale q.k - lse) over the row's query tokens and the head's query heads: its score becomes w
  * when t is among the row's newest fresh[r] tokens (int32 [rows]; NULL: its query tokens), which have none
  * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends without scoring; a
- * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Three kernels, no host
- * synchronisation.
+ * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Two or three kernels, no
+ * host synchronisation.
  */
 size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,
                                          int head_dim);

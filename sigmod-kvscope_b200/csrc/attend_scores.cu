@@ -6,13 +6,15 @@
 // order; nothing is added atomically.
 //
 // Few query rows (decode): the attention kernel has left its logits, and add_kernel reads them back, 4 bytes a token
-// and query row, mostly from L2 (64 rows of 4096 tokens, four query rows a KV head: see the figures at launch_score_kernel).
+// and query row, mostly from L2. 64 rows of up to 4096 tokens, four query rows a KV head: the pass adds 20 us to the
+// attention's 133; multiplying the keys again, as for windows, added 140.
 //
 // Many query rows (a window that scores a prompt): weigh_kernel multiplies the keys again, on the tcgen05 tensor cores with
 // the roles turned: 128 tokens are the rows of the product and up to 256 query rows its columns, so a token is a lane of
 // tensor memory, its thread reads the columns 32 at a time, takes their exponentials and adds them up in a register. Two
 // warpgroups take alternate tiles. The exponentials bound it: 16 a clock and SM, 2048 clocks for 128 x 256 against 1024
-// of the products.
+// of the products. Four prompts of up to 16001 tokens, 256 query rows a KV head: 55 us, of which the exponentials are 29
+// (992 us with mma.sync and the queries read from L1 for every tile).
 #include <algorithm>
 #include <type_traits>
 

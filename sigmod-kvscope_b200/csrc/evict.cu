@@ -8,7 +8,9 @@
 // equal to it are, and the warps write the kept positions of their runs, ascending, then -1. Scores crowd into a few exponents, so every lane counts in its
 // own column of bins, which is a bank of its own (with one histogram for all lanes, or eight, the additions of the first
 // pass waited for one another: 8 us of 8 x 8 units of 65536 tokens). The CTAs' counts are added through distributed
-// shared memory, in integers: no order matters.
+// shared memory, in integers: no order matters. The passes end early at a digit with which nothing more is kept.
+// What bounds it: 8 rows x 8 heads of 65536 tokens take 35 us (floor 5): a CTA's steps one after another -- 15000 cycles until
+// its scores are there, 5000 to 7000 a pass with its two cluster exchanges, 5000 for the lists -- at two CTAs an SM.
 //
 // compact: position j of a (row, head) takes the key, value and score of position kept[j] >= j, in place, in
 // chunks: a chunk's sources are all read before any of it is written, and later chunks only read positions past

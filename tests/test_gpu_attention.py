@@ -385,6 +385,40 @@ def test_two_streams_at_once(cuda_lib):
         assert torch.equal(out, want[k][0]) and torch.equal(lse, want[k][1])
 
 
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("wide", [False, True])
+def test_hundreds_of_rows_most_of_them_empty(cuda_lib, grouped, wide):
+    """More rows than a CTA has threads, long runs of rows with no tokens or no query, groups of every size."""
+    from ekv.runtime.attention import attend
+
+    rng = np.random.default_rng(5)
+    lens = [int(n) if rng.random() < 0.4 else 0 for n in rng.integers(1, 200, 420)]
+    lens[50:190] = [0] * 140
+    lens[300] = 1500
+    queries = [int(q) for q in rng.integers(0, 6 if wide else 3, 420)]
+    queries[200:280] = [0] * 80
+    queries[310] = 70 if wide else 1
+    edges = sorted({0, 420, 5, 6, 60, 61, 250, 251, 300, 302, *rng.integers(0, 420, 12).tolist()})
+    groups = [(a, b, min(3 + a % 7, min([-(-n // 16) for n in lens[a:b] if n] or [0]))) for a, b in zip(edges, edges[1:])]
+    x = make(40, lens, queries=queries, q_heads=64 if wide else 4, kv_heads=2, dim=64, groups=groups if grouped else None)
+    x = widen(x, 1 << 18) if wide else x
+    d = on_device(x)
+    more = {}
+    if grouped:
+        more = dict(group_start=torch.tensor(edges, dtype=torch.int32, device="cuda"),
+                    prefix_blocks=torch.tensor([b for _, _, b in groups], dtype=torch.int32, device="cuda"))
+    check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], **more), x, 0.1, torch.bfloat16)
+
+
+def test_scores_of_hundreds_of_rows(cuda_lib):
+    rng = np.random.default_rng(6)
+    lens = [int(n) if rng.random() < 0.5 else 0 for n in rng.integers(1, 150, 300)]
+    for top in (2, 60):
+        x = make(41, lens, queries=[int(q) for q in rng.integers(0, top, 300)], dim=64)
+        scores = torch.rand(300, 2, x["table"].shape[1] * 16, generator=torch.Generator().manual_seed(3))
+        run_scored(x, on_device(x), 0.1, scores, slots=rng.permutation(300).tolist(), decay=0.5)
+
+
 def test_a_row_that_is_shorter_than_its_groups_prefix(cuda_lib):
     from ekv.runtime.attention import attend
 
