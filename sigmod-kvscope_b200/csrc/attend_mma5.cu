@@ -14,12 +14,12 @@
 //     so most tiles need one pass over their scores, and the output in tensor memory is rescaled a few times a row, by the
 //     same threads; probabilities go back to tensor memory over the scores, rounded to the values' type.
 //
-// What bounds it: 256 query rows on 32768 tokens, 8 KV heads of 128, take 45 us and 1024 query rows 131-145 us (0.96 to 1.05
-// PFLOP/s, 57 to 62 % of the measured bf16 rate; the SM clock falls to 1.5 GHz under it). A tile's period is 3650 cycles, a
-// warpgroup's softmax (2150: 16 exponentials a clock and SM are 1024 of them, twice that when both warpgroups overlap) and
-// its two products with their hand-overs (1500) one after the other, where the tensor cores need 2048 for both warpgroups;
-// with the softmax left out the kernel takes 121 us. 18 us of each launch are beginnings and ends: the walk's first loads,
-// the queries, the first tile, 128 KB of sums out of every CTA.
+// What bounds it: 256 query rows on 32768 tokens, 8 KV heads of 128, take 44 us and 1024 query rows 139 us (0.99 PFLOP/s, 59 %
+// of the measured bf16 rate; the SM clock falls to 1.5 GHz under it; boxes differ by a tenth). A tile's period was 3650
+// cycles, a warpgroup's softmax (2150: 16 exponentials a clock and SM are 1024 of them, twice that when both warpgroups
+// overlap; a third of them now run on the FMA pipes) and its two products with their hand-overs (1500) one after the other,
+// where the tensor cores need 2048 for both warpgroups; with the softmax left out the kernel takes 121 us. Some 15 us of
+// each launch are beginnings and ends: the walk's first loads, the queries, the first tile, 128 KB of sums out of every CTA.
 #include <type_traits>
 
 #include "attend.cuh"
@@ -147,8 +147,12 @@ __device__ __forceinline__ void seen_softmax(const SoftmaxTile& a, float& m, flo
     for (int i = 0; i < 16; ++i) {
       float x, y;
       split(fma_pair(pair_of(s[c & 1][2 * i], s[c & 1][2 * i + 1]), scale2, from2), x, y);
-      x = exp2_fast(x);
-      y = exp2_fast(y);
+      if (i % 3 == 2) {  // 1024 query rows on 32768 tokens: 146 us with none of the pairs here, 139 with a third
+        exp2_pair(x, y);
+      } else {
+        x = exp2_fast(x);
+        y = exp2_fast(y);
+      }
       sum[i & 1] = add_pair(sum[i & 1], pair_of(x, y));
       u[i] = pack2<T>(x, y);
     }
@@ -411,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory
     const uint32_t s_at = tmem + w * 128 + lanes, o_at = tmem + 256 + w * 128 + lanes;
     uint32_t s_uses = 0, o_uses = 0;
-    const float grow = 8.f / p.scale_log2;
+    const float grow = fminf(8.f / p.scale_log2, 1e38f);  // finite: a row's first scores have to be above -inf + grow
     for (int t = begin; t < end;) {
       const Item it = walk.at(p, t, end);
       const Share sh = share_of(p, it);

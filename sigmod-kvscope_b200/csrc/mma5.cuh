@@ -101,6 +101,31 @@ __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
   return v;
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+// 2^x and 2^y, at least 2^-126, on the FMA pipes, for a part of the exponentials where the special-function units are what a
+// kernel waits for. x = n + f with n the nearest whole number (adding 1.5 2^23 leaves it in the low bits) and |f| <= 1/2; 2^f
+// by the polynomial of degree 5 through the Chebyshev nodes of [-1/2, 1/2], 2.2e-7 off at most with its float32 roundings
+// (ex2.approx: 2^-22); 2^n from its exponent bits. NaN stays NaN.
+__device__ __forceinline__ void exp2_pair(float& x, float& y) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(y));
+  const uint64_t v = pair_of(x, y), t = add_pair(v, pair_of(12582912.f, 12582912.f));
+  const uint64_t f = fma_pair(add_pair(t, pair_of(-12582912.f, -12582912.f)), pair_of(-1.f, -1.f), v);
+  uint64_t r = fma_pair(f, pair_of(1.3390863e-3f, 1.3390863e-3f), pair_of(9.676032e-3f, 9.676032e-3f));
+  r = fma_pair(r, f, pair_of(5.550357e-2f, 5.550357e-2f));
+  r = fma_pair(r, f, pair_of(2.4022107e-1f, 2.4022107e-1f));
+  r = fma_pair(r, f, pair_of(6.931472e-1f, 6.931472e-1f));
+  r = fma_pair(r, f, pair_of(1.0000001f, 1.0000001f));
+  float a, b;
+  split(t, a, b);
+  const float two_n = __int_as_float((__float_as_int(a) << 23) + 0x3f800000), two_m = __int_as_float((__float_as_int(b) << 23) + 0x3f800000);
+  split(mul_pair(r, pair_of(two_n, two_m)), x, y);
+}
 
 // The instruction's shape and types: M query or token rows of 128, N columns, float32 sums; `values_rows`: the second
 // operand's rows are the summed dimension (values), not its columns (keys).

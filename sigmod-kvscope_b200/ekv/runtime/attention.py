@@ -121,7 +121,9 @@ def attend(
     the group. An int is one group of every row, as an engine's common prefix length gives it.
 
     What lies behind a row may hold anything; values at positions that one of a row's query tokens sees and another does
-    not must be finite. Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a
+    not must be finite.
+
+    Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a
     token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
     in the tables, which the kernels skip. The call runs on the current stream of the query's device.
     """

@@ -106,6 +106,16 @@ def test_several_query_tokens_a_row(cuda_lib, queries, wide):
     check(got, x, 0.1, torch.float16)
 
 
+@pytest.mark.parametrize("scale", [1e-38, 1e-4, 1.0])
+def test_scales(cuda_lib, scale):
+    from ekv.runtime.attention import attend
+
+    x = make(42, [150, 700, 20], queries=[30, 1, 25], q_heads=16)
+    for y in (x, widen(x)):
+        d = on_device(y)
+        check(attend(d["query"], d["cache"], d["table"], d["lens"], scale, query_start=d["start"]), y, scale, torch.bfloat16)
+
+
 def test_more_query_tokens_than_cached_ones(cuda_lib):
     from ekv.runtime.attention import attend
 
@@ -315,6 +325,23 @@ def test_values_behind_a_row_may_be_anything(cuda_lib):
             x["cache"][x["table"][r, n // 16], 1, 15] = float("inf")
     d = on_device(x)
     check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1), x, 0.1, torch.float16, start=False)
+
+
+def test_keys_that_are_not_numbers_reach_the_output(cuda_lib):
+    """A NaN key that a query token sees makes its output NaN, wherever in a tile it stands; other rows keep theirs."""
+    from ekv.runtime.attention import attend, attend_scored
+
+    for at in (3, 20, 37, 64, 101, 126, 127, 200):
+        x = make(43, [400, 130, 300], queries=[40, 30, 20], q_heads=16, dim=64)
+        x["cache"][x["table"][0, at // 16], 0, at % 16, 1] = float("nan")
+        for y in (x, widen(x)):
+            d = on_device(y)
+            out, lse = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"])
+            assert torch.all(torch.isnan(out[:40, 8:])) and torch.all(torch.isnan(lse[:40, 8:]))
+            assert not torch.any(torch.isnan(out[:40, :8])) and not torch.any(torch.isnan(out[40:]))
+        scores = torch.zeros(3, 2, y["table"].shape[1] * 16, device="cuda")
+        attend_scored(d["query"], d["cache"], d["table"], d["lens"], 0.1, scores, query_start=d["start"])
+        assert torch.all(torch.isnan(scores[0, 1, :360])) and not torch.any(torch.isnan(scores[1:])) and not torch.any(torch.isnan(scores[0, 0]))
 
 
 def test_strided_tensors_and_a_wider_table(cuda_lib):
