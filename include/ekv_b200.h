@@ -478,8 +478,8 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  *          a row (tokens == rows). Token i of a row's n sees the positions below lens[r] - n + i + 1.
  * out [tokens][q_heads][head_dim] (element strides) receives softmax(scale q K^T) V and lse (may be NULL;
  * float32 [tokens][q_heads]) the natural log of the sum of exp(scale q.k); a query token that sees nothing gets
- * 0 and -inf. Tokens of no row keep what they have. What lies behind a row may hold anything; values at positions that one of
- * a row's query tokens sees and another does not must be finite.
+ * 0 and -inf. Tokens of no row keep what they have. What lies behind a row may hold anything; values at positions
+ * that one of a row's query tokens sees and another does not must be finite.
  *
  * groups > 0: the rows [group_start[g], group_start[g + 1]) (int32 [groups + 1]; NULL with groups = 1: every row)
  * share their first prefix_blocks[g] blocks (int32 [groups]; NULL with groups = 1: prefix_common blocks): their
@@ -507,9 +507,9 @@ int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, con
  * (int32 [rows]; NULL: slot r). A token of the row at position t < lens[r] receives, per KV head, the weight
  * w = sum of exp(scale q.k - lse) over the row's query tokens and the head's query heads: its score becomes w
  * when t is among the row's newest fresh[r] tokens (int32 [rows]; NULL: its query tokens), which have none
- * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends without scoring; a
- * slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. Two or three kernels, no
- * host synchronisation.
+ * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends
+ * without scoring; a slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required.
+ * Two or three kernels, no host synchronisation.
  */
 size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,
                                          int head_dim);
@@ -546,13 +546,15 @@ size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_t pool_bloc
 /*
  * ekv_compact_tokens -- the kept tokens of each row and KV head moved to the front of the row's blocks, in place.
  *
- * kv [pool_blocks][2][block_size][heads] rows of head_bytes bytes (strides in bytes, whole 16-byte units, 16 to 1024 bytes; any element type).
+ * kv [pool_blocks][2][block_size][heads] rows of head_bytes bytes (16 to 1024; strides in bytes; all in whole 16-byte
+ * units; any element type).
  * In every row with 0 <= new_lens[r] < lens[r], position j < new_lens[r] of KV head h takes the key, the value and,
  * with scores (as in ekv_attend_scored; may be NULL), the score of position kept[r][h][j] (int32, `columns` entries a
  * list, ascending strictly, below lens[r]); what lies behind new_lens[r] stays as it was. The lists keep the first
  * first_tokens positions in place, so blocks wholly among them may be shared between rows; every other block a
  * moving row holds must be its own. A row whose lists, blocks or slot break this is left as it was, with
- * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. Two kernels, with a memset before them for tables of more than 512 entries; no host synchronisation.
+ * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. Two kernels, with a memset before them for tables of
+ * more than 512 entries; no host synchronisation.
  */
 int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
                        int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,

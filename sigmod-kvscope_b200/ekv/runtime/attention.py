@@ -162,7 +162,7 @@ def attend(
             query.data_ptr(), q_stride[0], q_stride[1], kv_cache.data_ptr(), kv_stride[0], kv_stride[1], kv_stride[2],
             kv_stride[3], blocks, table.data_ptr(), table_stride, lens.data_ptr(), starts, tokens, rows, width, block_size,
             q_heads, kv_heads, dim, dtype,
-            scale, groups, members, prefix, common, out.data_ptr(), out_stride[0], out_stride[1], lse.data_ptr(),
+            float(scale), groups, members, prefix, common, out.data_ptr(), out_stride[0], out_stride[1], lse.data_ptr(),
             workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_attend")
@@ -233,7 +233,7 @@ def attend_scored(
             query.data_ptr(), q_stride[0], q_stride[1], kv_cache.data_ptr(), kv_stride[0], kv_stride[1], kv_stride[2],
             kv_stride[3], blocks, table.data_ptr(), table_stride, lens.data_ptr(), starts, tokens, rows, width, block_size,
             q_heads, kv_heads, dim, dtype,
-            scale, scores.data_ptr(), score_stride[0], score_stride[1], len(scores), places, new, decay,
+            float(scale), scores.data_ptr(), score_stride[0], score_stride[1], len(scores), places, new, float(decay),
             out.data_ptr(), out_stride[0], out_stride[1], lse.data_ptr(), workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_attend_scored")

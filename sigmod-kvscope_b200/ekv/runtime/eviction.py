@@ -74,7 +74,7 @@ def select_tokens(
     with _lib.on_device(device) as stream:
         rc = _lib.load().ekv_select_tokens(
             scores.data_ptr(), stride[0], stride[1], n_slots, capacity, places, length, counts,
-            max(min(count, 0x7FFFFFFF), -1), min(first_tokens, capacity), min(recent_tokens, capacity), rows, heads,
+            max(min(count, 0x7FFFFFFF), -1), min(int(first_tokens), capacity), min(int(recent_tokens), capacity), rows, heads,
             kept.data_ptr(), kept_stride[0], kept_stride[1], new, word, stream,
         )
     _lib.check(rc, "ekv_select_tokens")
@@ -140,7 +140,7 @@ def compact_tokens(
         rc = lib.ekv_compact_tokens(
             kv_cache.data_ptr(), s_block * item, s_part * item, s_pos * item, s_head * item, blocks, dim * item,
             table.data_ptr(), table.stride(0), length, rows, width, heads, block_size, kept.data_ptr(), kept_stride[0],
-            kept_stride[1], kept.shape[2], new, min(first_tokens, width * block_size), _lib.ptr(scores),
+            kept_stride[1], kept.shape[2], new, min(int(first_tokens), width * block_size), _lib.ptr(scores),
             score_stride[0], score_stride[1], len(scores) if scores is not None else 0, places,
             workspace.data_ptr(), size, word, stream,
         )

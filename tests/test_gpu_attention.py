@@ -437,6 +437,17 @@ def test_hundreds_of_rows_most_of_them_empty(cuda_lib, grouped, wide):
     check(attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], **more), x, 0.1, torch.bfloat16)
 
 
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_a_batch_with_nothing_in_its_cache(cuda_lib, rows, grouped):
+    from ekv.runtime.attention import attend
+
+    x = make(44, [0] * rows, queries=[2] * rows, width=40)
+    d = on_device(x)
+    out, lse = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=3 if grouped else None)
+    assert torch.all(out == 0) and torch.all(lse == float("-inf"))
+
+
 def test_scores_of_hundreds_of_rows(cuda_lib):
     rng = np.random.default_rng(6)
     lens = [int(n) if rng.random() < 0.5 else 0 for n in rng.integers(1, 150, 300)]
