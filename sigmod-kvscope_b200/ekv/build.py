@@ -33,6 +33,7 @@ def command(output: str = OUTPUT, extra: list[str] | None = None) -> list[str]:
         nvcc(),
         *ARCH_FLAGS,
         "-O3",
+        "--threads=0",  # the sources beside one another
         "-lineinfo",
         "-std=c++17",
         "-Xcompiler",
