@@ -5,7 +5,9 @@
 // l = sum 2^(x - m) and output o = sum 2^(x - m) v; when m grows to m', l and o are multiplied by 2^(m - m').
 // Parts of a row (its group's prefix, its own tokens, tiles of different CTAs) join the same way, so a
 // shared prefix is one launch whose query rows are those of every row of the group, and the two results meet
-// in the combine kernel: out = sum_j 2^(m_j - m) o_j / sum_j 2^(m_j - m) l_j.
+// in the combine kernel: out = sum_j 2^(m_j - m) o_j / sum_j 2^(m_j - m) l_j. A part that saw nothing has l = 0. m = -inf
+// does not say so: the maxima pass over NaN, so a part whose scores are all NaN ends with it and l = NaN, which has to reach
+// the row's sum, and through it the output and the log.
 //
 // attend_kernel. A CTA of four math warps and one copy warp walks its share of the launch's tiles (attend.cuh), two CTAs an
 // SM. The copy warp reads block ids and asks the TMA engine for the tile's key and value rows of one KV head, a block's
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][threadIdx.x]);
 #pragma unroll
         for (int w = 0; w < WN; ++w)
-          total += ms[w][threadIdx.x] == -INFINITY ? 0.f : ls[w][threadIdx.x] * exp2_fast(ms[w][threadIdx.x] - top);
+          total += ls[w][threadIdx.x] == 0.f ? 0.f : ls[w][threadIdx.x] * exp2_fast(ms[w][threadIdx.x] - top);
         int64_t target = -1;
         if (mrow < uq.nq * p.G) {
           const int i = mrow / p.G, token = uq.q0 + i, head = it.head * p.G + mrow - i * p.G;
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < WN; ++w) top = fmaxf(top, ms[w][wm * 16 + quad + 8 * j]);
-        f[j] = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - top);
+        f[j] = l[j] == 0.f ? 0.f : exp2_fast(m[j] - top);
       }
       const int rows = min(16, uq.nq * p.G - it.mt * MT);  // of the first of the WM: the others have no more
 #pragma unroll
@@ -657,10 +659,10 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_c
       float top = ml.x;
       for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
       top = fmaxf(top, m);
-      const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
+      const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
       const float keep = m == -INFINITY ? 0.f : exp2_fast(m - top);
       m = top;
-      l = l * keep + (f == 0.f ? 0.f : f * ml.y);
+      l = l * keep + f * ml.y;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) acc[d] *= keep;
       auto add = [&](int i0, const float(&from)[8][D / 32]) {

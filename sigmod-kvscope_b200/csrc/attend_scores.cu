@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kAddThreads) add_kernel(const __grid_constant_
   float* dst = sp.scores + (int64_t)slot * sp.s0 + (int64_t)head * sp.s1;
   const float* first = p.logits + ((int64_t)un.q.q0 * p.q_heads + head * p.G) * p.logits_s0;
   const float* lses = p.lse + (int64_t)un.q.q0 * p.q_heads + head * p.G;
+  const int32_t* ids = p.table + (int64_t)row * p.table_s0;
   for (int pos = 4 * (blockIdx.y * kAddThreads + threadIdx.x); pos < un.to; pos += 4 * gridDim.y * kAddThreads) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < un.q.nq; ++i) {
@@ -76,6 +77,13 @@ __global__ void __launch_bounds__(kAddThreads) add_kernel(const __grid_constant_
       for (int g = 0; g < p.G; ++g) {
         const float lse = lses[(int64_t)i * p.q_heads + g] * kLog2e;
         if (lse == -INFINITY) continue;  // it saw nothing
+        if (isnan(lse)) {  // what it saw has no weight that is a number; what it did not see (a logit of -inf) takes none
+          for (int e = 0; e < 4; ++e) {
+            const int id = pos + e < un.to - un.q.nq + i + 1 ? ids[(pos + e) >> p.block_shift] : -1;
+            if (id >= 0 && (int64_t)id < p.pool_blocks) w[e] = lse;
+          }
+          continue;
+        }
         const float4 x = *reinterpret_cast<const float4*>(first + ((int64_t)i * p.q_heads + g) * p.logits_s0 + pos);
         w[0] += exp2_fast(x.x - lse);
         w[1] += exp2_fast(x.y - lse);

@@ -476,3 +476,105 @@ def test_a_view_of_a_row_attends_to_its_blocks_alone(cuda_lib):
     got = attend(d["query"], d["cache"], view, view_lens, 0.1)
     x["table"], x["lens"] = view.cpu(), view_lens.cpu()
     check(got, x, 0.1, torch.bfloat16, start=False)
+
+
+# ---- queries and keys that are not numbers ------------------------------------------------------------------
+
+
+def nan_batch(kind):
+    """A batch for each way that parts of a row join: lengths, queries and head counts that pick it, and the call's arguments."""
+    shapes = {
+        "a CTA an item": dict(lens=[1, 17, 333]),
+        "tiles dealt": dict(lens=[1, 17, 333], width=40),
+        "split over CTAs": dict(lens=[1, 17, 9001]),
+        "24 query rows a head": dict(lens=[1, 17, 333], q_heads=48),
+        "48 query rows a head": dict(lens=[1, 17, 9001], q_heads=96),
+        "several query tokens": dict(lens=[1, 19, 1025], queries=[3, 3, 3]),
+        "many query rows": dict(lens=[1, 41, 3001], queries=[40, 40, 40], q_heads=16),
+        "one subtile of many": dict(lens=[1, 17, 3001], queries=[15, 10, 12], q_heads=16),
+        "behind a prefix": dict(lens=[65, 81, 700], groups=[(0, 3, 4)]),
+        "many behind a prefix": dict(lens=[1985, 2001, 2600], queries=[30, 30, 30], q_heads=16, groups=[(0, 3, 120)]),
+    }
+    x = make(50, **shapes[kind])
+    if "many" in kind:
+        x = widen(x, 1 << 17)  # the kernel for many query rows
+    prefix = shapes[kind].get("groups", [(0, 0, None)])[0][2]
+    return x, {} if prefix is None else dict(prefix_blocks=prefix)
+
+
+NAN_KINDS = ["a CTA an item", "tiles dealt", "split over CTAs", "24 query rows a head", "48 query rows a head",
+             "several query tokens", "many query rows", "one subtile of many", "behind a prefix", "many behind a prefix"]
+
+
+def put_nan(x, fault):
+    start, lens, table, cache = x["start"].tolist(), x["lens"].tolist(), x["table"], x["cache"]
+    for r, n in enumerate(lens):
+        if fault == "queries":  # a head of each row's newest query token, and in row 2 another's of its oldest
+            x["query"][start[r + 1] - 1, 5, 7] = float("nan")
+            x["query"][start[2], 0, 0] = float("nan")
+        elif fault == "newest keys":
+            cache[table[r, (n - 1) // 16], 0, (n - 1) % 16, 1, 3] = float("nan")
+        else:  # every key of 128 tokens, or of what the row has before its newest one
+            for t in range(max(0, n - 150), max(0, n - 22) if n > 150 else n - 1):
+                cache[table[r, t // 16], 0, t % 16, 0, 0] = float("nan")
+
+
+def same_nan(got, want):
+    np.testing.assert_array_equal(np.isnan(got.float().cpu().numpy()), np.isnan(want))
+
+
+@pytest.mark.parametrize("fault", ["queries", "newest keys", "a run of keys"])
+@pytest.mark.parametrize("kind", NAN_KINDS)
+def test_nan_reaches_every_output_that_it_is_part_of_and_no_other(cuda_lib, kind, fault):
+    from ekv.runtime.attention import attend
+
+    x, more = nan_batch(kind)
+    put_nan(x, fault)
+    d = on_device(x)
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], **more)
+    out, lse, _ = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(),
+                             0.1, x["start"].numpy())
+    assert np.isnan(lse).any() and not np.isnan(lse).all()
+    same_nan(got[0], out)
+    same_nan(got[1], lse)
+    check(got, x, 0.1, torch.bfloat16)
+
+
+@pytest.mark.parametrize("fault", ["queries", "newest keys", "a run of keys"])
+@pytest.mark.parametrize("kind", NAN_KINDS[:8])
+def test_nan_reaches_every_score_that_it_is_part_of_and_no_other(cuda_lib, kind, fault):
+    from ekv.runtime.attention import attend_scored
+
+    x, _ = nan_batch(kind)
+    put_nan(x, fault)
+    ok = np.ones(tuple(x["table"].shape), dtype=bool)
+    if kind != "a CTA an item":
+        x["table"][2, 3], ok[2, 3] = -1, False  # a block that is not there gives its tokens no weight
+    d = on_device(x)
+    used = max(x["lens"].tolist())
+    scores = torch.full((3, 2, x["table"].shape[1] * 16), 0.5, device="cuda")
+    attend_scored(d["query"], d["cache"], d["table"], d["lens"], 0.1, scores, query_start=d["start"])
+    _, lse, w = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(), 0.1,
+                           x["start"].numpy(), ok)
+    queries = (x["start"][1:] - x["start"][:-1]).tolist()
+    want = oat.accumulate(np.full((3, 2, used), 0.5), [0, 1, 2], x["lens"].tolist(), queries, w)
+    assert np.isnan(want).any() and not np.isnan(want).all()
+    # as for weights that are all numbers: 4e-5 of the largest a token can have, one from every query row
+    most = max(queries) * x["query"].shape[1] / 2
+    np.testing.assert_allclose(scores[..., :used].cpu().numpy(), want, rtol=1e-6, atol=4e-5 * most)
+    assert torch.all(scores[..., used:] == 0.5)
+
+
+def test_scores_in_a_table_too_wide_for_the_logits(cuda_lib):
+    """Two rows of one query token in a table of 2^23 and more positions: the weights come from the keys again."""
+    x = make(51, [700, 33], q_heads=16, kv_heads=1, dim=64)
+    x = widen(x, (1 << 23) + 64)
+    scores = torch.full((2, 1, x["table"].shape[1] * 16), 0.25)
+    from ekv.runtime.attention import attend_scored
+
+    d, got = on_device(x), scores.cuda()
+    check(attend_scored(d["query"], d["cache"], d["table"], d["lens"], 0.1, got), x, 0.1, torch.bfloat16)
+    _, _, w = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(), 0.1)
+    want = oat.accumulate(np.full((2, 1, 700), 0.25), [0, 1], [700, 33], [1, 1], w)
+    np.testing.assert_allclose(got[..., :700].cpu().numpy(), want, rtol=1e-6, atol=4e-5 * 16)
+    assert torch.all(got[..., 700:] == 0.25)
