@@ -15,8 +15,9 @@
 // compact: position j of a (row, head) takes the key, value and score of position kept[j] >= j, in place, in
 // chunks: a chunk's sources are all read before any of it is written, and later chunks only read positions past
 // it, so the copy that fills chunk k + 1 may run while chunk k is stored. check_kernel comes first: the list must ascend
-// strictly, from the identity on the protected first tokens, and no block the row writes may be another row's, or
-// occur twice in the row (each block a row holds is claimed once in an owner table); a row that fails is left as it was.
+// strictly, from the identity on the protected first tokens, and no block behind those may be another row's, or occur
+// twice in the row, also where its other holder protects it. A block is claimed once in an owner table, or marked as
+// protected there, which any number of rows may do; a row that fails is left as it was.
 #include <cooperative_groups.h>
 
 #include <mutex>
@@ -265,7 +266,7 @@ struct CompactParams {
   const int32_t* slots;
   int n_slots;
   int rows, width, heads, block_size, first, row_bytes;
-  int32_t* owner;  // [pool_blocks], 0: nobody's; NULL: few blocks, compared with one another
+  uint32_t* owner;  // [pool_blocks] the row that claimed it + 1, and kProtected; NULL: few blocks, compared with one another
   int32_t* bad;    // [rows] kRow* bits that rows find in each other, with an owner table
   int32_t* flags;  // [rows][heads] kRow* bits
   int32_t* hole;   // [rows][heads] the first position that takes another's token
@@ -287,12 +288,7 @@ __device__ __forceinline__ bool row_moves(const CompactParams& p, int row, int& 
 // clear, which is a launch less (four rows of 44 blocks: see ekv_compact_tokens).
 constexpr int kFewBlocks = 512;
 
-// The blocks [from, to) of a row that must be its own: all that it holds, but for those a moving row's protected tokens fill.
-__device__ __forceinline__ void own_blocks(const CompactParams& p, int row, int& from, int& to) {
-  int n, m;
-  from = row_moves(p, row, n, m) ? p.first / p.block_size : 0;
-  to = (n + p.block_size - 1) / p.block_size;
-}
+constexpr uint32_t kProtected = 0x80000000u;  // of an owner entry: a moving row keeps the block's tokens in place
 
 __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_constant__ CompactParams p) {
   __shared__ int s_hole, s_flags;
@@ -310,6 +306,7 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
   if (head == 0) {
     const int64_t most = (int64_t)p.width * p.block_size;
     if (threadIdx.x == 0 && p.lens[row] > most) set_status(p.status, EKV_STATUS_LEN_OVER_WIDTH);
+    // the blocks that must be the row's own: all that it holds, but for those a moving row's protected tokens fill
     const int blocks = (n + p.block_size - 1) / p.block_size, own = moves ? p.first / p.block_size : 0;
     for (int b = threadIdx.x; b < blocks; b += kCheckThreads) {
       const int id = p.table[(int64_t)row * p.table_s0 + b];
@@ -317,21 +314,22 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
       if (bad && moves) atomicOr(&s_flags, kRowBlock);
       if (p.owner == nullptr) {
         s_ids[b] = id;
-      } else if (!bad && b >= own) {
-        const int other = atomicCAS(&p.owner[id], 0, row + 1);
-        if (other != 0) {  // claimed before, by another row or by this one
-          atomicOr(&p.bad[row], kRowShared);
-          atomicOr(&p.bad[other - 1], kRowShared);
-        }
+      } else if (!bad) {
+        // whichever of two comes second sees the other: a second claim is bad for both rows, a claim of what some row
+        // protects for the one that claims
+        const uint32_t other = b >= own ? atomicCAS(&p.owner[id], 0u, (uint32_t)row + 1) : atomicOr(&p.owner[id], kProtected);
+        const uint32_t claimed = other & ~kProtected;
+        if (b >= own && other != 0) atomicOr(&p.bad[row], kRowShared);
+        if (claimed != 0) atomicOr(&p.bad[claimed - 1], kRowShared);
       }
     }
     if (p.owner == nullptr && moves) {
       __syncthreads();
       for (int i = threadIdx.x; i < p.rows * p.width; i += kCheckThreads) {
         const int r = i / p.width, b = i - r * p.width;
-        int from, to;
-        own_blocks(p, r, from, to);
-        if (b < from || b >= to) continue;
+        int held, kept;
+        row_moves(p, r, held, kept);
+        if (b >= (held + p.block_size - 1) / p.block_size) continue;
         const int id = p.table[(int64_t)r * p.table_s0 + b];
         bool shared = false;
         for (int mine = own; mine < blocks; ++mine) shared |= s_ids[mine] == id && (r != row || mine != b);
@@ -574,7 +572,7 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
   const CompactParams p{static_cast<uint8_t*>(kv), kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, pool_blocks,
                         table, table_stride, lens, kept, kept_stride_row, kept_stride_head, columns, new_lens, scores,
                         score_stride_slot, score_stride_head, slots, n_slots, rows, width, heads, block_size, first_tokens,
-                        head_bytes, few ? nullptr : reinterpret_cast<int32_t*>(ws + w.owner), reinterpret_cast<int32_t*>(ws + w.bad),
+                        head_bytes, few ? nullptr : reinterpret_cast<uint32_t*>(ws + w.owner), reinterpret_cast<int32_t*>(ws + w.bad),
                         reinterpret_cast<int32_t*>(ws + w.flags), reinterpret_cast<int32_t*>(ws + w.hole), status};
   launch_chained(check_kernel, dim3(rows * heads), dim3(kCheckThreads), 0, s, p);
   int rc = check_launch("check_kernel");

@@ -335,3 +335,83 @@ def test_a_bounded_cache_over_many_steps(cuda_lib):
             lens[r] = t + 1
     assert evictions >= 2
     np.testing.assert_allclose(scores[1, 0, : lens[1] - 1].cpu().numpy(), weight[1][0], rtol=1e-5, atol=1e-4)
+
+
+# ---- protected blocks ---------------------------------------------------------------------------------
+
+
+def first_then_every_other(rows, heads, first, columns):
+    """Lists that keep the first tokens in place and every other one behind them."""
+    kept = first + 2 + 2 * torch.arange(columns, dtype=torch.int32)
+    kept = torch.cat([torch.arange(first, dtype=torch.int32), kept])[:columns]
+    return kept.expand(rows, heads, columns).contiguous()
+
+
+@pytest.mark.parametrize("lens, new, moved", [([100] * 4, [50] * 4, (0, 2, 3)), ([100, 100, 14, 100], [50, 50, 9, 50], (0, 2, 3)),
+                                              ([100] * 4, [100, 50, 50, 50], (2, 3))])
+def test_compact_refuses_to_write_another_rows_protected_block(cuda_lib, lens, new, moved):
+    """Row 1 lists, where its own tokens go, a block of which other rows keep the first tokens in place; they stay as they
+    are, also where those rows are moved, are shorter than what is kept in place, or are not moved at all."""
+    cache, _, table = batch(11, lens, width=7)
+    table[3, 0] = table[0, 0]  # a prefix of two rows
+    broken = table.clone()
+    broken[1, 2] = table[0, 0]
+    refused("STATUS_BLOCK_SHARED", cache, broken, lens, first_then_every_other(4, 2, 16, 50), new, first=16, moved=moved)
+
+
+def test_compact_refuses_a_row_that_repeats_its_own_protected_block(cuda_lib):
+    cache, _, table = batch(12, [100] * 4)
+    kept = first_then_every_other(4, 2, 33, 50)
+    for where in (2, 5):  # among the blocks that tokens move to, and among those that they leave
+        broken = table.clone()
+        broken[2, where] = table[2, 1]
+        refused("STATUS_BLOCK_SHARED", cache, broken, [100] * 4, kept, [50] * 4, first=33, moved=(0, 1, 3))
+
+
+def test_many_rows_with_one_prefix_and_some_that_would_write_it(cuda_lib):
+    """Claims and protections of the same blocks from many CTAs at once: the outcome is the same in every run."""
+    import ekv._lib as L
+    from ekv.runtime.eviction import compact_tokens
+
+    rows = 96
+    cache, _, table = batch(13, [100] * rows, heads=1, dim=64)
+    table[:, :2] = table[0, :2].clone()
+    wrong = [5, 50]  # of different blocks
+    for r in wrong:
+        table[r, 3 + r % 3] = table[0, r % 2]
+    kept = first_then_every_other(rows, 1, 32, 60)
+    new = [60] * rows
+    want, _ = oat.compact(cache.view(torch.uint8).numpy(), None, table.numpy(), [100] * rows, kept.numpy(),
+                          [-1 if r in wrong else 60 for r in range(rows)], list(range(rows)))
+    for _ in range(5):
+        got, status = cache.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+        compact_tokens(got, table.cuda(), ints([100] * rows), kept.cuda(), ints(new), first_tokens=32, status=status)
+        assert int(status) == L.STATUS_BLOCK_SHARED
+        np.testing.assert_array_equal(got.cpu().view(torch.uint8).numpy(), want)
+
+
+def test_a_replayed_graph_over_a_large_table(cuda_lib):
+    """More than 512 table entries: the owner table is cleared by every replay, so one batch leaves the next nothing."""
+    from ekv.runtime.eviction import compact_tokens
+
+    lens = [500, 640, 30, 700]
+    cache, _, table = batch(14, lens, width=200)
+    kept = first_then_every_other(4, 2, 16, 200)
+    dev, tab, new, status = cache.cuda(), table.cuda(), ints([200, 200, 30, 200]), torch.zeros(1, dtype=torch.int32, device="cuda")
+    dev_lens, dev_kept = ints(lens), kept.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        compact_tokens(dev, tab, dev_lens, dev_kept, new, first_tokens=16, status=status)
+    shared = table.clone()
+    shared[3, 5] = table[1, 0]
+    for now, left in ((table, ()), (shared, (3,)), (table.flip(0).contiguous(), ())):
+        now_lens = lens if now is not shared else [500, 640, 0, 700]
+        dev.copy_(cache)
+        tab.copy_(now)
+        dev_lens.copy_(torch.tensor(now_lens, dtype=torch.int32))
+        status.zero_()
+        graph.replay()
+        assert (int(status) != 0) == bool(left)
+        want, _ = oat.compact(cache.view(torch.uint8).numpy(), None, now.numpy(), now_lens, kept.numpy(),
+                              [-1 if r in left else m for r, m in enumerate([200, 200, 30, 200])], list(range(4)))
+        np.testing.assert_array_equal(dev.cpu().view(torch.uint8).numpy(), want)
