@@ -555,6 +555,10 @@ size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_t pool_bloc
  * moving row holds must be its own. A row whose lists, blocks or slot break this is left as it was, with
  * EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID or _BAD_SLOT. Two kernels, with a memset before them for tables of
  * more than 512 entries; no host synchronisation.
+ *
+ * The status word speaks for the whole batch. ekv_compact_tokens_lens is the same call that also says what became of each
+ * row: result_lens int32 [rows] (may be NULL; shares no memory with lens or new_lens) receives the tokens that the row now
+ * holds, new_lens[r] where it was moved and lens[r] where it was left. Only blocks behind that length are free for others.
  */
 int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
                        int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
@@ -563,6 +567,13 @@ int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part
                        const int32_t* new_lens, int first_tokens, float* scores, int64_t score_stride_slot,
                        int64_t score_stride_head, int n_slots, const int32_t* slots, void* workspace,
                        size_t workspace_bytes, uint32_t* status, void* stream);
+int ekv_compact_tokens_lens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                            int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
+                            int64_t table_stride, const int32_t* lens, int rows, int width, int heads, int block_size,
+                            const int32_t* kept, int64_t kept_stride_row, int64_t kept_stride_head, int columns,
+                            const int32_t* new_lens, int first_tokens, float* scores, int64_t score_stride_slot,
+                            int64_t score_stride_head, int n_slots, const int32_t* slots, int32_t* result_lens,
+                            void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -270,6 +270,7 @@ struct CompactParams {
   int32_t* bad;    // [rows] kRow* bits that rows find in each other, with an owner table
   int32_t* flags;  // [rows][heads] kRow* bits
   int32_t* hole;   // [rows][heads] the first position that takes another's token
+  int32_t* result_lens;  // [rows] the tokens that the rows hold afterwards, or NULL
   uint32_t* status;
 };
 
@@ -379,12 +380,16 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const __grid_cons
   const int row = unit / p.heads, head = unit - row * p.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int n, m;
-  if (!row_moves(p, row, n, m)) return;  // as every CTA of the cluster does
+  const bool reports = threadIdx.x == 0 && rank == 0 && head == 0 && only == 0, moves = row_moves(p, row, n, m);
   int bad = 0;  // a row is moved whole or not at all
-  for (int h = lane; h < p.heads; h += 32) bad |= p.flags[row * p.heads + h];
-  bad = __reduce_or_sync(kFullMask, bad) | (p.owner != nullptr ? p.bad[row] : 0);
+  if (moves) {  // as every CTA of the cluster finds
+    for (int h = lane; h < p.heads; h += 32) bad |= p.flags[row * p.heads + h];
+    bad = __reduce_or_sync(kFullMask, bad) | (p.owner != nullptr ? p.bad[row] : 0);
+  }
+  if (reports && p.result_lens != nullptr) p.result_lens[row] = moves && !bad ? m : p.lens[row];
+  if (!moves) return;
   if (bad) {
-    if (threadIdx.x == 0 && rank == 0 && head == 0 && only == 0)
+    if (reports)
       set_status(p.status, (bad & kRowShared ? EKV_STATUS_BLOCK_SHARED : 0u) | (bad & kRowList ? EKV_STATUS_BAD_LIST : 0u) |
                                (bad & kRowBlock ? EKV_STATUS_BAD_BLOCK_ID : 0u) | (bad & kRowSlot ? EKV_STATUS_BAD_SLOT : 0u));
     return;
@@ -479,6 +484,12 @@ struct CompactLayout {
   size_t owner, bad, flags, hole, total;
 };
 
+// Whether two arrays of `count` int32 share memory.
+bool overlap(const int32_t* a, const int32_t* b, int count) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), size = (uintptr_t)count * 4;
+  return x < y + size && y < x + size;
+}
+
 CompactLayout compact_layout(int rows, int heads, int64_t pool_blocks) {
   CompactLayout w{};
   w.owner = 0;
@@ -536,13 +547,14 @@ extern "C" size_t ekv_compact_tokens_workspace_bytes(int rows, int heads, int64_
   return compact_layout(rows, heads, pool_blocks).total;
 }
 
-extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
-                                  int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
-                                  int64_t table_stride, const int32_t* lens, int rows, int width, int heads, int block_size,
-                                  const int32_t* kept, int64_t kept_stride_row, int64_t kept_stride_head, int columns,
-                                  const int32_t* new_lens, int first_tokens, float* scores, int64_t score_stride_slot,
-                                  int64_t score_stride_head, int n_slots, const int32_t* slots, void* workspace,
-                                  size_t workspace_bytes, uint32_t* status, void* stream) {
+extern "C" int ekv_compact_tokens_lens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                                       int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
+                                       int64_t table_stride, const int32_t* lens, int rows, int width, int heads,
+                                       int block_size, const int32_t* kept, int64_t kept_stride_row,
+                                       int64_t kept_stride_head, int columns, const int32_t* new_lens, int first_tokens,
+                                       float* scores, int64_t score_stride_slot, int64_t score_stride_head, int n_slots,
+                                       const int32_t* slots, int32_t* result_lens, void* workspace,
+                                       size_t workspace_bytes, uint32_t* status, void* stream) {
   clear_error();
   if (!kv || !table || !lens || !kept || !new_lens) return fail(EKV_EINVAL, "a required device pointer is NULL");
   if (rows <= 0 || width <= 0 || heads <= 0 || block_size <= 0 || pool_blocks <= 0 || columns <= 0)
@@ -562,6 +574,8 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
     if ((heads > 1 && score_stride_head < most) || (n_slots > 1 && score_stride_slot < most))
       return fail(EKV_EINVAL, "scores must hold at least width * block_size tokens for every slot and head");
   }
+  if (result_lens && (overlap(result_lens, lens, rows) || overlap(result_lens, new_lens, rows)))
+    return fail(EKV_EINVAL, "result_lens must share no memory with lens or new_lens");
   const CompactLayout w = compact_layout(rows, heads, pool_blocks);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
@@ -573,7 +587,7 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
                         table, table_stride, lens, kept, kept_stride_row, kept_stride_head, columns, new_lens, scores,
                         score_stride_slot, score_stride_head, slots, n_slots, rows, width, heads, block_size, first_tokens,
                         head_bytes, few ? nullptr : reinterpret_cast<uint32_t*>(ws + w.owner), reinterpret_cast<int32_t*>(ws + w.bad),
-                        reinterpret_cast<int32_t*>(ws + w.flags), reinterpret_cast<int32_t*>(ws + w.hole), status};
+                        reinterpret_cast<int32_t*>(ws + w.flags), reinterpret_cast<int32_t*>(ws + w.hole), result_lens, status};
   launch_chained(check_kernel, dim3(rows * heads), dim3(kCheckThreads), 0, s, p);
   int rc = check_launch("check_kernel");
   if (rc != EKV_OK) return rc;
@@ -588,4 +602,17 @@ extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_
   while (C < 8 && units * (split + 1) * C * 2 <= 4 * sms) C *= 2;
   launch_chained_cluster(move_kernel, dim3((unsigned)(units * C * (split ? 2 : 1))), dim3(kMoveThreads), 0, s, (unsigned)C, p, split);
   return check_launch("move_kernel");
+}
+
+extern "C" int ekv_compact_tokens(void* kv, int64_t kv_stride_block, int64_t kv_stride_part, int64_t kv_stride_pos,
+                                  int64_t kv_stride_head, int64_t pool_blocks, int head_bytes, const int32_t* table,
+                                  int64_t table_stride, const int32_t* lens, int rows, int width, int heads, int block_size,
+                                  const int32_t* kept, int64_t kept_stride_row, int64_t kept_stride_head, int columns,
+                                  const int32_t* new_lens, int first_tokens, float* scores, int64_t score_stride_slot,
+                                  int64_t score_stride_head, int n_slots, const int32_t* slots, void* workspace,
+                                  size_t workspace_bytes, uint32_t* status, void* stream) {
+  return ekv_compact_tokens_lens(kv, kv_stride_block, kv_stride_part, kv_stride_pos, kv_stride_head, pool_blocks, head_bytes,
+                                 table, table_stride, lens, rows, width, heads, block_size, kept, kept_stride_row,
+                                 kept_stride_head, columns, new_lens, first_tokens, scores, score_stride_slot,
+                                 score_stride_head, n_slots, slots, nullptr, workspace, workspace_bytes, status, stream);
 }

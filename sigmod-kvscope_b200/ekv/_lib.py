@@ -147,6 +147,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _p, _i64, _i64, _i32, _p, _i32,  # kept columns new_lens first_tokens
          _p, _i64, _i64, _i32, _p, _p, _sz, _p, _p],  # scores n_slots slots workspace bytes status stream
     ),
+    "ekv_compact_tokens_lens": (
+        _i32,
+        [_p, _i64, _i64, _i64, _i64, _i64, _i32,  # kv and byte strides, pool_blocks head_bytes
+         _p, _i64, _p, _i32, _i32, _i32, _i32,  # table lens rows width heads block_size
+         _p, _i64, _i64, _i32, _p, _i32,  # kept columns new_lens first_tokens
+         _p, _i64, _i64, _i32, _p, _p, _p, _sz, _p, _p],  # scores n_slots slots result_lens workspace bytes status stream
+    ),
 }
 
 _lib: ctypes.CDLL | None = None

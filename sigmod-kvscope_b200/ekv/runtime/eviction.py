@@ -91,6 +91,7 @@ def compact_tokens(
     first_tokens: int = 0,
     scores: torch.Tensor | None = None,
     slots: torch.Tensor | None = None,
+    result_lens: torch.Tensor | None = None,
     status: torch.Tensor | None = None,
 ) -> None:
     """Move each row's kept tokens to the front of its blocks, in place.
@@ -102,7 +103,10 @@ def compact_tokens(
 
     Blocks wholly among the first ``first_tokens`` tokens may be shared between rows; every other block of a row that
     shrinks must be its own. A row whose lists, blocks or slot break this is left as it was, with the reason in
-    ``status`` (EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID, _BAD_SLOT).
+    ``status`` (EKV_STATUS_BAD_LIST, _BLOCK_SHARED, _BAD_BLOCK_ID, _BAD_SLOT), which speaks for the whole batch.
+    ``result_lens`` (int32 [rows], memory of its own) receives the tokens each row holds afterwards: ``new_lens[r]``
+    where the row was moved, ``lens[r]`` where it was left. These are the rows' lengths from here on; only the blocks
+    behind them are free.
     """
     if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.stride(4) != 1:
         raise ValueError(f"expected a KV cache [blocks, 2, block, heads, dim] with contiguous heads, got {tuple(kv_cache.shape)}")
@@ -127,6 +131,7 @@ def compact_tokens(
         raise ValueError("slots map rows to scores: there are none")
     if first_tokens < 0:
         raise ValueError("first_tokens must not be negative")
+    after = _index("result_lens", result_lens, rows, device)
     word = _status(status, device)
     if rows == 0:
         return
@@ -137,11 +142,11 @@ def compact_tokens(
     kept_stride = kept.stride()
     with _lib.on_device(device) as stream:
         workspace = kv_cache.new_empty(size, dtype=torch.uint8)
-        rc = lib.ekv_compact_tokens(
+        rc = lib.ekv_compact_tokens_lens(
             kv_cache.data_ptr(), s_block * item, s_part * item, s_pos * item, s_head * item, blocks, dim * item,
             table.data_ptr(), table.stride(0), length, rows, width, heads, block_size, kept.data_ptr(), kept_stride[0],
             kept_stride[1], kept.shape[2], new, min(int(first_tokens), width * block_size), _lib.ptr(scores),
-            score_stride[0], score_stride[1], len(scores) if scores is not None else 0, places,
+            score_stride[0], score_stride[1], len(scores) if scores is not None else 0, places, after,
             workspace.data_ptr(), size, word, stream,
         )
     _lib.check(rc, "ekv_compact_tokens")

@@ -179,3 +179,15 @@ def test_the_python_calls_refuse_what_is_not_on_a_device_or_does_not_fit():
         compact_tokens(cache, table, lens, torch.zeros(2, 2, 64, dtype=torch.int32), lens)
     with pytest.raises(ValueError, match="KV cache"):
         compact_tokens(cache[:, 0], table, lens, torch.zeros(2, 2, 64, dtype=torch.int32), lens)
+
+
+def test_compact_tokens_lens_refuses_what_compact_tokens_refuses_and_shared_memory(lib):
+    args = dict(kv=FAKE, s0=16384, s1=8192, s2=512, s3=256, pool=64, head_bytes=256, table=FAKE, ts=8, lens=FAKE, rows=4,
+                width=8, heads=2, bs=16, kept=FAKE, k0=256, k1=128, columns=128, new=ctypes.c_void_p(0x2000), first=0, scores=None,
+                ss0=0, ss1=0, n_slots=0, slots=None, result=ctypes.c_void_p(0x3000), ws=FAKE, ws_bytes=1 << 30, status=None, stream=None)
+    for over, code in [(dict(kv=None), L.EINVAL), (dict(rows=0), L.EINVAL), (dict(ws_bytes=100), L.ERANGE),
+                       (dict(result=FAKE), L.EINVAL),                      # the lengths themselves
+                       (dict(result=ctypes.c_void_p(0x1000 + 12)), L.EINVAL),  # from their last entry on
+                       (dict(result=ctypes.c_void_p(0x2000 - 12)), L.EINVAL),  # up to the new lengths' first
+                       (dict(result=ctypes.c_void_p(0x1000 + 16), ws_bytes=0), L.ERANGE)]:  # right behind them: the next check
+        assert lib.ekv_compact_tokens_lens(*{**args, **over}.values()) == code

@@ -415,3 +415,59 @@ def test_a_replayed_graph_over_a_large_table(cuda_lib):
         want, _ = oat.compact(cache.view(torch.uint8).numpy(), None, now.numpy(), now_lens, kept.numpy(),
                               [-1 if r in left else m for r, m in enumerate([200, 200, 30, 200])], list(range(4)))
         np.testing.assert_array_equal(dev.cpu().view(torch.uint8).numpy(), want)
+
+
+# ---- what became of each row ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("width", [7, 300])
+def test_compact_reports_each_rows_length(cuda_lib, width):
+    """Moved, not shrinking, with nothing in its cache, and refused for each reason: with few blocks and with many."""
+    import ekv._lib as L
+    from ekv.runtime.eviction import compact_tokens
+
+    lens = [100, 100, 0, 100, 100, 100, 100, 100, 100, 1]
+    cache, _, table = batch(15, lens, width=width)
+    scores = torch.rand(10, 2, width * 16, device="cuda")
+    table[4, 3] = table[3, 2]  # rows 3 and 4 share a block, the kept lists of row 5 do not ascend, row 6 has a block outside the pool
+    kept = lists(10, 2, 50)
+    kept[5, 1, 7] = 3
+    table[6, 6] = -1
+    slots = [0, 1, 2, 3, 4, 5, 6, 7, 10, 9]  # row 8's is outside the table
+    new = [50, 100, 0, 50, 50, 50, 50, 50, 50, 0]
+    after, status = ints([-7] * 11), torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = cache.cuda()
+    compact_tokens(got, table.cuda(), ints(lens), kept.cuda(), ints(new), scores=scores, slots=ints(slots), result_lens=after,
+                   status=status)
+    assert int(status) == L.STATUS_BLOCK_SHARED | L.STATUS_BAD_LIST | L.STATUS_BAD_BLOCK_ID | L.STATUS_BAD_SLOT
+    assert after.tolist() == [50, 100, 0, 100, 100, 100, 100, 50, 100, 0, -7]
+    moved = [m if r in (0, 7, 9) else -1 for r, m in enumerate(new)]
+    want, _ = oat.compact(cache.view(torch.uint8).numpy(), None, table.numpy(), lens, kept.numpy(), moved, list(range(10)))
+    np.testing.assert_array_equal(got.cpu().view(torch.uint8).numpy(), want)
+
+
+def test_a_refused_row_goes_on_with_all_of_its_tokens(cuda_lib):
+    """Select, compact and attend by the reported lengths: the refused row attends as before, the moved one to what it kept."""
+    from ekv.runtime.attention import attend
+    from ekv.runtime.eviction import compact_tokens, select_tokens
+
+    lens = [100, 100, 100]
+    gen = torch.Generator().manual_seed(16)
+    table = torch.randperm(21, generator=gen).reshape(3, 7).to(torch.int32)
+    table[2, :2] = table[1, :2].clone()  # a shared prefix that no first_tokens covers
+    cache = torch.randn(21, 2, 16, 2, 64, generator=gen).half()
+    query = torch.randn(3, 4, 64, generator=gen).half()
+    scores = torch.rand(3, 2, 112, generator=gen)
+    dev, after = cache.cuda(), ints([0] * 3)
+    kept, new = select_tokens(scores.cuda(), ints(lens), 40, first_tokens=4, recent_tokens=8)
+    compact_tokens(dev, table.cuda(), ints(lens), kept, new, first_tokens=4, scores=scores.cuda(), result_lens=after)
+    assert after.tolist() == [40, 100, 100] and new.tolist() == [40, 40, 40]
+    out, _ = attend(query.cuda(), dev, table.cuda(), after, 0.1)
+    whole, _ = attend(query.cuda(), cache.cuda(), table.cuda(), ints(lens), 0.1)
+    assert torch.equal(out[1:], whole[1:])
+    for h in range(2):
+        at = kept[0, h, :40].cpu().long()
+        k, v = (cache[table[0, at // 16].long(), part, at % 16, h].double() for part in (0, 1))
+        p = torch.softmax(query[0, 2 * h : 2 * h + 2].double() @ k.T * 0.1, -1)
+        # half a step of the output and one of each probability, both relative to 2^-11
+        assert torch.all((out[0, 2 * h : 2 * h + 2].double().cpu() - p @ v).abs() <= 2**-11 * ((p @ v).abs() + 1.1 * v.abs().max()) + 1e-4)
