@@ -17,6 +17,7 @@ the score by which ``eviction`` decides which tokens of a bounded cache to keep.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 
@@ -43,6 +44,14 @@ def _index(name: str, t: torch.Tensor | None, size: int, device: torch.device) -
             or (size > 1 and t.stride(0) != 1)):
         raise ValueError(f"{name} must be a contiguous int32 tensor of at least {size} entries on {device}")
     return t.data_ptr()
+
+
+def _count(name: str, value) -> int:
+    """A count of any whole-number type; a fraction is refused, not cut to one."""
+    try:
+        return operator.index(value)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number, got {value!r}") from None
 
 
 def _batch(query: torch.Tensor, kv_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor) -> tuple:
@@ -127,22 +136,23 @@ def attend(
     token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
     in the tables, which the kernels skip. The call runs on the current stream of the query's device.
     """
+    whole = prefix_blocks is None or isinstance(prefix_blocks, torch.Tensor)
+    common = 0 if whole else _count("prefix_blocks", prefix_blocks)
     device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride = _batch(query, kv_cache, table, lens)
     tokens, q_heads, dim = q_shape
     rows, width = table_shape
     blocks, _, block_size, kv_heads, _ = kv_shape
-    groups = common = 0
+    groups = 0
     prefix = None
     if isinstance(prefix_blocks, torch.Tensor):
         groups = prefix_blocks.shape[0] if prefix_blocks.dim() == 1 else 0
         if groups == 0 or (group_start is None and groups != 1):
             raise ValueError("prefix_blocks must hold a count per group, and several groups need group_start")
         prefix = _index("prefix_blocks", prefix_blocks, groups, device)
-    elif prefix_blocks is not None:
-        common = int(prefix_blocks)
+    elif common:
         if common < 0:
             raise ValueError("prefix_blocks must not be negative")
-        groups = 1 if common else 0
+        common, groups = min(common, width), 1
     if group_start is not None and prefix is None:
         raise ValueError("group_start needs the groups' prefix_blocks")
     starts = _index("query_start", query_start, rows + 1, device)

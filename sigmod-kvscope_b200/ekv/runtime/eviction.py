@@ -14,7 +14,7 @@ import functools
 import torch
 
 from .. import _lib
-from .attention import _index, _status, check_scores
+from .attention import _count, _index, _status, check_scores
 
 
 @functools.lru_cache(maxsize=256)
@@ -43,6 +43,8 @@ def select_tokens(
     equal scores go to the older token. ``kept`` int32 [rows, heads, capacity] lists the kept positions in ascending
     order, then -1; ``new_lens`` int32 [rows] counts them.
     """
+    first_tokens, recent_tokens = _count("first_tokens", first_tokens), _count("recent_tokens", recent_tokens)
+    count = 0 if isinstance(keep, torch.Tensor) else _count("keep", keep)
     device = scores.device
     if scores.dim() != 3:
         raise ValueError(f"scores must be a float32 [slots, heads, tokens] tensor, got {tuple(scores.shape)}")
@@ -59,7 +61,7 @@ def select_tokens(
         raise ValueError(f"{n_slots} score slots for {rows} rows")
     if first_tokens < 0 or recent_tokens < 0:
         raise ValueError("first_tokens and recent_tokens must not be negative")
-    counts, count = (_index("keep", keep, rows, device), 0) if isinstance(keep, torch.Tensor) else (None, int(keep))
+    counts = _index("keep", keep, rows, device) if isinstance(keep, torch.Tensor) else None
     if kept is None:
         kept = scores.new_empty((rows, heads, capacity), dtype=torch.int32)
     elif kept.shape != (rows, heads, capacity) or kept.dtype is not torch.int32 or kept.device != device or kept.stride(2) != 1:
@@ -74,7 +76,7 @@ def select_tokens(
     with _lib.on_device(device) as stream:
         rc = _lib.load().ekv_select_tokens(
             scores.data_ptr(), stride[0], stride[1], n_slots, capacity, places, length, counts,
-            max(min(count, 0x7FFFFFFF), -1), min(int(first_tokens), capacity), min(int(recent_tokens), capacity), rows, heads,
+            max(min(count, 0x7FFFFFFF), -1), min(first_tokens, capacity), min(recent_tokens, capacity), rows, heads,
             kept.data_ptr(), kept_stride[0], kept_stride[1], new, word, stream,
         )
     _lib.check(rc, "ekv_select_tokens")
@@ -108,6 +110,7 @@ def compact_tokens(
     where the row was moved, ``lens[r]`` where it was left. These are the rows' lengths from here on; only the blocks
     behind them are free.
     """
+    first_tokens = _count("first_tokens", first_tokens)
     if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.stride(4) != 1:
         raise ValueError(f"expected a KV cache [blocks, 2, block, heads, dim] with contiguous heads, got {tuple(kv_cache.shape)}")
     device = kv_cache.device
@@ -145,7 +148,7 @@ def compact_tokens(
         rc = lib.ekv_compact_tokens_lens(
             kv_cache.data_ptr(), s_block * item, s_part * item, s_pos * item, s_head * item, blocks, dim * item,
             table.data_ptr(), table.stride(0), length, rows, width, heads, block_size, kept.data_ptr(), kept_stride[0],
-            kept_stride[1], kept.shape[2], new, min(int(first_tokens), width * block_size), _lib.ptr(scores),
+            kept_stride[1], kept.shape[2], new, min(first_tokens, width * block_size), _lib.ptr(scores),
             score_stride[0], score_stride[1], len(scores) if scores is not None else 0, places, after,
             workspace.data_ptr(), size, word, stream,
         )

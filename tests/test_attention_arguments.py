@@ -191,3 +191,22 @@ def test_compact_tokens_lens_refuses_what_compact_tokens_refuses_and_shared_memo
                        (dict(result=ctypes.c_void_p(0x2000 - 12)), L.EINVAL),  # up to the new lengths' first
                        (dict(result=ctypes.c_void_p(0x1000 + 16), ws_bytes=0), L.ERANGE)]:  # right behind them: the next check
         assert lib.ekv_compact_tokens_lens(*{**args, **over}.values()) == code
+
+
+@pytest.mark.parametrize("wrong", [0.5, 512.0, "3", None])
+def test_counts_have_to_be_whole_numbers(wrong):
+    """A fraction is refused before anything else is looked at: cut to a whole number, a `keep` of one half would keep nothing."""
+    from ekv.runtime.attention import attend
+    from ekv.runtime.eviction import compact_tokens, select_tokens
+
+    scores, lens = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+    cache, table = torch.zeros(9, 2, 16, 2, 128, dtype=torch.bfloat16), torch.zeros(2, 4, dtype=torch.int32)
+    kept = torch.zeros(2, 2, 64, dtype=torch.int32)
+    calls = [lambda: select_tokens(scores, lens, wrong), lambda: select_tokens(scores, lens, 4, first_tokens=wrong),
+             lambda: select_tokens(scores, lens, 4, recent_tokens=wrong),
+             lambda: compact_tokens(cache, table, lens, kept, lens, first_tokens=wrong)]
+    if wrong is not None:  # which means that no prefix is shared
+        calls.append(lambda: attend(torch.zeros(2, 8, 128, dtype=torch.bfloat16), cache, table, lens, 0.1, prefix_blocks=wrong))
+    for call in calls:
+        with pytest.raises(ValueError, match="whole number"):
+            call()

@@ -471,3 +471,23 @@ def test_a_refused_row_goes_on_with_all_of_its_tokens(cuda_lib):
         p = torch.softmax(query[0, 2 * h : 2 * h + 2].double() @ k.T * 0.1, -1)
         # half a step of the output and one of each probability, both relative to 2^-11
         assert torch.all((out[0, 2 * h : 2 * h + 2].double().cpu() - p @ v).abs() <= 2**-11 * ((p @ v).abs() + 1.1 * v.abs().max()) + 1e-4)
+
+
+def test_counts_of_any_whole_number_type(cuda_lib):
+    from ekv.runtime.attention import attend
+    from ekv.runtime.eviction import compact_tokens, select_tokens
+
+    scores = torch.rand(2, 1, 90, generator=torch.Generator().manual_seed(17)).cuda()
+    want = select_tokens(scores, ints([90, 70]), 40, first_tokens=3, recent_tokens=5)
+    for kind in (np.int64, np.uint8, lambda v: torch.tensor(v).numpy(), lambda v: type("Count", (), {"__index__": lambda _: v})()):
+        got = select_tokens(scores, ints([90, 70]), kind(40), first_tokens=kind(3), recent_tokens=kind(5))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for keep in (2**40, -(2**40)):
+        assert select_tokens(scores, ints([90, 70]), keep, first_tokens=2**40)[1].tolist() == [90, 70]
+    cache, _, table = batch(18, [90, 70], heads=1, dim=64)
+    compact_tokens(cache.cuda(), table.cuda(), ints([90, 70]), want[0], want[1], first_tokens=np.int32(3))
+    query = torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(19)).bfloat16().cuda()
+    table[1] = table[0].clone()
+    dev = torch.randn(cache.shape, generator=torch.Generator().manual_seed(20)).bfloat16().cuda()
+    out = [attend(query, dev, table.cuda(), ints([90, 90]), 0.1, prefix_blocks=n)[0] for n in (6, np.int64(6), 2**31, 2**32, 2**40)]
+    assert all(torch.equal(out[0], o) for o in out)
