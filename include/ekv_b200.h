@@ -483,7 +483,8 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  *
  * groups > 0: the rows [group_start[g], group_start[g + 1]) (int32 [groups + 1]; NULL with groups = 1: every row)
  * share their first prefix_blocks[g] blocks (int32 [groups]; NULL with groups = 1: prefix_common blocks): their
- * tables list the same ids there, of which the longest row's are read, once for the group.
+ * tables list the same ids there, of which the longest row's are read, once for the group. A row that holds less of them than
+ * the longest reads what it has itself.
  *
  * A table entry outside [0, pool_blocks) is skipped with EKV_STATUS_BAD_BLOCK_ID, a length past the table
  * clamped with EKV_STATUS_LEN_OVER_WIDTH, a row whose query tokens are not tokens of the batch skipped with

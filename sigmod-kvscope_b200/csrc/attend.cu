@@ -723,6 +723,8 @@ __device__ __forceinline__ void running_sum(int32_t* cum, int units, int* scratc
 
 // One CTA: what every row leaves to its group (whole blocks that it has, so that the prefix launch reads no position
 // that no row of the group holds), each group's longest such part and the row it is read from, and both phases' counts.
+// A row that has less than its group's longest part leaves it nothing and reads all of its tokens itself: to the prefix launch
+// the values behind it would have a probability of zero, and zero times another row's NaN is not zero.
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams pp) {
   const AttendParams& p = pp.p;
   extern __shared__ uint8_t s_plan[];
@@ -742,8 +744,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   }
   __syncthreads();
   bool more = false;
-  const int own_tokens = pp.mt_own == kWideRows ? 2 * kTile : kTile;
-  running_sum(pp.cum_own, p.rows, scratch, [&](int r) {
+  for (int r = threadIdx.x; r < p.rows; r += kPlanThreads) {
     const QueryRange q = row_queries(p, r, true);
     const int to = row_tokens(p, r, true);
     int lo = 0, hi = p.groups;  // the last group that starts at or before r
@@ -753,15 +754,24 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     }
     const bool in = r >= starts[lo] && r < starts[lo + 1];
     const int from = in ? min(blocks[lo] << p.block_shift, to >> p.block_shift << p.block_shift) : 0;
-    if (in) atomicMax(lead + lo, (unsigned long long)(uint32_t)from << 32 | (uint32_t)~(uint32_t)r);
+    if (in && q.nq > 0) atomicMax(lead + lo, (unsigned long long)(uint32_t)from << 32 | (uint32_t)~(uint32_t)r);
     p.row_info[r] = make_int4(q.q0, q.nq, from, to);
     p.row_group[r] = in ? lo : -1;
-    for (int i = 0; i < min(q.nq, 8); ++i) p.limits[q.q0 + i] = min(to - q.nq + i + 1, from);
     more |= q.nq > 8;
-    return to > from && q.nq > 0 ? (to - from + own_tokens - 1) / own_tokens * p.heads * ((q.nq * p.G + pp.mt_own - 1) / pp.mt_own)
-                                 : 0;
-  });
+  }
   more = __syncthreads_or(more);
+  const int own_tokens = pp.mt_own == kWideRows ? 2 * kTile : kTile;
+  running_sum(pp.cum_own, p.rows, scratch, [&](int r) {
+    int4 v = p.row_info[r];  // this thread's own entries
+    const int g = p.row_group[r], nq = v.y, to = v.w;
+    if (g >= 0 && v.z < (int)(lead[g] >> 32)) {
+      v.z = 0;
+      p.row_info[r] = v;
+      p.row_group[r] = -1;
+    }
+    for (int i = 0; i < min(nq, 8); ++i) p.limits[v.x + i] = min(to - nq + i + 1, v.z);
+    return to > v.z && nq > 0 ? (to - v.z + own_tokens - 1) / own_tokens * p.heads * ((nq * p.G + pp.mt_own - 1) / pp.mt_own) : 0;
+  });
   // rows of many query tokens: their limits by a warp
   for (int r = threadIdx.x >> 5; r < p.rows && more; r += kPlanThreads / 32) {
     const int4 v = p.row_info[r];

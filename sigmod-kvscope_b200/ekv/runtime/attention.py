@@ -127,9 +127,10 @@ def attend(
 
     ``prefix_blocks`` int32 [groups]: the rows ``group_start[g]`` to ``group_start[g + 1]`` (int32 [groups + 1];
     without it one group of every row) begin with the same ``prefix_blocks[g]`` blocks, which are read once for
-    the group. An int is one group of every row, as an engine's common prefix length gives it.
+    the group. An int is one group of every row, as an engine's common prefix length gives it. A row that does not hold
+    as much of the prefix as the longest of its group reads what it has itself.
 
-    What lies behind a row may hold anything; values at positions that one of a row's query tokens sees and another does
+    What lies behind a row may hold anything, another row's tokens in a shared prefix too; values at positions that one of a row's query tokens sees and another does
     not must be finite.
 
     Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a

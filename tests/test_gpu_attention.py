@@ -578,3 +578,29 @@ def test_scores_in_a_table_too_wide_for_the_logits(cuda_lib):
     want = oat.accumulate(np.full((2, 1, 700), 0.25), [0, 1], [700, 33], [1, 1], w)
     np.testing.assert_allclose(got[..., :700].cpu().numpy(), want, rtol=1e-6, atol=4e-5 * 16)
     assert torch.all(got[..., 700:] == 0.25)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("queries, lens", [([1] * 5, [60, 0, 200, 97, 1]), ([3, 1, 0, 12, 2], [60, 5, 900, 640, 96]),
+                                           ([40] * 5, [90, 20, 700, 130, 96])])
+def test_a_row_shorter_than_its_groups_prefix_sees_nothing_of_the_others(cuda_lib, queries, lens, wide):
+    """Shared blocks whose keys and values are not numbers behind the shorter rows: the longer rows hold them, the others do not."""
+    from ekv.runtime.attention import attend
+
+    x = make(52, lens, queries=queries, q_heads=16, groups=[(0, 5, 6)], width=60)
+    for t in range(61, 96):
+        x["cache"][x["table"][0, t // 16], 1, t % 16] = float("nan") if t % 2 else float("inf")
+        x["cache"][x["table"][0, t // 16], 0, t % 16, 1] = float("nan") if t > 92 else 1.0
+    x = widen(x, 1 << 17) if wide else x
+    d = on_device(x)
+    got = attend(d["query"], d["cache"], d["table"], d["lens"], 0.1, query_start=d["start"], prefix_blocks=6)
+    want, lse, _ = oat.attend(x["query"].float().numpy(), x["cache"].float().numpy(), x["table"].numpy(), x["lens"].numpy(), 0.1,
+                              x["start"].numpy())
+    u = torch.finfo(torch.bfloat16).eps / 2
+    start = x["start"].tolist()
+    for r in [r for r in range(5) if lens[r] <= 61]:
+        a, b = start[r], start[r + 1]
+        o, e = got[0][a:b].double().cpu().numpy(), got[1][a:b].double().cpu().numpy()
+        biggest = 6.0  # no value of these rows is larger
+        np.testing.assert_allclose(e, lse[a:b], rtol=0, atol=3e-5)
+        assert np.all(np.abs(o - want[a:b]) <= 1.05 * u * (np.abs(want[a:b]) + 1.01 * biggest) + 3e-5 * biggest)
