@@ -509,7 +509,9 @@ int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, con
  * w = sum of exp(scale q.k - lse) over the row's query tokens and the head's query heads: its score becomes w
  * when t is among the row's newest fresh[r] tokens (int32 [rows]; NULL: its query tokens), which have none
  * yet, and decay * score + w otherwise (decay in [0, 1]; with 0 the old score is not read). slots[r] < 0 attends
- * without scoring; a slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required.
+ * without scoring; a slot past the table or given to two rows does too, with EKV_STATUS_BAD_SLOT. lse is required. out may be
+ * q's own memory in ekv_attend, and here with up to 16 query rows a KV head on average (and a table whose logits fit 1 GiB);
+ * with more the queries are read again behind the output, and the call is refused.
  * Two or three kernels, no host synchronisation.
  */
 size_t ekv_attend_scored_workspace_bytes(int rows, int tokens, int width, int block_size, int q_heads, int kv_heads,

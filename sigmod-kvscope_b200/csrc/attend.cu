@@ -976,6 +976,20 @@ int64_t kept_logits(int tokens, int rows, int width, int block_size, int q_heads
   return pick_mt(tokens, rows, q_heads / kv_heads, kv_heads, 128, 0) == 16 && n <= (1ll << 28) ? n : 0;
 }
 
+// Whether [tokens][heads][dim] arrays of 2-byte elements share memory, as far as their first bytes and strides tell: apart as a
+// whole, or by columns of a common row or of a common head.
+bool share_memory(const void* a, int64_t a0, int64_t a1, const void* b, int64_t b0, int64_t b1, int tokens, int heads, int dim) {
+  const int64_t from_a = (int64_t)(uintptr_t)a / 2, from_b = (int64_t)(uintptr_t)b / 2;
+  const int64_t row_a = (heads - 1) * a1 + dim, row_b = (heads - 1) * b1 + dim;
+  if (from_a + (tokens - 1) * a0 + row_a <= from_b || from_b + (tokens - 1) * b0 + row_b <= from_a) return false;
+  auto apart = [&](int64_t period, int64_t size_a, int64_t size_b) {
+    const int64_t d = ((from_b - from_a) % period + period) % period;
+    return d >= size_a && period - d >= size_b;
+  };
+  if (a0 == b0 && a0 > 0 && apart(a0, row_a, row_b)) return false;
+  return !(a0 == b0 && a1 == b1 && a1 > 0 && a0 % a1 == 0 && apart(a1, dim, dim));
+}
+
 struct AttendCall {
   AttendParams p;
   Workspace w;
@@ -1032,6 +1046,8 @@ int prepare(AttendCall& c, const void* q, int64_t q_stride_token, int64_t q_stri
   const Workspace& w = c.w = workspace_layout(rows, tokens, groups, q_heads, head_dim, c.mt, logits);
   if (!workspace || workspace_bytes < w.total || ((uintptr_t)workspace & 255))
     return fail(EKV_ERANGE, "the workspace must hold %zu bytes at a 256-byte boundary", w.total);
+  if (scored && logits == 0 && share_memory(q, q_stride_token, q_stride_head, out, out_stride_token, out_stride_head, tokens, q_heads, head_dim))
+    return fail(EKV_EINVAL, "the output must share no memory with the query, which is read again for the weights");
   int rc = current_device(&c.device);
   if (rc != EKV_OK) return rc;
   if ((rc = sm_count(c.device, &c.sms)) != EKV_OK) return rc;

@@ -135,7 +135,8 @@ def attend(
 
     Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a
     token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
-    in the tables, which the kernels skip. The call runs on the current stream of the query's device.
+    in the tables, which the kernels skip. ``out`` may be the query itself. The call runs on the current stream of the
+    query's device.
     """
     whole = prefix_blocks is None or isinstance(prefix_blocks, torch.Tensor)
     common = 0 if whole else _count("prefix_blocks", prefix_blocks)
@@ -217,7 +218,8 @@ def attend_scored(
     themselves plus it. A prompt's last tokens score the whole prompt with ``fresh = lens``. A negative slot attends
     without scoring; slots must otherwise be one row's alone.
 
-    The other arguments, and the ``(out, lse)`` returned, are ``attend``'s.
+    The other arguments, and the ``(out, lse)`` returned, are ``attend``'s; but with more than 16 query rows a KV head
+    (on average) the queries are read again for the weights, and an ``out`` that shares memory with them is refused.
     """
     device, dtype, q_shape, kv_shape, table_shape, q_stride, kv_stride, table_stride = _batch(query, kv_cache, table, lens)
     tokens, q_heads, dim = q_shape

@@ -210,3 +210,21 @@ def test_counts_have_to_be_whole_numbers(wrong):
     for call in calls:
         with pytest.raises(ValueError, match="whole number"):
             call()
+
+
+def test_attend_scored_refuses_an_output_over_queries_that_it_reads_again(lib):
+    """256 query tokens of four heads' groups: 64 query rows a row and KV head. Apart as a whole or by columns is accepted, as far
+    as this machine without a device goes."""
+    at = lambda n: ctypes.c_void_p(0x100000 + n)
+    size = 256 * 1024 * 2
+    shape = dict(tokens=256, rows=4, start=FAKE, q=at(0))
+    for over in (dict(out=at(0)), dict(out=at(256)), dict(out=at(size - 2048)), dict(out=at(2048 - size)),
+                 dict(out=at(2048), os0=2048), dict(qs0=2048, os0=2048, out=at(1024)), dict(qs0=2048, os0=2048, qs1=256, os1=256, out=at(128)),
+                 dict(qs0=0, out=at(512))):
+        assert lib.ekv_attend_scored(*scored_args(**{**shape, **over})) == L.EINVAL and b"share" in lib.ekv_last_error_string(), over
+    for over in (dict(out=at(size)), dict(out=at(-size)), dict(qs0=2048, os0=2048, out=at(2048)),  # a row's other half
+                 dict(qs0=2048, os0=2048, qs1=256, os1=256, out=at(256))):  # a head's other half
+        assert lib.ekv_attend_scored(*scored_args(**{**shape, **over})) != L.EINVAL, over
+    # with one query token a row its logits are kept
+    assert lib.ekv_attend_scored(*scored_args()) != L.EINVAL
+    assert lib.ekv_attend(*attend_args(**{**shape, "out": at(0)})) != L.EINVAL

@@ -604,3 +604,34 @@ def test_a_row_shorter_than_its_groups_prefix_sees_nothing_of_the_others(cuda_li
         biggest = 6.0  # no value of these rows is larger
         np.testing.assert_allclose(e, lse[a:b], rtol=0, atol=3e-5)
         assert np.all(np.abs(o - want[a:b]) <= 1.05 * u * (np.abs(want[a:b]) + 1.01 * biggest) + 3e-5 * biggest)
+
+
+@pytest.mark.parametrize("kind", NAN_KINDS)
+def test_an_output_over_the_query_itself(cuda_lib, kind):
+    from ekv.runtime.attention import attend, attend_scored
+
+    x, more = nan_batch(kind)
+    d = on_device(x)
+    args = (d["cache"], d["table"], d["lens"], 0.1)
+    want = attend(d["query"], *args, query_start=d["start"], **more)
+    query = d["query"].clone()
+    got = attend(query, *args, query_start=d["start"], out=query, **more)
+    assert got[0] is query and torch.equal(query, want[0]) and torch.equal(got[1], want[1])
+    if more:
+        return
+    scores = [torch.zeros(3, 2, x["table"].shape[1] * 16, device="cuda") for _ in range(2)]
+    attend_scored(d["query"], *args, scores[0], query_start=d["start"])
+    query = d["query"].clone()
+    if "many" in kind or "query rows a head" in kind:
+        with pytest.raises(ValueError, match="share no memory"):
+            attend_scored(query, *args, scores[1], query_start=d["start"], out=query)
+        assert torch.equal(query, d["query"]) and not scores[1].any()
+        # the other half of each token's row is memory of its own
+        both = torch.zeros(len(query), 2, *query.shape[1:], dtype=query.dtype, device="cuda")
+        both[:, 0] = query
+        attend_scored(both[:, 0], *args, scores[1], query_start=d["start"], out=both[:, 1])
+        assert torch.equal(both[:, 1], want[0]) and torch.equal(both[:, 0], query)
+    else:
+        attend_scored(query, *args, scores[1], query_start=d["start"], out=query)
+        assert torch.equal(query, want[0])
+    assert torch.equal(scores[0], scores[1])
