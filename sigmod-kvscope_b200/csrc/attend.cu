@@ -705,18 +705,23 @@ struct PlanParams {
   int mt_own, mt_prefix;
 };
 
-// Running sums of n over [0, units) into cum, with every thread; count(u) is unit u's tiles.
+// Running sums of n over [0, units) into cum, with every thread; count(u) is unit u's tiles. Too many to be dealt are none.
 template <typename Count>
-__device__ __forceinline__ void running_sum(int32_t* cum, int units, int* scratch, Count count) {
+__device__ __forceinline__ void running_sum(const AttendParams& p, int32_t* cum, int units, int* scratch, Count count) {
   int carry = 0;
   for (int base = 0; base < units; base += kPlanThreads) {
     const int u = base + threadIdx.x;
     int total = 0;
     const int n = u < units ? count(u) : 0;
-    const int before = block_exclusive_scan<kPlanThreads>(n, scratch, &total);
-    if (u < units) cum[u] = carry + before;
-    carry += total;
+    const int before = tiles_before<kPlanThreads>(n, scratch, &total);
+    if (u < units) cum[u] = add_tiles(carry, before);
+    carry = add_tiles(carry, total);
     __syncthreads();
+  }
+  if (carry == kTooMany) {
+    for (int u = threadIdx.x; u < units; u += kPlanThreads) cum[u] = 0;
+    if (threadIdx.x == 0) set_status(p.status, EKV_STATUS_BAD_QROW);
+    carry = 0;
   }
   if (threadIdx.x == 0) cum[units] = carry;
 }
@@ -761,7 +766,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
   }
   more = __syncthreads_or(more);
   const int own_tokens = pp.mt_own == kWideRows ? 2 * kTile : kTile;
-  running_sum(pp.cum_own, p.rows, scratch, [&](int r) {
+  running_sum(p, pp.cum_own, p.rows, scratch, [&](int r) {
     int4 v = p.row_info[r];  // this thread's own entries
     const int g = p.row_group[r], nq = v.y, to = v.w;
     if (g >= 0 && v.z < (int)(lead[g] >> 32)) {
@@ -778,7 +783,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
     for (int i = 8 + lane; i < v.y; i += 32) p.limits[v.x + i] = min(v.w - v.y + i + 1, v.z);
   }
   const int prefix_tokens = pp.mt_prefix == kWideRows ? 2 * kTile : kTile;
-  running_sum(pp.cum_prefix, p.groups, scratch, [&](int g) {
+  running_sum(p, pp.cum_prefix, p.groups, scratch, [&](int g) {
     const int a = starts[g], b = starts[g + 1];
     const int to = b > a ? (int)(lead[g] >> 32) : 0, row = to > 0 ? (int)~(uint32_t)lead[g] : 0;
     // the query tokens of the rows [a, b), which follow one another

@@ -142,6 +142,38 @@ __device__ __forceinline__ int unit_tiles(const AttendParams& p, const Unit& un,
   return un.template tiles<TOKENS>() * p.heads * un.m_tiles(p, MT);
 }
 
+// Sums of tile counts. The host bounds a launch's tiles below 2^31 by its query tokens, which a query_start or group_start
+// that descends gives to several units at once: such sums stop at kTooMany, and a launch that reaches it has no tiles.
+constexpr int kTooMany = 0x7fffffff;
+__device__ __forceinline__ int add_tiles(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, (uint32_t)kTooMany); }
+
+// The units' tiles before this thread's, and of all of them.
+template <int THREADS>
+__device__ __forceinline__ int tiles_before(int mine, int* scratch, int* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto before = [&](int v) {  // of the lanes below
+    int incl = v;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int n = __shfl_up_sync(kFullMask, incl, off);
+      if (lane >= off) incl = add_tiles(incl, n);
+    }
+    const int below = __shfl_up_sync(kFullMask, incl, 1);
+    return make_int2(lane > 0 ? below : 0, incl);
+  };
+  const int2 in_warp = before(mine);
+  __syncthreads();
+  if (lane == 31) scratch[warp] = in_warp.y;
+  __syncthreads();
+  if (warp == 0) {
+    const int2 warps = before(lane < THREADS / 32 ? scratch[lane] : 0);
+    if (lane < THREADS / 32) scratch[lane] = warps.x;
+    if (lane == THREADS / 32 - 1) scratch[THREADS / 32] = warps.y;
+  }
+  __syncthreads();
+  *total = scratch[THREADS / 32];
+  return add_tiles(scratch[warp], in_warp.x);
+}
+
 // What a CTA is dealt: tiles [begin, end) of W, the first of them in unit `unit`, whose tiles start at `base`.
 struct Deal {
   int begin, end, W, unit, base;
@@ -188,9 +220,14 @@ __device__ __forceinline__ Deal deal(const AttendParams& p, int units, int MT, i
       const int u = base + threadIdx.x;
       mine = u < units ? unit_tiles<TOKENS>(p, unit_at<PREFIX>(p, u, report), MT) : 0;
       int total = 0;
-      before = d.W + block_exclusive_scan<THREADS>(mine, scratch, &total);
-      d.W += total;
+      before = add_tiles(d.W, tiles_before<THREADS>(mine, scratch, &total));
+      d.W = add_tiles(d.W, total);
     }
+  }
+  const bool too_many = d.W == kTooMany;
+  if (too_many) {
+    d.W = before = 0;
+    if (report && threadIdx.x == 0) set_status(p.status, EKV_STATUS_BAD_QROW);
   }
   const int n = sharing_ctas(d.W, gridDim.x);
   if (threadIdx.x == 0) found[0] = found[1] = 0;
@@ -206,7 +243,7 @@ __device__ __forceinline__ Deal deal(const AttendParams& p, int units, int MT, i
     } else if (units > THREADS) {
       mine = u < units ? unit_tiles<TOKENS>(p, unit_at<PREFIX>(p, u, false), MT) : 0;
       int total = 0;
-      before = carry + block_exclusive_scan<THREADS>(mine, scratch, &total);
+      before = too_many ? 0 : carry + tiles_before<THREADS>(mine, scratch, &total);
       carry += total;
     }
     if (u < units && before <= d.begin && d.begin < before + mine) {  // one thread at most

@@ -635,3 +635,35 @@ def test_an_output_over_the_query_itself(cuda_lib, kind):
         attend_scored(query, *args, scores[1], query_start=d["start"], out=query)
         assert torch.equal(query, want[0])
     assert torch.equal(scores[0], scores[1])
+
+
+@pytest.mark.parametrize("grouped", [False, True])
+def test_rows_that_claim_the_same_query_tokens_over_and_over(cuda_lib, grouped):
+    """A query_start that goes up and down gives every second row all 4096 tokens, 2^31 tiles and more in all, which the sizes
+    of a call that ascends cannot reach: nothing is attended to, the status says so, and the next call is as ever."""
+    import ekv._lib as L
+    from ekv.runtime.attention import attend
+
+    rows, tokens, width = 2048, 4096, 4107
+    assert rows // 2 * (tokens * 8 // 16) * (65700 // 64) > 2**31
+    gen = torch.Generator().manual_seed(53)
+    cache = torch.randn(2, 2, 16, 1, 128, generator=gen).bfloat16().cuda()
+    query = torch.randn(tokens, 8, 128, generator=gen).bfloat16().cuda()
+    table = torch.zeros(rows, width, dtype=torch.int32, device="cuda")
+    start = torch.tensor([tokens * (r % 2) for r in range(rows + 1)], dtype=torch.int32, device="cuda")
+    more = dict(prefix_blocks=torch.zeros(1, dtype=torch.int32, device="cuda")) if grouped else {}
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lens = torch.full((rows,), 65700, dtype=torch.int32, device="cuda")
+    out, lse = attend(query, cache, table, lens, 0.1, query_start=start, status=status, **more)
+    assert int(status) == L.STATUS_BAD_QROW
+    assert not out.any() and torch.all(lse == float("-inf"))
+    ascending = torch.arange(0, 2 * rows + 1, 2, dtype=torch.int32, device="cuda")
+    short = torch.full((rows,), 9, dtype=torch.int32, device="cuda")
+    status.zero_()
+    out, lse = attend(query, cache, table, short, 0.1, query_start=ascending, status=status, **more)
+    want = oat.attend(query[:6].float().cpu().numpy(), cache.float().cpu().numpy(), np.zeros((3, 1), dtype=int), np.array([9] * 3), 0.1,
+                      np.array([0, 2, 4, 6]))
+    assert int(status) == 0
+    np.testing.assert_allclose(lse[:6].cpu().numpy(), want[1], rtol=0, atol=3e-5)
+    u = torch.finfo(torch.bfloat16).eps / 2
+    assert np.all(np.abs(out[:6].double().cpu().numpy() - want[0]) <= 1.05 * u * (np.abs(want[0]) + 1.01 * 6) + 3e-5 * 6)
