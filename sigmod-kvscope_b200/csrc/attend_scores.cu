@@ -72,16 +72,13 @@ __global__ void __launch_bounds__(kAddThreads) add_kernel(const __grid_constant_
   const int32_t* ids = p.table + (int64_t)row * p.table_s0;
   for (int pos = 4 * (blockIdx.y * kAddThreads + threadIdx.x); pos < un.to; pos += 4 * gridDim.y * kAddThreads) {
     float w[4] = {0.f, 0.f, 0.f, 0.f};
+    int seen = 0;  // by query tokens whose log-sum-exp is no number
     for (int i = 0; i < un.q.nq; ++i) {
 #pragma unroll 4
       for (int g = 0; g < p.G; ++g) {
         const float lse = lses[(int64_t)i * p.q_heads + g] * kLog2e;
-        if (lse == -INFINITY) continue;  // it saw nothing
-        if (isnan(lse)) {  // what it saw has no weight that is a number; what it did not see (a logit of -inf) takes none
-          for (int e = 0; e < 4; ++e) {
-            const int id = pos + e < un.to - un.q.nq + i + 1 ? ids[(pos + e) >> p.block_shift] : -1;
-            if (id >= 0 && (int64_t)id < p.pool_blocks) w[e] = lse;
-          }
+        if (!(lse > -INFINITY)) {  // it saw nothing, or something that is no number
+          if (lse != -INFINITY) seen = un.to - un.q.nq + i + 1;
           continue;
         }
         const float4 x = *reinterpret_cast<const float4*>(first + ((int64_t)i * p.q_heads + g) * p.logits_s0 + pos);
@@ -90,6 +87,12 @@ __global__ void __launch_bounds__(kAddThreads) add_kernel(const __grid_constant_
         w[2] += exp2_fast(x.z - lse);
         w[3] += exp2_fast(x.w - lse);
       }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (pos + e >= seen) break;
+      const int id = ids[(pos + e) >> p.block_shift];
+      if (id >= 0 && (int64_t)id < p.pool_blocks) w[e] = NAN;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
