@@ -18,6 +18,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "ekv_common.cuh"
 
@@ -26,6 +27,18 @@ namespace ekv {
 constexpr int kTile = 64;          // tokens of a tile
 constexpr int kAttendMaxRows = 2048;
 constexpr int kAttendMaxCtas = 512;
+
+// Two values rounded to the cache's type, in one register.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
 
 struct AttendParams {
   CUtensorMap kmap, vmap;  // the caches as (head dim, KV head, token of the block, block)
@@ -345,38 +358,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-__device__ __forceinline__ float log2_fast(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 constexpr float kLn2 = 0.69314718055994531f;
 
 // ---- host ---------------------------------------------------------------------------------------------------
 
-// What a kernel of one instantiation was last set up for on each device: the attribute and occupancy calls cost
-// microseconds, and only a batch of another number of rows changes the shared memory it asks for.
+// The CTAs of a kernel of one instantiation that an SM holds, by device; 0 until its shared memory, the same for every launch,
+// has been asked for there (the attribute and occupancy calls cost microseconds).
 struct LaunchCache {
   std::mutex lock;
-  size_t smem[kMaxDevices] = {};  // the most shared memory allowed so far
-  size_t asked[kMaxDevices] = {};  // the size `resident` was found for
   int resident[kMaxDevices] = {};
 };
 
 template <typename Kernel>
 int prepare_launch(LaunchCache& cache, Kernel kernel, const char* name, int device, int threads, size_t smem, int* resident) {
   std::lock_guard<std::mutex> hold(cache.lock);
-  if (smem > cache.smem[device]) {
+  if (cache.resident[device] == 0) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
       return check_launch(name);
-    cache.smem[device] = smem;
-  }
-  if (cache.asked[device] != smem) {
     int n = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) return check_launch(name);
     if (n < 1) return fail(EKV_ENOTSUP, "%s does not fit this device", name);
-    cache.asked[device] = smem;
     cache.resident[device] = n;
   }
   *resident = cache.resident[device];

@@ -52,17 +52,6 @@ struct WideTail {
   int scratch[kThreads / 32 + 1], found[2];
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
 // ---- the walk that all warps share ---------------------------------------------------------------------------
 
 // How an item's tiles fall to the two warpgroups: with one subtile of rows the even tiles to the first and the odd ones

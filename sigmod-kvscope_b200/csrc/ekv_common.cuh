@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "ekv_b200.h"
@@ -29,11 +30,14 @@ int current_device(int* device);
 
 // The SMs of a device, asked once.
 inline int sm_count(int device, int* sms) {
-  static int known[kMaxDevices] = {};
-  if (known[device] == 0 &&
-      cudaDeviceGetAttribute(&known[device], cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
-    return check_launch("cudaDeviceGetAttribute");
-  *sms = known[device];
+  static std::atomic<int> known[kMaxDevices] = {};  // calls from several threads find the same number
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+      return check_launch("cudaDeviceGetAttribute");
+    known[device].store(n, std::memory_order_relaxed);
+  }
+  *sms = n;
   return EKV_OK;
 }
 

@@ -20,8 +20,6 @@
 // protected there, which any number of rows may do; a row that fails is left as it was.
 #include <cooperative_groups.h>
 
-#include <mutex>
-
 #include "ekv_common.cuh"
 
 namespace ekv {
