@@ -477,8 +477,8 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  *   query_start  int32 [rows + 1]: row r's query tokens are [query_start[r], query_start[r + 1]); NULL: one token
  *          a row (tokens == rows). Token i of a row's n sees the positions below lens[r] - n + i + 1.
  * out [tokens][q_heads][head_dim] (element strides) receives softmax(scale q K^T) V and lse (may be NULL;
- * float32 [tokens][q_heads]) the natural log of the sum of exp(scale q.k); a query token that sees nothing gets
- * 0 and -inf. Tokens of no row keep what they have. What lies behind a row may hold anything; values at positions
+ * float32 [tokens][q_heads]) the natural log of the sum of exp(scale q.k); a query token that sees nothing, or only scores of
+ * -inf, gets 0 and -inf, one with a NaN or that sees a NaN key gets NaN in both. Tokens of no row keep what they have. What lies behind a row may hold anything; values at positions
  * that one of a row's query tokens sees and another does not must be finite.
  *
  * groups > 0: the rows [group_start[g], group_start[g + 1]) (int32 [groups + 1]; NULL with groups = 1: every row)
@@ -488,7 +488,7 @@ size_t ekv_attend_workspace_bytes(int rows, int tokens, int groups, int q_heads,
  *
  * A table entry outside [0, pool_blocks) is skipped with EKV_STATUS_BAD_BLOCK_ID, a length past the table
  * clamped with EKV_STATUS_LEN_OVER_WIDTH, a row whose query tokens are not tokens of the batch skipped with
- * EKV_STATUS_BAD_QROW. Supported: head_dim 64 and 128, block_size 8, 16, 32 and 64, rows <= 2048, scale > 0, base
+ * EKV_STATUS_BAD_QROW (query_start and group_start ascend; where they do not, rows whose ranges overlap get no defined output). Supported: head_dim 64 and 128, block_size 8, 16, 32 and 64, rows <= 2048, scale > 0, base
  * addresses and strides in whole 16-byte units. One or two kernels (four with groups), no host synchronisation.
  */
 int ekv_attend(const void* q, int64_t q_stride_token, int64_t q_stride_head, const void* kv,

@@ -133,8 +133,9 @@ def attend(
     What lies behind a row may hold anything, another row's tokens in a shared prefix too; values at positions that one of a row's query tokens sees and another does
     not must be finite.
 
-    Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing gets 0 and -inf, a
-    token of no row keeps what the buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
+    Returns ``(out, lse)``, float32 [tokens, q_heads] for ``lse``; a token that sees nothing, or only scores of -inf,
+    gets 0 and -inf, one that is NaN itself or sees a NaN key gets NaN in both, a token of no row keeps what the
+    buffers held. ``status`` (one int32) receives the EKV_STATUS_* bits of faults
     in the tables, which the kernels skip. ``out`` may be the query itself. The call runs on the current stream of the
     query's device.
     """
