@@ -307,19 +307,38 @@ __global__ void __launch_bounds__(kCheckThreads) check_kernel(const __grid_const
     if (threadIdx.x == 0 && p.lens[row] > most) set_status(p.status, EKV_STATUS_LEN_OVER_WIDTH);
     // the blocks that must be the row's own: all that it holds, but for those a moving row's protected tokens fill
     const int blocks = (n + p.block_size - 1) / p.block_size, own = moves ? p.first / p.block_size : 0;
-    for (int b = threadIdx.x; b < blocks; b += kCheckThreads) {
-      const int id = p.table[(int64_t)row * p.table_s0 + b];
+    auto outside = [&](int id) {
       const bool bad = id < 0 || id >= p.pool_blocks;
       if (bad && moves) atomicOr(&s_flags, kRowBlock);
-      if (p.owner == nullptr) {
-        s_ids[b] = id;
-      } else if (!bad) {
+      return bad;
+    };
+    if (p.owner == nullptr) {
+      for (int b = threadIdx.x; b < blocks; b += kCheckThreads) outside(s_ids[b] = p.table[(int64_t)row * p.table_s0 + b]);
+    } else {
+      // eight blocks of a thread at a time, whose ids, and then whose claims, are under way together (four rows of 2112 blocks,
+      // 2048 of them shared: 25.5 us for the call, 27.4 with one block after another)
+      for (int b0 = threadIdx.x; b0 < blocks; b0 += 8 * kCheckThreads) {
+        int id[8];
+        uint32_t other[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int b = b0 + k * kCheckThreads;
+          id[k] = b < blocks ? p.table[(int64_t)row * p.table_s0 + b] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int b = b0 + k * kCheckThreads;
+          other[k] = b >= blocks || outside(id[k]) ? 0u
+                     : b >= own ? atomicCAS(&p.owner[id[k]], 0u, (uint32_t)row + 1) : atomicOr(&p.owner[id[k]], kProtected);
+        }
         // whichever of two comes second sees the other: a second claim is bad for both rows, a claim of what some row
         // protects for the one that claims
-        const uint32_t other = b >= own ? atomicCAS(&p.owner[id], 0u, (uint32_t)row + 1) : atomicOr(&p.owner[id], kProtected);
-        const uint32_t claimed = other & ~kProtected;
-        if (b >= own && other != 0) atomicOr(&p.bad[row], kRowShared);
-        if (claimed != 0) atomicOr(&p.bad[claimed - 1], kRowShared);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t claimed = other[k] & ~kProtected;
+          if (b0 + k * kCheckThreads >= own && other[k] != 0) atomicOr(&p.bad[row], kRowShared);
+          if (claimed != 0) atomicOr(&p.bad[claimed - 1], kRowShared);
+        }
       }
     }
     if (p.owner == nullptr && moves) {
